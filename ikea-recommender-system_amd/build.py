@@ -21,7 +21,11 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "recommenders", "hip")
 LIB = os.path.join(OUT_DIR, "libikea_rec_hip.so")
 OBJ = os.path.join(HERE, "build", "obj")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wno-unused-result"]
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): the compiler forms them from ordinary float code, and
+# some of their forms have returned wrong results on MI355X; every fp32 operation stays scalar (the host pass warns
+# that it does not know the feature, which is harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 LINK = ["-L/opt/rocm/lib", "-lrccl"]
 
 
