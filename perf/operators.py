@@ -19,35 +19,35 @@ _SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 def listed():
     return [
         # a batch of short click sessions, fp32 as the trainers run, every position trained
-        {"name": "delta train, sessions f32", "op": "delta", "B": 1024, "T": 50, "Hk": 2, "Hv": 2, "Dk": 64, "Dv": 64,
+        {"name": "delta train sessions f32", "op": "delta", "B": 1024, "T": 50, "Hk": 2, "Hv": 2, "Dk": 64, "Dv": 64,
          "type": "f32", "ragged": True, "state": False, "train": True},
         # the headline batch in bf16, two value heads on one key head
-        {"name": "delta train, sessions bf16", "op": "delta", "B": 4096, "T": 50, "Hk": 1, "Hv": 2, "Dk": 64, "Dv": 64,
+        {"name": "delta train sessions bf16", "op": "delta", "B": 4096, "T": 50, "Hk": 1, "Hv": 2, "Dk": 64, "Dv": 64,
          "type": "bf16", "ragged": True, "state": False, "train": True},
         # whole customer histories instead of sessions: few long rows, state carried in and out
-        {"name": "delta train, histories bf16", "op": "delta", "B": 4, "T": 4096, "Hk": 4, "Hv": 8, "Dk": 128, "Dv": 128,
+        {"name": "delta train histories bf16", "op": "delta", "B": 4, "T": 4096, "Hk": 4, "Hv": 8, "Dk": 128, "Dv": 128,
          "type": "bf16", "ragged": True, "state": True, "train": True},
         # one long history read in before serving starts
-        {"name": "delta prefill, one history", "op": "delta", "B": 1, "T": 8191, "Hk": 8, "Hv": 8, "Dk": 128, "Dv": 128,
+        {"name": "delta prefill one history", "op": "delta", "B": 1, "T": 8191, "Hk": 8, "Hv": 8, "Dk": 128, "Dv": 128,
          "type": "bf16", "ragged": False, "state": True, "train": False},
         # the next click of one visitor
-        {"name": "delta step, one visitor", "op": "step", "B": 1, "Hk": 2, "Hv": 2, "Dk": 64, "Dv": 64, "type": "f32"},
+        {"name": "delta step one visitor", "op": "step", "B": 1, "Hk": 2, "Hv": 2, "Dk": 64, "Dv": 64, "type": "f32"},
         # the next click of many visitors at once
-        {"name": "delta step, 512 visitors", "op": "step", "B": 512, "Hk": 8, "Hv": 8, "Dk": 128, "Dv": 128, "type": "bf16"},
+        {"name": "delta step 512 visitors", "op": "step", "B": 512, "Hk": 8, "Hv": 8, "Dk": 128, "Dv": 128, "type": "bf16"},
         # the small configuration: 10k items, dim 32, batch 64
-        {"name": "linear ce, 10k items", "op": "ce", "N": 64, "V": 10001, "D": 32, "type": "bf16", "bias": True, "ignored": 0.0},
+        {"name": "linear ce 10k items", "op": "ce", "N": 64, "V": 10001, "D": 32, "type": "bf16", "bias": True, "ignored": 0.0},
         # the headline configuration: 1M items, dim 128, batch 4096
-        {"name": "linear ce, 1M items", "op": "ce", "N": 4096, "V": 1000001, "D": 128, "type": "bf16", "bias": True,
+        {"name": "linear ce 1M items", "op": "ce", "N": 4096, "V": 1000001, "D": 128, "type": "bf16", "bias": True,
          "ignored": 0.0},
         # every position of a padded session batch, the pads ignored, odd sizes
-        {"name": "linear ce, every position", "op": "ce", "N": 13111, "V": 78341, "D": 256, "type": "f16", "bias": False,
+        {"name": "linear ce every position", "op": "ce", "N": 13111, "V": 78341, "D": 256, "type": "f16", "bias": False,
          "ignored": 0.4},
         # the small catalogue scored for one visitor
-        {"name": "q4 scores, 10k items", "op": "q4", "M": 1, "N": 10001, "K": 64, "G": 32, "type": "bf16", "bias": True},
+        {"name": "q4 scores 10k items", "op": "q4", "M": 1, "N": 10001, "K": 64, "G": 32, "type": "bf16", "bias": True},
         # the 1M catalogue scored for one visitor
-        {"name": "q4 scores, 1M items", "op": "q4", "M": 1, "N": 1000001, "K": 128, "G": 32, "type": "f32", "bias": True},
+        {"name": "q4 scores 1M items", "op": "q4", "M": 1, "N": 1000001, "K": 128, "G": 32, "type": "f32", "bias": True},
         # the largest catalogue scored for a few visitors
-        {"name": "q4 scores, 5M items", "op": "q4", "M": 16, "N": 5000001, "K": 256, "G": 64, "type": "bf16", "bias": False},
+        {"name": "q4 scores 5M items", "op": "q4", "M": 16, "N": 5000001, "K": 256, "G": 64, "type": "bf16", "bias": False},
     ]
 
 
