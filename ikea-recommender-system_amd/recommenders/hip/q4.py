@@ -1,0 +1,73 @@
+"""Item scores from a 4-bit item table (csrc/q4.hip): the output layer of a
+served model at a quarter of its bf16 bytes.
+
+    codes, scales = q4_pack(model_W, group=32)          # once
+    scores = q4_scores(h, codes, scales, bias)          # (M, N) fp32, per request
+    top = scores.topk(20)
+
+codes  (N, K / 2) uint8, two codes a byte, the even column in the low half;
+scales (N, K / group) bfloat16; a weight is scales[n, k // group]·(code − 8).
+K is a multiple of `group` (32, 64 or 128) and at most 1024; any number of
+items N and of rows M.  Sums are kept in fp32; x may be fp32 or bf16 and
+enters exactly.  Capturable; no workspace, no host synchronisation.  Weights
+have to be finite.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import call, ptr
+from .operands import TYPES, fail, launch, stride, tensor, whole
+
+GROUPS = (32, 64, 128)
+K_MAX = 1024
+
+
+def _table(K, group):
+    if group not in GROUPS:
+        fail("group", f"{' / '.join(map(str, GROUPS))} is expected, got {group}")
+    if K == 0 or K % group or K > K_MAX:
+        fail("columns", f"a multiple of the group size {group} up to {K_MAX} is expected, got {K}")
+
+
+def q4_pack(W, group=32):
+    """Quantise a (N, K) fp32 or bf16 table: (codes, scales).  Per group the scale is max |w| / 7 rounded to bf16 and a
+    code is round(w / scale) + 8, ties to even, clamped to 0 .. 15."""
+    tensor("W", W, (None, None), (torch.float32, torch.bfloat16))
+    N, K = W.shape
+    _table(K, group)
+    codes = torch.empty(N, K // 2, dtype=torch.uint8, device=W.device)
+    scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=W.device)
+    if N:
+        with launch(W) as st:
+            call("rg_q4_pack", ptr(W), TYPES[W.dtype], stride(W, 0) or K, N, K, group, ptr(codes), ptr(scales), st)
+    return codes, scales
+
+
+def q4_scores(x, codes, scales, bias=None, out=None):
+    """x (M, K) · table (N, K)ᵀ + bias -> (M, N) fp32.  out: written instead of a new tensor; its rows may be strided."""
+    tensor("x", x, (None, None), (torch.float32, torch.bfloat16))
+    M, K = x.shape
+    whole("codes", codes, (None, K // 2), (torch.uint8,), x.device)
+    N = codes.shape[0]
+    whole("scales", scales, (N, None), (torch.bfloat16,), x.device)
+    groups = scales.shape[1]
+    if groups == 0 or K % groups:
+        fail("scales", f"{groups} groups do not divide {K} columns")
+    _table(K, K // groups)
+    for name, t in (("codes", codes), ("scales", scales)):
+        if N and t.data_ptr() % 16:
+            fail(name, "has to start at a multiple of 16 bytes")
+    if bias is not None:
+        whole("bias", bias, (N,), (torch.float32,), x.device)
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.float32, device=x.device)
+    else:
+        tensor("out", out, (M, N), (torch.float32,), x.device)
+        if M > 1 and out.stride(0) < N:
+            fail("out", f"rows overlap: stride {out.stride(0)}, {N} items")
+    if M and N:
+        with launch(x) as st:
+            call("rg_q4_scores", ptr(x), TYPES[x.dtype], stride(x, 0) or K, ptr(codes), ptr(scales), ptr(bias), M, N, K,
+                 K // groups, ptr(out), stride(out, 0) or N, st)
+    return out

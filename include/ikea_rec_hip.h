@@ -611,6 +611,39 @@ int rg_comm_allreduce(void* comm, const void* send, void* recv, int64_t n, int d
 int rg_comm_allgather(void* comm, const void* send, void* recv, int64_t n, int dtype, rg_stream_t stream);
 int rg_comm_reduce_scatter(void* comm, const void* send, void* recv, int64_t n, int dtype, rg_stream_t stream);
 
+/* ---- Gated delta rule (csrc/delta.hip): a linear-attention recurrence beside rg_gru_fwd / rg_gru_bwd.  Per value head
+ * S_t = exp(g_t) S_{t-1} + beta_t k_t (v_t - exp(g_t) S_{t-1}^T k_t)^T, o_t = scale S_t^T q_t, S a Dk x Dv matrix.
+ * q, k (B, T, Hk, Dk), v and d_o (B, T, Hv, Dv) of `type` (0 fp32, 1 bf16), g, beta (B, T, Hv) fp32; Hv a multiple of
+ * Hk; Dk, Dv multiples of 8 up to 128.  strides: HOST array of 18, the (B, T, H) strides in elements of q, k, v, g, beta,
+ * d_o; rows (the last dimension) are contiguous, those of q, k, d_o start at multiples of 16 bytes.  lens (B) int64,
+ * optional: positions at or behind it are not read, do not change the state and get zeros.  Contiguous: o, dv
+ * (B, T, Hv, Dv), dq, dk (B, T, Hk, Dk), dg, dbeta (B, T, Hv), the states (B, Hv, Dk, Dv) fp32.
+ * For the backward pass the forward leaves U (B, Hv, T, Dv) and S0 (rg_delta_chunk_floats values, when T > 64); both
+ * optional otherwise.  dX is of U's size, dS of S0's.  state0, dstate, dstate0 optional (NULL: zero / not wanted).
+ * rg_delta_step: one token, q, k (B, Hk, Dk), v (B, Hv, Dv); state updated in place, its rows state_stride apart. */
+int64_t rg_delta_chunk_floats(int B, int T, int Hv, int Dk, int Dv);
+int rg_delta_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const int64_t* strides,
+                 const int64_t* lens, const float* state0, int type, int B, int T, int Hk, int Hv, int Dk, int Dv,
+                 float scale, void* o, float* state, float* U, float* S0, rg_stream_t stream);
+int rg_delta_bwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const void* d_o,
+                 const int64_t* strides, const int64_t* lens, const float* state0, const float* dstate, const float* U,
+                 const float* S0, int type, int B, int T, int Hk, int Hv, int Dk, int Dv, float scale, float* dX,
+                 float* dS, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* dstate0, rg_stream_t stream);
+int rg_delta_step(const void* q, const void* k, const void* v, const float* g, const float* beta,
+                  const int64_t* strides, int type, int B, int Hk, int Hv, int Dk, int Dv, float scale, float* state,
+                  int64_t state_stride, void* o, rg_stream_t stream);
+
+/* ---- Scores from a 4-bit item table (csrc/q4.hip): beside rg_head_fwd for serving.  Element types of the
+ * operator entry points below: 0 fp32, 1 bf16, 2 fp16.  codes (N, K/2), two a byte, the even column in the low half;
+ * scales (N, K/G) bf16; weight = scale·(code - 8).  G = 32, 64 or 128, K a multiple of G up to 1024; codes and scales
+ * start at multiples of 16 bytes and are contiguous; ldw / ldx / ldy are row strides in elements (wtype, xtype 0 or 1).
+ * rg_q4_pack: scale = bf16(max|w| / 7) of a group, code = clamp(round(w / scale) + 8, 0, 15).
+ * rg_q4_scores: y[m, n] = sum_k x[m, k]·weight[n, k] + bias[n] (bias optional), fp32. */
+int rg_q4_pack(const void* W, int wtype, int64_t ldw, int64_t N, int K, int G, uint8_t* codes, uint16_t* scales,
+               rg_stream_t stream);
+int rg_q4_scores(const void* x, int xtype, int64_t ldx, const uint8_t* codes, const uint16_t* scales,
+                 const float* bias, int M, int64_t N, int K, int G, float* y, int64_t ldy, rg_stream_t stream);
+
 /* items per online-softmax partial block of rg_head_fwd: pmax/psum/parg hold ceil(A/that) x B */
 int rg_partial_block(void);
 int rg_abi_version(void);   /* 2 (changes since 1) */
