@@ -1,0 +1,651 @@
+// Linear cross entropy over a large item vocabulary on half-precision activations, without keeping the logits: beside the
+// fp32 training heads (csrc/head.hip, csrc/head_flash.hip), for any number of rows, ignored rows and widths.
+//     z = h Wᵀ + b,   loss_r = lse(z_r) − z_{r, t_r},   dz = g (softmax(z) − onehot),   dh = dz W,  dW = dzᵀ h,  db = Σ_r dz
+//
+// Two passes of the same shape; each recomputes z tile by tile and feeds it on from registers (8 N V D flops; 6 with the
+// N x V logits kept).  A workgroup holds a block of one matrix ("X") in registers and streams the other ("Y") through
+// LDS in chunks of 64 rows:
+//     S = Y_c Xᵀ (MFMA),   P = f(S) rounded to the inputs' type,   Oᵀ += Y_cᵀ P (MFMA)
+//   forward   X = rows of h, Y = W: f = 2^(z − m) with a running reference m; O = Σ_v 2^(z − m) W_v and the sum of P per
+//             row and split of the vocabulary; joined by k_ce_join, which takes W[t] off in fp32 (a one-hot inside P
+//             would be rounded with it).
+//   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r); O = dW, and Σ_r P = db from the unrounded P.
+// The accumulator of S (16 rows of Y x 16 of X per tile; lane (kg, n) holds rows 4·kg + i of column n) is already the B
+// operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  Biases and −lse enter
+// as S's start value, so they cost no instruction.  Per 32 rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D
+// MFMA flops: with 48 or 64 columns of X a wave, LDS bandwidth stays behind the MFMAs.
+//
+// Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
+// packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
+// P is rounded to bf16 / fp16 for the second product (half a step of the type, once, as its other operand is held); sums
+// of P, lse, O and the gradients are fp32, and each output is rounded once.  fp16 keeps small probabilities out of its
+// subnormals by a power of two: forwards P <= 2^15, backwards g is scaled to [2^13, 2^14] at its largest.
+#include "common.h"
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef short ce_s4 __attribute__((ext_vector_type(4)));
+typedef short ce_s8 __attribute__((ext_vector_type(8)));
+
+#define CE_CH 64           // rows of Y per chunk
+#define CE_PAD 512         // packed rows are allocated in multiples of this
+#define CE_L2E 1.4426950408889634f
+#define CE_LN2 0.6931471805599453f
+#define CE_LOW (-3.0e38f)  // the running reference before any logit
+#define CE_HEAD 8.f        // log2 of the largest P before the reference moves
+
+template <typename T>
+struct CeT;
+template <>
+struct CeT<__bf16> {
+  typedef bf16x8 V;
+  static constexpr float OFF = 0.f;
+  static __device__ __forceinline__ f4 mm(V a, V b, f4 c) { return mfma16bf(a, b, c); }
+};
+template <>
+struct CeT<_Float16> {
+  typedef h16x8 V;
+  static constexpr float OFF = 7.f;
+  static __device__ __forceinline__ f4 mm(V a, V b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+struct CeArgs {
+  const void *X, *Y;
+  int64_t ldx, ldy;        // row strides in elements
+  int nx, ny;              // rows (host bounds)
+  int D;                   // columns of W's rows (h's packed copy has DP, zeros behind D)
+  const int* count;        // packed rows
+  const float* bias;       // (V) or null
+  const float* recs;       // backward: [chunk][3][64] −lse, g, target (as int bits)
+  int nsplit, nblock;
+  float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][V][D], pl slabs [split][V]
+  void* dW;
+  float* db;
+  const float* scale;      // backward: {factor on g, its inverse}; null: 1
+};
+
+// 16-byte chunk c of row r sits at place c ^ swz(r): 16 rows' reads of one column spread over all banks
+template <int DP>
+__device__ __forceinline__ int ce_swz(int r) {
+  return DP == 64 ? (r >> 1) & 7 : r & 15;
+}
+
+// FWD: forward pass (else backward); GRAD: with the second product
+template <typename T, int DP, int NX, int NW, bool FWD, bool GRAD>
+__global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
+  typedef typename CeT<T>::V V;
+  constexpr int KS = DP / 32, RB = DP * 2, FB = GRAD ? DP / 16 : 1;
+  constexpr int LOADS = CE_CH * RB / (NW * 1024);
+  static_assert(LOADS >= 1, "a chunk is at least one load a wave");
+  __shared__ __attribute__((aligned(16))) uint8_t y0[CE_CH * RB], y1[CE_CH * RB];
+  __shared__ __attribute__((aligned(16))) float r0[3 * CE_CH], r1[3 * CE_CH];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // neighbouring blocks of one split run on one XCD (workgroups go round the 8 XCDs) and share its L2
+  int split, block;
+  if (a.nsplit % 8 == 0) {
+    const int k = blockIdx.x >> 3;
+    split = (blockIdx.x & 7) + 8 * (k / a.nblock);
+    block = k % a.nblock;
+  } else {
+    split = blockIdx.x / a.nblock;
+    block = blockIdx.x % a.nblock;
+  }
+  const int rows = *a.count;
+  const int nx = FWD ? rows : a.nx, ny = FWD ? a.ny : rows;
+  const int x0 = block * 16 * NX * NW + wave * 16 * NX;
+  if (FWD && block * 16 * NX * NW >= nx) return;
+  const int nch = (ny + CE_CH - 1) / CE_CH;
+  const int c0 = (int)((int64_t)nch * split / a.nsplit), c1 = (int)((int64_t)nch * (split + 1) / a.nsplit);
+
+  const T* Y = (const T*)a.Y;
+  const int ycols = FWD ? a.D : DP;
+  auto issue = [&](int c, uint8_t* y, float* r) __attribute__((always_inline)) {
+    const int64_t at = (int64_t)c * CE_CH;
+    const int64_t left = ny - at;   // rows
+    const int64_t bytes = left <= 0 ? 0 : ((left < CE_CH ? left : CE_CH) - 1) * a.ldy * 2 + ycols * 2;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(Y) + at * a.ldy, 0, (int)bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int e = (i * NW + wave) * 64 + lane, row = e / (RB / 16), p = e % (RB / 16);
+      const int col = (p ^ ce_swz<DP>(row)) * 8;
+      const int off = col < ycols ? (int)(row * a.ldy + col) * 2 : 0x7ffffff0;
+      rg_blds16(rs, y + (i * NW + wave) * 1024, off, 0);
+    }
+    if (wave == 0) {
+      if constexpr (FWD) {   // 64 biases
+        const int nb = a.bias != nullptr ? (int)(left < CE_CH ? left : CE_CH) * 4 : 0;
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.bias) + (a.bias ? at : 0), 0,
+                                                          nb < 0 ? 0 : nb, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)r, 4, lane * 4, 0, 0, 0);
+      } else {
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.recs) + at * 3, 0,
+                                                          left > 0 ? 3 * CE_CH * 4 : 0, 0x00020000);
+        if (lane < 48) rg_blds16(rb, r, 16 * lane, 0);
+      }
+    }
+  };
+  if (c0 < c1) issue(c0, y0, r0);
+
+  V xf[NX][KS];
+  float ref[NX], top[NX], sum[NX], xb[NX];
+  const T* X = (const T*)a.X;
+  const int xcols = FWD ? DP : a.D;
+#pragma unroll
+  for (int t = 0; t < NX; ++t) {
+    const int64_t x = x0 + 16 * t + n;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int col = 32 * s + 8 * kg;
+      xf[t][s] = x < nx && col < xcols ? *reinterpret_cast<const V*>(X + x * a.ldx + col) : (V)(T)0.f;
+    }
+    ref[t] = CE_LOW;
+    top[t] = CE_LOW;   // reference + head room, natural units
+    sum[t] = 0.f;
+    xb[t] = !FWD && a.bias != nullptr && x < nx ? a.bias[x] * CE_L2E : 0.f;
+  }
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+  f4 O[FB][NX];
+#pragma unroll
+  for (int f = 0; f < FB; ++f)
+#pragma unroll
+    for (int t = 0; t < NX; ++t) O[f][t] = zero;
+
+  auto work = [&](int c, uint8_t* y, const float* r) __attribute__((always_inline)) {
+    bool mine = false;   // backward: a target of this chunk among this wave's items
+    if constexpr (!FWD) {
+      const int t = __float_as_int(r[2 * CE_CH + lane]) - x0;
+      mine = __any(t >= 0 && t < 16 * NX);
+    }
+    const bool tail = FWD && c * CE_CH + CE_CH > ny;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f4 S[2][NX];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 32 * h + 16 * j + n;
+        const f4 start = *reinterpret_cast<const f4*>(r + 32 * h + 16 * j + 4 * kg);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const V f = *reinterpret_cast<const V*>(y + row * RB + (((4 * s + kg) ^ ce_swz<DP>(row)) << 4));
+#pragma unroll
+          for (int t = 0; t < NX; ++t) S[j][t] = CeT<T>::mm(f, xf[t][s], s == 0 ? start : S[j][t]);
+        }
+      }
+      V P[NX];
+      if constexpr (FWD) {
+        if (tail) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c * CE_CH + 32 * h + 16 * j + 4 * kg + i >= ny)
+#pragma unroll
+                for (int t = 0; t < NX; ++t) S[j][t][i] = -__builtin_inff();
+        }
+        float cm[NX];
+        bool up = false;
+#pragma unroll
+        for (int t = 0; t < NX; ++t) {
+          cm[t] = fmaxf(fmaxf(fmaxf(S[0][t][0], S[0][t][1]), fmaxf(S[0][t][2], S[0][t][3])),
+                        fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
+          up |= cm[t] > top[t];
+        }
+        if (__any(up)) {   // rare after the first chunks: the reference moves, what was summed follows
+#pragma unroll
+          for (int t = 0; t < NX; ++t) {
+            float m = fmaxf(cm[t], __shfl_xor(cm[t], 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float now = fmaxf(ref[t], m * CE_L2E), fac = __builtin_amdgcn_exp2f(ref[t] - now);
+            ref[t] = now;
+            top[t] = (now + CE_HEAD) * CE_LN2;
+            sum[t] *= fac;
+#pragma unroll
+            for (int f = 0; f < FB; ++f) O[f][t] *= fac;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NX; ++t) {
+          const float b = CeT<T>::OFF - ref[t];
+          float p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
+            sum[t] += p[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[i];
+        }
+      } else {
+        f4 g[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) g[j] = *reinterpret_cast<const f4*>(r + CE_CH + 32 * h + 16 * j + 4 * kg);
+#pragma unroll
+        for (int t = 0; t < NX; ++t) {
+          float p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, xb[t])) * g[i >> 2][i & 3];
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int tg = __float_as_int(r[2 * CE_CH + 32 * h + 16 * (i >> 2) + 4 * kg + (i & 3)]);
+              if (tg == x0 + 16 * t + n) p[i] -= g[i >> 2][i & 3];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[t] += p[i];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[i];
+        }
+      }
+      if constexpr (GRAD) {
+        const int row = 32 * h + 4 * kg + (n >> 2);
+#pragma unroll
+        for (int f = 0; f < FB; ++f) {
+          const int ch = 2 * f + ((n >> 1) & 1), half = 8 * (n & 1);
+          uint8_t* p0 = y + row * RB + ((ch ^ ce_swz<DP>(row)) << 4) + half;
+          uint8_t* p1 = y + (row + 16) * RB + ((ch ^ ce_swz<DP>(row + 16)) << 4) + half;
+          const ce_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ce_s4*)p0);
+          const ce_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ce_s4*)p1);
+          const ce_s8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int t = 0; t < NX; ++t) O[f][t] = CeT<T>::mm(__builtin_bit_cast(V, v), P[t], O[f][t]);
+        }
+      }
+    }
+  };
+  __syncthreads();
+  for (int c = c0; c < c1; c += 2) {
+    if (c + 1 < c1) issue(c + 1, y1, r1);
+    __builtin_amdgcn_sched_barrier(0);
+    work(c, y0, r0);
+    __syncthreads();
+    if (c + 1 < c1) {
+      if (c + 2 < c1) issue(c + 2, y0, r0);
+      __builtin_amdgcn_sched_barrier(0);
+      work(c + 1, y1, r1);
+      __syncthreads();
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < NX; ++t) {
+    sum[t] += __shfl_xor(sum[t], 16);
+    sum[t] += __shfl_xor(sum[t], 32);
+    const int64_t x = x0 + 16 * t + n;
+    if (x >= nx) continue;
+    if constexpr (FWD) {
+      const int64_t at = (int64_t)split * a.nx + x;
+      if (kg == 0) {
+        a.pm[at] = ref[t];
+        a.pl[at] = sum[t];
+      }
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int f = 0; f < FB; ++f) *reinterpret_cast<f4*>(a.pO + at * DP + 16 * f + 4 * kg) = O[f][t];
+      }
+    } else {
+      const float back = a.scale != nullptr ? a.scale[1] : 1.f;
+      if (a.nsplit > 1) {
+        const int64_t at = (int64_t)split * a.nx + x;
+        if (a.db != nullptr && kg == 0) a.pl[at] = sum[t] * back;
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+          if (16 * f + 4 * kg < a.D) *reinterpret_cast<f4*>(a.pO + at * a.D + 16 * f + 4 * kg) = O[f][t] * back;
+      } else {
+        if (a.db != nullptr && kg == 0) a.db[x] = sum[t] * back;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+          if (16 * f + 4 * kg < a.D)
+            *reinterpret_cast<T4*>((T*)a.dW + x * a.D + 16 * f + 4 * kg) =
+                __builtin_convertvector(O[f][t] * back, T4);
+      }
+    }
+  }
+}
+
+// Rows with a target >= 0, in order: tc (their targets, −1 for one that is no item), rows (their places), inv (the way
+// back, −1: ignored), count; the losses of ignored rows.  One workgroup, a run of rows per thread.
+__global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ tgt, int64_t st, int N, int npad, int V,
+                                                  int* __restrict__ count, int* __restrict__ rows,
+                                                  int* __restrict__ tc, int* __restrict__ inv,
+                                                  float* __restrict__ loss) {
+  __shared__ int part[16];
+  const int tid = threadIdx.x, per = (N + 1023) / 1024, lo = min(N, tid * per), hi = min(N, lo + per);
+  int k = 0;
+  for (int r = lo; r < hi; ++r) k += tgt[r * st] >= 0;
+  int up = k;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(up, o);
+    if ((tid & 63) >= o) up += x;
+  }
+  if ((tid & 63) == 63) part[tid >> 6] = up;
+  __syncthreads();
+  int all = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < (tid >> 6)) up += part[w];
+    all += part[w];
+  }
+  int at = up - k;
+  for (int r = lo; r < hi; ++r) {
+    const int64_t t = tgt[r * st];
+    if (t >= 0) {
+      rows[at] = r;
+      tc[at] = t < V ? (int)t : -1;
+      inv[r] = at++;
+    } else {
+      inv[r] = -1;
+      loss[r] = 0.f;
+    }
+  }
+  if (tid == 0) *count = all;
+  for (int c = all + tid; c < npad; c += 1024) rows[c] = -1;
+}
+
+// packed copy of the listed rows, zeros behind column D and behind the last row
+__global__ __launch_bounds__(256) void k_ce_pack(const uint16_t* __restrict__ h, int64_t ldh, int D, int DP, int npad,
+                                                 const int* __restrict__ rows, uint16_t* __restrict__ hp) {
+  const int e = blockIdx.x * 256 + threadIdx.x, c = e / (DP / 8), col = (e % (DP / 8)) * 8;
+  if (c >= npad) return;
+  const int r = rows[c];
+  ce_s8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (r >= 0 && col < D) v = *reinterpret_cast<const ce_s8*>(h + r * ldh + col);
+  *reinterpret_cast<ce_s8*>(hp + (int64_t)c * DP + col) = v;
+}
+
+// one wave per packed row: lse over the splits, the loss, and (GRAD) dh for g = 1 in fp32
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, const float* __restrict__ pl,
+                                                 const float* __restrict__ pO, int nsplit, int N, int D, int DP,
+                                                 const T* __restrict__ hp, const T* __restrict__ W, int64_t ldw,
+                                                 const float* __restrict__ bias, const int* __restrict__ count,
+                                                 const int* __restrict__ rows, const int* __restrict__ tc,
+                                                 float* __restrict__ loss, float* __restrict__ lse,
+                                                 float* __restrict__ dh) {
+  const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c >= *count) return;
+  float m = CE_LOW;
+  for (int s = lane; s < nsplit; s += 64) m = fmaxf(m, pm[(int64_t)s * N + c]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float l = 0.f;
+  for (int s = lane; s < nsplit; s += 64)
+    l += pl[(int64_t)s * N + c] * __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  const int t = tc[c];
+  const T* w = W + (int64_t)(t < 0 ? 0 : t) * ldw;
+  float z = 0.f;
+  for (int f = lane; f < D; f += 64) z = __builtin_fmaf((float)hp[(int64_t)c * DP + f], (float)w[f], z);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) z += __shfl_xor(z, o);
+  // a target that is no item: NaN in the loss and, through lse, in the gradients
+  const float all = t < 0 ? __builtin_nanf("") : CE_LN2 * (m - CeT<T>::OFF + __log2f(l));
+  if (lane == 0) {
+    loss[rows[c]] = all - (z + (bias != nullptr && t >= 0 ? bias[t] : 0.f));
+    lse[c] = all;
+  }
+  if constexpr (GRAD) {
+    const float one = 1.f / l;
+    for (int f = lane; f < D; f += 64) {
+      float o = 0.f;
+      for (int s = 0; s < nsplit; ++s)
+        o = __builtin_fmaf(pO[((int64_t)s * N + c) * DP + f], __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m), o);
+      dh[(int64_t)c * D + f] = t < 0 ? __builtin_nanf("") : __builtin_fmaf(o, one, -(float)w[f]);
+    }
+  }
+}
+
+// fp16: the power of two that brings the largest |g| of the listed rows to [2^13, 2^14), and its inverse
+__global__ __launch_bounds__(1024) void k_ce_scale(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
+                                                   int N, float* __restrict__ scale) {
+  __shared__ float part[16];
+  float m = 0.f;
+  for (int r = threadIdx.x; r < N; r += 1024)
+    if (inv[r] >= 0) m = fmaxf(m, fabsf(g[r * sg]));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, part[w]);
+    int e = 0;
+    if (m > 0.f && m < __builtin_inff()) (void)frexpf(m, &e);   // m in [2^(e−1), 2^e)
+    e = min(max(14 - e, -120), 120);
+    scale[0] = ldexpf(1.f, e);
+    scale[1] = ldexpf(1.f, -e);
+  }
+}
+
+// dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
+                                               const int* __restrict__ count, const int* __restrict__ tc,
+                                               const float* __restrict__ lse, const float* __restrict__ dh0, int N,
+                                               int npad, int D, const float* __restrict__ scale, T* __restrict__ dh,
+                                               float* __restrict__ recs) {
+  const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= npad) return;
+  if (lane == 0 && r >= *count) {   // behind the last packed row
+    float* rec = recs + (int64_t)(r / CE_CH) * 3 * CE_CH + r % CE_CH;
+    rec[0] = -__builtin_inff();
+    rec[CE_CH] = 0.f;
+    rec[2 * CE_CH] = __int_as_float(-1);
+  }
+  if (r >= N) return;
+  const int c = inv[r];
+  const float gr = c >= 0 ? g[r * sg] : 0.f;
+  for (int f = lane * 4; f < D; f += 256) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const f4 v = c >= 0 ? *reinterpret_cast<const f4*>(dh0 + (int64_t)c * D + f) * gr : (f4){0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<T4*>(dh + (int64_t)r * D + f) = __builtin_convertvector(v, T4);
+  }
+  if (lane == 0 && c >= 0) {
+    float* rec = recs + (int64_t)(c / CE_CH) * 3 * CE_CH + c % CE_CH;
+    rec[0] = -lse[c];
+    rec[CE_CH] = scale != nullptr ? gr * scale[0] : gr;
+    rec[2 * CE_CH] = __int_as_float(tc[c]);
+  }
+}
+
+// backward slabs added up in a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_slabs(const float* __restrict__ pO, const float* __restrict__ pl,
+                                                  int nsplit, int V, int D, T* __restrict__ dW, float* __restrict__ db) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const int64_t n = (int64_t)V * D / 4, step = (int64_t)gridDim.x * 256;
+  const f4* p = reinterpret_cast<const f4*>(pO);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    f4 x = p[i];
+    for (int s = 1; s < nsplit; ++s) x += p[s * n + i];
+    reinterpret_cast<T4*>(dW)[i] = __builtin_convertvector(x, T4);
+  }
+  if (db != nullptr)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < V; i += step) {
+      float x = pl[i];
+      for (int s = 1; s < nsplit; ++s) x += pl[(int64_t)s * V + i];
+      db[i] = x;
+    }
+}
+
+// ------------------------------------------------------------------ host ----
+static int ce_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+// columns of X a workgroup holds (waves x 16 x tiles): 8 waves, two on a SIMD, so that one's exponentials run beside the
+// other's MFMAs; tiles as registers allow (O takes DP / 4 of them per tile)
+static int ce_nx(int DP) { return DP == 64 ? 4 : DP == 128 ? 3 : 2; }
+#define CE_NW 8
+
+// splits of the streamed axis: fewest rounds of 256 workgroups times a split's chunks (and about 8 chunks' worth of
+// start and end); `most` bounds the partial results
+static int ce_splits(int64_t nblock, int64_t nch, int64_t most) {
+  if (most > nch) most = nch;
+  int best = 1;
+  double cost = 1e30;
+  for (int64_t s = 1; s <= most && s <= 512; ++s) {
+    if (s > 8 && s % 8) continue;
+    const double c = (double)((nblock * s + 255) / 256) * ((nch + s - 1) / s + 8);
+    if (c < cost * 0.999) cost = c, best = (int)s;
+  }
+  return best;
+}
+
+struct CePlan {
+  int DP, xw, npad, fblocks, fsplits, bblocks, bsplits;
+};
+static CePlan ce_plan(int N, int V, int D) {
+  CePlan p;
+  p.DP = ce_dp(D);
+  p.xw = 16 * CE_NW * ce_nx(p.DP);
+  p.npad = (int)ce_up(N, CE_PAD);
+  p.fblocks = (N + p.xw - 1) / p.xw;
+  // partial results: at most 2^28 values
+  p.fsplits = ce_splits(p.fblocks, (V + CE_CH - 1) / CE_CH, ((int64_t)1 << 28) / ((int64_t)p.npad * p.DP) + 1);
+  p.bblocks = (V + p.xw - 1) / p.xw;
+  p.bsplits = p.bblocks >= 2048 ? 1 : ce_splits(p.bblocks, (N + CE_CH - 1) / CE_CH, ((int64_t)1 << 28) / ((int64_t)V * D) + 1);
+  return p;
+}
+
+static int ce_check(int64_t N, int64_t V, int D, int type) {
+  if (type != 1 && type != 2) return RG_ERR_ARG;
+  if (N <= 0 || N > (1 << 24) || V <= 0 || V > 0x7ffffff0 - 4096 || D <= 0 || D % 8 || D > 256) return RG_ERR_SHAPE;
+  return RG_OK;
+}
+
+// forward scratch (floats): pm, pl, pO; backward: scale, recs, pO slabs, pl slabs
+extern "C" int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass) {
+  if (ce_check(N, V, D, 1) != RG_OK) return 0;
+  const CePlan p = ce_plan(N, V, D);
+  if (pass == 0) return 2 * (int64_t)p.fsplits * N + 64;
+  if (pass == 1) return 2 * (int64_t)p.fsplits * N + 64 + (int64_t)p.fsplits * N * p.DP;
+  return 64 + 3 * (int64_t)p.npad + (p.bsplits > 1 ? (int64_t)p.bsplits * V * (D + 1) + 64 : 0);
+}
+// what the backward pass needs of the forward (bytes): packed h, lists, lse, dh for g = 1
+extern "C" int64_t rg_linear_ce_saved_bytes(int N, int V, int D) {
+  if (ce_check(N, V, D, 1) != RG_OK) return 0;
+  const int64_t npad = ce_up(N, CE_PAD);
+  return 256 + npad * (ce_dp(D) * 2 + 4 * 4) + (int64_t)N * D * 4;
+}
+struct CeSaved {
+  void* hp;
+  int *count, *rows, *tc, *inv;
+  float *lse, *dh0;
+};
+static CeSaved ce_saved(void* base, int N, int D) {
+  const int64_t npad = ce_up(N, CE_PAD);
+  CeSaved s;
+  uint8_t* p = (uint8_t*)base;
+  s.count = (int*)p;
+  p += 256;
+  s.hp = p;
+  p += npad * ce_dp(D) * 2;
+  s.rows = (int*)p;
+  s.tc = s.rows + npad;
+  s.inv = s.tc + npad;
+  s.lse = (float*)(s.inv + npad);
+  s.dh0 = s.lse + npad;
+  return s;
+}
+
+template <typename T, int DP, int NX, bool FWD, bool GRAD>
+static int ce_pass(const CeArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((k_ce_pass<T, DP, NX, CE_NW, FWD, GRAD>), dim3(a.nblock * a.nsplit), dim3(64 * CE_NW), 0, st, a);
+  RG_LAUNCH_CHECK();
+  return RG_OK;
+}
+template <typename T, bool FWD, bool GRAD>
+static int ce_pass(int DP, const CeArgs& a, hipStream_t st) {
+  return DP == 64    ? ce_pass<T, 64, 4, FWD, GRAD>(a, st)
+         : DP == 128 ? ce_pass<T, 128, 3, FWD, GRAD>(a, st)
+                     : ce_pass<T, 256, 2, FWD, GRAD>(a, st);
+}
+
+template <typename T>
+static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, const int64_t* tgt,
+                  int64_t st_t, int N, int V, int D, bool grad, float* work, void* saved, float* loss, hipStream_t st) {
+  const CePlan p = ce_plan(N, V, D);
+  const CeSaved s = ce_saved(saved, N, D);
+  hipLaunchKernelGGL(k_ce_rows, dim3(1), dim3(1024), 0, st, tgt, st_t, N, p.npad, V, s.count, s.rows, s.tc, s.inv, loss);
+  hipLaunchKernelGGL(k_ce_pack, dim3((p.npad * (p.DP / 8) + 255) / 256), dim3(256), 0, st, (const uint16_t*)h, ldh, D,
+                     p.DP, p.npad, s.rows, (uint16_t*)s.hp);
+  RG_LAUNCH_CHECK();
+  CeArgs a = {};
+  a.X = s.hp, a.ldx = p.DP, a.nx = N, a.Y = W, a.ldy = ldw, a.ny = V, a.D = D, a.count = s.count, a.bias = bias;
+  a.nsplit = p.fsplits, a.nblock = p.fblocks;
+  a.pm = work, a.pl = work + (int64_t)p.fsplits * N;
+  a.pO = work + ce_up(2 * (int64_t)p.fsplits * N, 64);
+  const int rc = grad ? ce_pass<T, true, true>(p.DP, a, st) : ce_pass<T, true, false>(p.DP, a, st);
+  if (rc != RG_OK) return rc;
+  auto join = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((N + 3) / 4), dim3(256), 0, st, a.pm, a.pl, a.pO, p.fsplits, N, D, p.DP,
+                       (const T*)s.hp, (const T*)W, ldw, bias, s.count, s.rows, s.tc, loss, s.lse, s.dh0);
+  };
+  if (grad)
+    join(k_ce_join<T, true>);
+  else
+    join(k_ce_join<T, false>);
+  RG_LAUNCH_CHECK();
+  return RG_OK;
+}
+
+template <typename T>
+static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g, int64_t sg, int N, int V, int D,
+                  const void* saved, float* work, void* dh, void* dW, float* db, hipStream_t st) {
+  const CePlan p = ce_plan(N, V, D);
+  const CeSaved s = ce_saved(const_cast<void*>(saved), N, D);
+  float *scale = nullptr, *recs = work + 64;
+  if (CeT<T>::OFF != 0.f) {
+    scale = work;
+    hipLaunchKernelGGL(k_ce_scale, dim3(1), dim3(1024), 0, st, g, sg, s.inv, N, scale);
+  }
+  hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.dh0, N,
+                     p.npad, D, scale, (T*)dh, recs);
+  RG_LAUNCH_CHECK();
+  CeArgs a = {};
+  a.X = W, a.ldx = ldw, a.nx = V, a.Y = s.hp, a.ldy = p.DP, a.ny = N, a.D = D, a.count = s.count, a.bias = bias;
+  a.recs = recs, a.nsplit = p.bsplits, a.nblock = p.bblocks, a.dW = dW, a.db = db, a.scale = scale;
+  a.pO = recs + 3 * (int64_t)p.npad, a.pl = a.pO + ce_up((int64_t)p.bsplits * V * D, 64);
+  const int rc = ce_pass<T, false, true>(p.DP, a, st);
+  if (rc != RG_OK) return rc;
+  if (p.bsplits > 1) {
+    const int64_t blocks = ((int64_t)V * D / 4 + 255) / 256;
+    hipLaunchKernelGGL(k_ce_slabs<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, a.pO, a.pl,
+                       p.bsplits, V, D, (T*)dW, db);
+    RG_LAUNCH_CHECK();
+  }
+  return RG_OK;
+}
+
+// 16-byte rows; a chunk's 64 rows have to stay within a buffer's 2 GB
+static bool ce_rows_ok(const void* p, int64_t ld, int D) {
+  return p != nullptr && ((uintptr_t)p & 15) == 0 && ld >= D && ld % 8 == 0 && ld < ((int64_t)1 << 23);
+}
+
+extern "C" int rg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias,
+                                const int64_t* target, int64_t target_stride, int type, int N, int V, int D, int grad,
+                                float* work, void* saved, float* loss, hipStream_t stream) {
+  const int rc = ce_check(N, V, D, type);
+  if (rc != RG_OK) return rc;
+  if (!ce_rows_ok(h, ldh, D) || !ce_rows_ok(W, ldw, D) || target == nullptr || work == nullptr || saved == nullptr ||
+      loss == nullptr || (((uintptr_t)work | (uintptr_t)saved) & 15))
+    return RG_ERR_ARG;
+  return type == 1 ? ce_fwd<__bf16>(h, ldh, W, ldw, bias, target, target_stride, N, V, D, grad != 0, work, saved, loss, stream)
+                   : ce_fwd<_Float16>(h, ldh, W, ldw, bias, target, target_stride, N, V, D, grad != 0, work, saved, loss, stream);
+}
+
+extern "C" int rg_linear_ce_bwd(const void* W, int64_t ldw, const float* bias, const float* dloss, int64_t dloss_stride,
+                                int type, int N, int V, int D, const void* saved, float* work, void* dh, void* dW,
+                                float* db, hipStream_t stream) {
+  const int rc = ce_check(N, V, D, type);
+  if (rc != RG_OK) return rc;
+  if (!ce_rows_ok(W, ldw, D) || dloss == nullptr || saved == nullptr || work == nullptr || dh == nullptr ||
+      dW == nullptr || (((uintptr_t)work | (uintptr_t)saved | (uintptr_t)dh | (uintptr_t)dW) & 15) ||
+      (db != nullptr && bias == nullptr))
+    return RG_ERR_ARG;
+  return type == 1 ? ce_bwd<__bf16>(W, ldw, bias, dloss, dloss_stride, N, V, D, saved, work, dh, dW, db, stream)
+                   : ce_bwd<_Float16>(W, ldw, bias, dloss, dloss_stride, N, V, D, saved, work, dh, dW, db, stream);
+}

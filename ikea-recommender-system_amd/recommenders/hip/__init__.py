@@ -25,7 +25,8 @@ U64 = C.c_uint64
 # entry points returning int64_t (all others return int)
 RESTYPE_I64 = {"rg_sampled_work_bytes", "rg_head_work_bytes", "rg_head_plane_bytes", "rg_gru_wide_work_bytes",
                "rg_scatter_rows_work_bytes", "rg_flash_dw_work_bytes", "rg_shard_dedup_work_bytes",
-               "rg_flash_topk_work_bytes", "rg_flash_zs_bytes", "rg_delta_chunk_floats"}
+               "rg_flash_topk_work_bytes", "rg_flash_zs_bytes", "rg_delta_chunk_floats",
+               "rg_linear_ce_work_floats", "rg_linear_ce_saved_bytes"}
 
 # name -> argtypes
 SIGNATURES = {
@@ -152,6 +153,10 @@ SIGNATURES = {
     "rg_delta_fwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P],
     "rg_delta_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P, P],
     "rg_delta_step": [P, P, P, P, P, P, I, I, I, I, I, I, F, P, I64, P, P],
+    "rg_linear_ce_work_floats": [I, I, I, I],
+    "rg_linear_ce_saved_bytes": [I, I, I],
+    "rg_linear_ce_fwd": [P, I64, P, I64, P, P, I64, I, I, I, I, I, P, P, P, P],
+    "rg_linear_ce_bwd": [P, I64, P, P, I64, I, I, I, I, P, P, P, P, P, P],
     "rg_q4_pack": [P, I, I64, I64, I, I, P, P, P],
     "rg_q4_scores": [P, I, I64, P, P, P, I, I64, I, I, P, I64, P],
 }

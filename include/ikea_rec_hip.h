@@ -633,6 +633,23 @@ int rg_delta_step(const void* q, const void* k, const void* v, const float* g, c
                   const int64_t* strides, int type, int B, int Hk, int Hv, int Dk, int Dv, float scale, float* state,
                   int64_t state_stride, void* o, rg_stream_t stream);
 
+/* ---- Linear cross entropy on half-precision activations (csrc/linear_ce.hip): output layer and loss without logits in
+ * memory, beside the fp32 heads (rg_head_*, rg_flash_*).  z = h W^T + bias, loss_r = lse(z_r) - z_{r, target_r};
+ * h (N, D), W (V, D) of `type` (1 bf16, 2 fp16), row strides ldh / ldw in elements, rows at multiples of 16 bytes; bias
+ * (V) fp32 optional; target (N) int64, stride target_stride.  Negative targets: row ignored (loss and gradient 0);
+ * targets >= V: NaN.  D a multiple of 8 up to 256, N <= 2^24.  grad = 1: also prepares the backward pass.
+ * rg_linear_ce_bwd: dloss (N) fp32; dh (N, D), dW (V, D) contiguous of `type`, db (V) fp32 or NULL.  `saved`
+ * (rg_linear_ce_saved_bytes) goes from the forward to the backward call; `work` (rg_linear_ce_work_floats of pass 0:
+ * forward, 1: forward with grad, 2: backward) only within one. */
+int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass);
+int64_t rg_linear_ce_saved_bytes(int N, int V, int D);
+int rg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, const int64_t* target,
+                     int64_t target_stride, int type, int N, int V, int D, int grad, float* work, void* saved,
+                     float* loss, rg_stream_t stream);
+int rg_linear_ce_bwd(const void* W, int64_t ldw, const float* bias, const float* dloss, int64_t dloss_stride, int type,
+                     int N, int V, int D, const void* saved, float* work, void* dh, void* dW, float* db,
+                     rg_stream_t stream);
+
 /* ---- Scores from a 4-bit item table (csrc/q4.hip): beside rg_head_fwd for serving.  Element types of the
  * operator entry points below: 0 fp32, 1 bf16, 2 fp16.  codes (N, K/2), two a byte, the even column in the low half;
  * scales (N, K/G) bf16; weight = scale·(code - 8).  G = 32, 64 or 128, K a multiple of G up to 1024; codes and scales

@@ -69,3 +69,42 @@ def test_delta_c_entry_refusals():
         return lib.rg_delta_step(p, p, p, p, p, s, 0, B, 1, 1, 16, 16, 1.0, state, stride, p, None)
     assert step(stride=255) == -1 and step(stride=252) == -1 and step(state=p + 4) == -1 and step(B=0) == -3
     assert lib.rg_delta_chunk_floats(2, 64, 3, 8, 8) == 0 and lib.rg_delta_chunk_floats(2, 65, 3, 8, 16) == 2 * 3 * 8 * 16
+
+
+def test_linear_ce_refuses_before_the_device():
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, t = torch.randn(4, 16).bfloat16(), torch.randn(9, 16).bfloat16(), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="HIP device"):
+        linear_ce(h, W, t)
+    with pytest.raises(ValueError, match="type"):
+        linear_ce(h.float(), W, t)
+    with pytest.raises(ValueError, match="saved"):
+        linear_ce_backward(None, t)
+
+
+def test_linear_ce_c_entry_refusals():
+    from recommenders.hip import load_library
+    lib = load_library()
+    p = 4096   # an aligned address that is never read: every call below is refused first
+
+    def fwd(h=p, ldh=16, W=p, ldw=16, t=p, type=1, N=4, V=9, D=16, work=p, saved=p, loss=p):
+        return lib.rg_linear_ce_fwd(h, ldh, W, ldw, None, t, 1, type, N, V, D, 1, work, saved, loss, None)
+    assert fwd(type=0) == -1 and fwd(h=None) == -1 and fwd(h=p + 8) == -1 and fwd(ldh=15) == -1 and fwd(ldw=20) == -1
+    assert fwd(ldw=1 << 23) == -1 and fwd(t=None) == -1 and fwd(work=p + 4) == -1 and fwd(loss=None) == -1
+    assert fwd(N=0) == -3 and fwd(V=0) == -3 and fwd(D=12) == -3 and fwd(D=264, ldh=264, ldw=264) == -3
+    assert fwd(N=(1 << 24) + 1) == -3
+
+    def bwd(W=p, g=p, dh=p, dW=p, db=None, D=16):
+        return lib.rg_linear_ce_bwd(W, 16, None, g, 1, 1, 4, 9, D, p, p, dh, dW, db, None)
+    assert bwd(W=None) == -1 and bwd(g=None) == -1 and bwd(dh=None) == -1 and bwd(dW=p + 2) == -1 and bwd(db=p) == -1
+    assert bwd(D=0) == -3
+
+
+@pytest.mark.parametrize("N,V,D", [(1, 1, 8), (64, 10001, 32), (4096, 1000001, 128), (13111, 78341, 256), (8192, 5000001, 256),
+                                   (1 << 24, 100, 64)])
+def test_linear_ce_partial_results_stay_small(N, V, D):
+    """Splits are bounded: partial sums of a pass take at most 2^28 values beyond one set of results."""
+    from recommenders.hip import load_library
+    lib = load_library()
+    for k in (1, 2):
+        assert 0 < lib.rg_linear_ce_work_floats(N, V, D, k) <= (1 << 28) + 4 * (N + 512) * 256 + 4 * V * (D + 1) + 4 * 512 * N
