@@ -6,14 +6,19 @@
 // N x V logits kept).  A workgroup holds a block of one matrix ("X") in registers and streams the other ("Y") through
 // LDS in chunks of 64 rows:
 //     S = Y_c Xᵀ (MFMA),   P = f(S) rounded to the inputs' type,   Oᵀ += Y_cᵀ P (MFMA)
-//   forward   X = rows of h, Y = W: f = 2^(z − m) with a running reference m; O = Σ_v 2^(z − m) W_v and the sum of P per
+//   forward   X = rows of h, Y = W: f = 2^(z − m) with a reference m of the row; O = Σ_v 2^(z − m) W_v and the sum of P per
 //             row and split of the vocabulary; joined by k_ce_join, which takes W[t] off in fp32 (a one-hot inside P
 //             would be rounded with it).
 //   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r); O = dW, and Σ_r P = db from the unrounded P.
 // The accumulator of S (16 rows of Y x 16 of X per tile; lane (kg, n) holds rows 4·kg + i of column n) is already the B
-// operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  Biases and −lse enter
-// as S's start value, so they cost no instruction.  Per 32 rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D
-// MFMA flops: with 48 or 64 columns of X a wave, LDS bandwidth stays behind the MFMAs.
+// operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  Forwards the biases
+// are S's start value and cost no instruction; backwards −lse and
+// log2 |g| enter with the exponent's scaling (as a start value of size 20 they would cost S its low bits: db was off by
+// 1.5e-6 instead of 1e-7) and bf16's bias factors are left to the end.  That matters because the exponentials, not the
+// MFMAs, take the longer at small D: an element costs a scaling, an exponential (four issue slots), a sum and half a
+// conversion, so there is no running maximum either: forwards the reference only moves when a lane's eight powers
+// sum to more than LIM, which needs one comparison per eight elements.  Per 32 rows of Y a
+// wave reads 2·32·D values from LDS for 4·16·NX·32·D MFMA flops.
 //
 // Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
 // packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
@@ -31,20 +36,20 @@ typedef short ce_s8 __attribute__((ext_vector_type(8)));
 #define CE_L2E 1.4426950408889634f
 #define CE_LN2 0.6931471805599453f
 #define CE_LOW (-3.0e38f)  // the running reference before any logit
-#define CE_HEAD 8.f        // log2 of the largest P before the reference moves
+#define CE_BIG 30.f        // |bias| · log2 e up to which an item's bias is taken out of its probabilities' exponents
 
 template <typename T>
 struct CeT;
 template <>
 struct CeT<__bf16> {
   typedef bf16x8 V;
-  static constexpr float OFF = 0.f;
+  static constexpr float OFF = 0.f, LIM = 0x1p40f;
   static __device__ __forceinline__ f4 mm(V a, V b, f4 c) { return mfma16bf(a, b, c); }
 };
 template <>
 struct CeT<_Float16> {
   typedef h16x8 V;
-  static constexpr float OFF = 7.f;
+  static constexpr float OFF = 7.f, LIM = 0x1p15f;
   static __device__ __forceinline__ f4 mm(V a, V b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -57,7 +62,7 @@ struct CeArgs {
   int D;                   // columns of W's rows (h's packed copy has DP, zeros behind D)
   const int* count;        // packed rows
   const float* bias;       // (V) or null
-  const float* recs;       // backward: [chunk][3][64] −lse, g, target (as int bits)
+  const float* recs;       // backward: [chunk][3][64] log2 |g| − lse · log2 e, g, target (as int bits)
   int nsplit, nblock;
   float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][V][D], pl slabs [split][V]
   void* dW;
@@ -71,12 +76,14 @@ __device__ __forceinline__ int ce_swz(int r) {
   return DP == 64 ? (r >> 1) & 7 : r & 15;
 }
 
-// FWD: forward pass (else backward); GRAD: with the second product
-template <typename T, int DP, int NX, int NW, bool FWD, bool GRAD>
+// FWD: forward pass (else backward); GRAD: with the second product; BIAS: backward with biases
+template <typename T, int DP, int NX, int NW, bool FWD, bool GRAD, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
   typedef typename CeT<T>::V V;
   constexpr int KS = DP / 32, RB = DP * 2, FB = GRAD ? DP / 16 : 1;
   constexpr int LOADS = CE_CH * RB / (NW * 1024);
+  // the swizzled addresses of a tile's reads, remade for each: kept over the loop they would cost a tile's registers
+  constexpr bool REMAKE = DP == 256 && NX > 1;
   static_assert(LOADS >= 1, "a chunk is at least one load a wave");
   __shared__ __attribute__((aligned(16))) uint8_t y0[CE_CH * RB], y1[CE_CH * RB];
   __shared__ __attribute__((aligned(16))) float r0[3 * CE_CH], r1[3 * CE_CH];
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
   if (c0 < c1) issue(c0, y0, r0);
 
   V xf[NX][KS];
-  float ref[NX], top[NX], sum[NX], xb[NX];
+  float ref[NX], sum[NX], xb[NX];
   const T* X = (const T*)a.X;
   const int xcols = FWD ? DP : a.D;
 #pragma unroll
@@ -141,9 +148,15 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
       xf[t][s] = x < nx && col < xcols ? *reinterpret_cast<const V*>(X + x * a.ldx + col) : (V)(T)0.f;
     }
     ref[t] = CE_LOW;
-    top[t] = CE_LOW;   // reference + head room, natural units
     sum[t] = 0.f;
-    xb[t] = !FWD && a.bias != nullptr && x < nx ? a.bias[x] * CE_L2E : 0.f;
+    xb[t] = BIAS && x < nx ? a.bias[x] * CE_L2E : 0.f;
+  }
+  // bf16 has fp32's range: an item's bias factor 2^xb is left out of P and multiplied into its sums at the end
+  bool whole = true;
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int t = 0; t < NX; ++t) whole &= fabsf(xb[t]) <= CE_BIG;
+    whole = CeT<T>::OFF == 0.f && __all(whole);
   }
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   f4 O[FB][NX];
@@ -153,100 +166,121 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     for (int t = 0; t < NX; ++t) O[f][t] = zero;
 
   auto work = [&](int c, uint8_t* y, const float* r) __attribute__((always_inline)) {
-    bool mine = false;   // backward: a target of this chunk among this wave's items
+    // backward: a target of this chunk among this wave's items; a negative g among this chunk's rows
+    bool mine = false, sign = false;
     if constexpr (!FWD) {
       const int t = __float_as_int(r[2 * CE_CH + lane]) - x0;
       mine = __any(t >= 0 && t < 16 * NX);
+      sign = __any(r[CE_CH + lane] < 0.f);
     }
     const bool tail = FWD && c * CE_CH + CE_CH > ny;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      f4 S[2][NX];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = 32 * h + 16 * j + n;
-        const f4 start = *reinterpret_cast<const f4*>(r + 32 * h + 16 * j + 4 * kg);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const V f = *reinterpret_cast<const V*>(y + row * RB + (((4 * s + kg) ^ ce_swz<DP>(row)) << 4));
-#pragma unroll
-          for (int t = 0; t < NX; ++t) S[j][t] = CeT<T>::mm(f, xf[t][s], s == 0 ? start : S[j][t]);
-        }
-      }
       V P[NX];
+      int nn = n;
+      if constexpr (REMAKE) asm volatile("" : "+v"(nn));
+      f4 S[2][NX];
+      const int at = 32 * h + 4 * kg;   // this lane's rows: at .. at + 3 and 16 further on
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int t = 0; t < NX; ++t) S[j][t] = FWD ? *reinterpret_cast<const f4*>(r + at + 16 * j) : zero;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint8_t* p = y + (32 * h + nn) * RB + (((4 * s + kg) ^ ce_swz<DP>(nn)) << 4);
+        const V f0 = *reinterpret_cast<const V*>(p), f1 = *reinterpret_cast<const V*>(p + 16 * RB);
+#pragma unroll
+        for (int t = 0; t < NX; ++t) S[0][t] = CeT<T>::mm(f0, xf[t][s], S[0][t]);
+#pragma unroll
+        for (int t = 0; t < NX; ++t) S[1][t] = CeT<T>::mm(f1, xf[t][s], S[1][t]);
+      }
       if constexpr (FWD) {
         if (tail) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int i = 0; i < 8; ++i)
+            if (c * CE_CH + at + 16 * (i >> 2) + (i & 3) >= ny)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (c * CE_CH + 32 * h + 16 * j + 4 * kg + i >= ny)
-#pragma unroll
-                for (int t = 0; t < NX; ++t) S[j][t][i] = -__builtin_inff();
+              for (int t = 0; t < NX; ++t) S[i >> 2][t][i & 3] = -__builtin_inff();
         }
-        float cm[NX];
-        bool up = false;
-#pragma unroll
-        for (int t = 0; t < NX; ++t) {
-          cm[t] = fmaxf(fmaxf(fmaxf(S[0][t][0], S[0][t][1]), fmaxf(S[0][t][2], S[0][t][3])),
-                        fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
-          up |= cm[t] > top[t];
-        }
-        if (__any(up)) {   // rare after the first chunks: the reference moves, what was summed follows
+        float p[NX][8], add[NX];
+        auto powers = [&]() __attribute__((always_inline)) {
+          bool up = false;
 #pragma unroll
           for (int t = 0; t < NX; ++t) {
-            float m = fmaxf(cm[t], __shfl_xor(cm[t], 16));
+            const float b = CeT<T>::OFF - ref[t];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
+            add[t] = ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
+            up |= !(add[t] <= CeT<T>::LIM);
+          }
+          return up;
+        };
+        if (__any(powers())) {   // rare after a split's first chunk: the reference moves, what was summed follows
+#pragma unroll
+          for (int t = 0; t < NX; ++t) {
+            float m = fmaxf(fmaxf(fmaxf(S[0][t][0], S[0][t][1]), fmaxf(S[0][t][2], S[0][t][3])),
+                            fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
+            m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
             const float now = fmaxf(ref[t], m * CE_L2E), fac = __builtin_amdgcn_exp2f(ref[t] - now);
             ref[t] = now;
-            top[t] = (now + CE_HEAD) * CE_LN2;
             sum[t] *= fac;
 #pragma unroll
             for (int f = 0; f < FB; ++f) O[f][t] *= fac;
           }
+          powers();
         }
 #pragma unroll
         for (int t = 0; t < NX; ++t) {
-          const float b = CeT<T>::OFF - ref[t];
-          float p[8];
+          sum[t] += add[t];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
-            sum[t] += p[i];
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[i];
+          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[t][i];
         }
       } else {
-        f4 g[2];
+        f4 e[2];   // log2(|g| / Σ exp) of this lane's rows
 #pragma unroll
-        for (int j = 0; j < 2; ++j) g[j] = *reinterpret_cast<const f4*>(r + CE_CH + 32 * h + 16 * j + 4 * kg);
+        for (int j = 0; j < 2; ++j) e[j] = *reinterpret_cast<const f4*>(r + at + 16 * j);
+        float p[NX][8];
+        if (whole) {
 #pragma unroll
-        for (int t = 0; t < NX; ++t) {
-          float p[8];
+          for (int t = 0; t < NX; ++t)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, xb[t])) * g[i >> 2][i & 3];
-          if (mine) {
+            for (int i = 0; i < 8; ++i)
+              p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, e[i >> 2][i & 3]));
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int tg = __float_as_int(r[2 * CE_CH + 32 * h + 16 * (i >> 2) + 4 * kg + (i & 3)]);
-              if (tg == x0 + 16 * t + n) p[i] -= g[i >> 2][i & 3];
+          for (int t = 0; t < NX; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, e[i >> 2][i & 3] + xb[t]));
+        }
+        if (mine || sign) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float g = r[CE_CH + at + 16 * (i >> 2) + (i & 3)];
+            const int tg = __float_as_int(r[2 * CE_CH + at + 16 * (i >> 2) + (i & 3)]);
+#pragma unroll
+            for (int t = 0; t < NX; ++t) {
+              if (g < 0.f) p[t][i] = -p[t][i];
+              if (tg == x0 + 16 * t + n) p[t][i] -= whole ? g * __builtin_amdgcn_exp2f(-xb[t]) : g;
             }
           }
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum[t] += p[i];
+        for (int t = 0; t < NX; ++t) {
+          if constexpr (BIAS)
+            sum[t] += ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[i];
+          for (int i = 0; i < 8; ++i) P[t][i] = (T)p[t][i];
         }
       }
       if constexpr (GRAD) {
-        const int row = 32 * h + 4 * kg + (n >> 2);
+        const int row = 32 * h + 4 * kg + (nn >> 2);
 #pragma unroll
         for (int f = 0; f < FB; ++f) {
-          const int ch = 2 * f + ((n >> 1) & 1), half = 8 * (n & 1);
-          uint8_t* p0 = y + row * RB + ((ch ^ ce_swz<DP>(row)) << 4) + half;
-          uint8_t* p1 = y + (row + 16) * RB + ((ch ^ ce_swz<DP>(row + 16)) << 4) + half;
+          const int ch = 2 * f + ((nn >> 1) & 1);
+          uint8_t* p0 = y + row * RB + ((ch ^ ce_swz<DP>(row)) << 4) + 8 * (nn & 1);
+          uint8_t* p1 = p0 + 16 * RB;   // 16 rows on, the same swizzle
           const ce_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ce_s4*)p0);
           const ce_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ce_s4*)p1);
           const ce_s8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -287,7 +321,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
         for (int f = 0; f < FB; ++f) *reinterpret_cast<f4*>(a.pO + at * DP + 16 * f + 4 * kg) = O[f][t];
       }
     } else {
-      const float back = a.scale != nullptr ? a.scale[1] : 1.f;
+      const float back = (a.scale != nullptr ? a.scale[1] : 1.f) * (BIAS && whole ? __builtin_amdgcn_exp2f(xb[t]) : 1.f);
       if (a.nsplit > 1) {
         const int64_t at = (int64_t)split * a.nx + x;
         if (a.db != nullptr && kg == 0) a.pl[at] = sum[t] * back;
@@ -446,8 +480,9 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
   }
   if (lane == 0 && c >= 0) {
     float* rec = recs + (int64_t)(c / CE_CH) * 3 * CE_CH + c % CE_CH;
-    rec[0] = -lse[c];
-    rec[CE_CH] = scale != nullptr ? gr * scale[0] : gr;
+    const float w = scale != nullptr ? gr * scale[0] : gr;
+    rec[0] = __log2f(fabsf(w)) - lse[c] * CE_L2E;
+    rec[CE_CH] = w;
     rec[2 * CE_CH] = __int_as_float(tc[c]);
   }
 }
@@ -475,9 +510,11 @@ __global__ __launch_bounds__(256) void k_ce_slabs(const float* __restrict__ pO, 
 // ------------------------------------------------------------------ host ----
 static int ce_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-// columns of X a workgroup holds (waves x 16 x tiles): 8 waves, two on a SIMD, so that one's exponentials run beside the
-// other's MFMAs; tiles as registers allow (O takes DP / 4 of them per tile)
-static int ce_nx(int DP) { return DP == 64 ? 4 : DP == 128 ? 3 : 2; }
+// a workgroup holds CE_NW · CE_NX · 16 = 256 rows of X: eight waves, two on a SIMD, so that one's exponentials run beside
+// the other's MFMAs, and two tiles a wave.  Measured (4096 x 1M x 128 bf16 / 7867 rows x 78K x 256 fp16, whole
+// step): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
+// two to six tiles each 5.2 ms and more (nothing beside the exponentials).
+#define CE_NX 2
 #define CE_NW 8
 
 // splits of the streamed axis: fewest rounds of 256 workgroups times a split's chunks (and about 8 chunks' worth of
@@ -500,7 +537,7 @@ struct CePlan {
 static CePlan ce_plan(int N, int V, int D) {
   CePlan p;
   p.DP = ce_dp(D);
-  p.xw = 16 * CE_NW * ce_nx(p.DP);
+  p.xw = 16 * CE_NW * CE_NX;
   p.npad = (int)ce_up(N, CE_PAD);
   p.fblocks = (N + p.xw - 1) / p.xw;
   // partial results: at most 2^28 values
@@ -551,17 +588,18 @@ static CeSaved ce_saved(void* base, int N, int D) {
   return s;
 }
 
-template <typename T, int DP, int NX, bool FWD, bool GRAD>
+template <typename T, int DP, bool FWD, bool GRAD, bool BIAS>
 static int ce_pass(const CeArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_ce_pass<T, DP, NX, CE_NW, FWD, GRAD>), dim3(a.nblock * a.nsplit), dim3(64 * CE_NW), 0, st, a);
+  hipLaunchKernelGGL((k_ce_pass<T, DP, CE_NX, CE_NW, FWD, GRAD, BIAS>), dim3(a.nblock * a.nsplit),
+                     dim3(64 * CE_NW), 0, st, a);
   RG_LAUNCH_CHECK();
   return RG_OK;
 }
-template <typename T, bool FWD, bool GRAD>
+template <typename T, bool FWD, bool GRAD, bool BIAS>
 static int ce_pass(int DP, const CeArgs& a, hipStream_t st) {
-  return DP == 64    ? ce_pass<T, 64, 4, FWD, GRAD>(a, st)
-         : DP == 128 ? ce_pass<T, 128, 3, FWD, GRAD>(a, st)
-                     : ce_pass<T, 256, 2, FWD, GRAD>(a, st);
+  return DP == 64    ? ce_pass<T, 64, FWD, GRAD, BIAS>(a, st)
+         : DP == 128 ? ce_pass<T, 128, FWD, GRAD, BIAS>(a, st)
+                     : ce_pass<T, 256, FWD, GRAD, BIAS>(a, st);
 }
 
 template <typename T>
@@ -578,7 +616,7 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
   a.nsplit = p.fsplits, a.nblock = p.fblocks;
   a.pm = work, a.pl = work + (int64_t)p.fsplits * N;
   a.pO = work + ce_up(2 * (int64_t)p.fsplits * N, 64);
-  const int rc = grad ? ce_pass<T, true, true>(p.DP, a, st) : ce_pass<T, true, false>(p.DP, a, st);
+  const int rc = grad ? ce_pass<T, true, true, false>(p.DP, a, st) : ce_pass<T, true, false, false>(p.DP, a, st);
   if (rc != RG_OK) return rc;
   auto join = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((N + 3) / 4), dim3(256), 0, st, a.pm, a.pl, a.pO, p.fsplits, N, D, p.DP,
@@ -609,7 +647,7 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
   a.X = W, a.ldx = ldw, a.nx = V, a.Y = s.hp, a.ldy = p.DP, a.ny = N, a.D = D, a.count = s.count, a.bias = bias;
   a.recs = recs, a.nsplit = p.bsplits, a.nblock = p.bblocks, a.dW = dW, a.db = db, a.scale = scale;
   a.pO = recs + 3 * (int64_t)p.npad, a.pl = a.pO + ce_up((int64_t)p.bsplits * V * D, 64);
-  const int rc = ce_pass<T, false, true>(p.DP, a, st);
+  const int rc = bias != nullptr ? ce_pass<T, false, true, true>(p.DP, a, st) : ce_pass<T, false, true, false>(p.DP, a, st);
   if (rc != RG_OK) return rc;
   if (p.bsplits > 1) {
     const int64_t blocks = ((int64_t)V * D / 4 + 255) / 256;

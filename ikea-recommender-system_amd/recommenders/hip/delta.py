@@ -26,7 +26,7 @@ import ctypes as C
 import torch
 
 from . import call, ptr
-from .operands import TYPES, fail, launch, stride, tensor, whole
+from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole
 
 _IO = (torch.float32, torch.bfloat16)
 
@@ -35,10 +35,12 @@ class Saved:
     """What the backward pass needs of a forward call: its operands (not copied: they have to keep their values) and the
     updates and chunk states it left."""
 
-    def __init__(self, q, k, v, g, beta, scale, lens, state, U, S0):
-        self.operands = (q, k, v, g, beta, lens, state)
-        self.versions = [None if t is None else t._version for t in self.operands]
-        self.scale, self.U, self.S0 = scale, U, S0
+    def __init__(self, plan, operands, scale, U, S0):
+        self.plan, self.operands, self.scale, self.U, self.S0 = plan, operands, scale, U, S0
+        self.versions = [version(t) for t in operands]
+
+
+_plans, _plans_back, _plans_step = Plans(), Plans(), Plans()
 
 
 def _strides(*rows):
@@ -46,55 +48,80 @@ def _strides(*rows):
     return (C.c_int64 * 18)(*flat, *([0] * (18 - len(flat))))
 
 
-def _heads(q, k, v, lead):
-    tensor("q", q, (*lead, None, None), _IO, align=16)
-    Hk, Dk = q.shape[-2:]
-    tensor("k", k, (*q.shape,), (q.dtype,), q.device, align=16)
-    tensor("v", v, (*q.shape[:-2], None, None), (q.dtype,), q.device, align=16)
-    Hv, Dv = v.shape[-2:]
-    if Hk == 0 or Hv == 0 or Hv % Hk:
-        fail("v", f"{Hv} value heads are no multiple of {Hk} key heads")
-    for name, d in (("q", Dk), ("v", Dv)):
-        if d == 0 or d % 8 or d > 128:
-            fail(name, f"a head width that is a multiple of 8 up to 128 is expected, got {d}")
-    return Hk, Hv, Dk, Dv
+class _Plan:
+    """Checks of the operands that forward, backward and step share.  lead: (B, T) or (B,)."""
+
+    def __init__(self, q, k, v, g, beta, lead):
+        tensor("q", q, (*[None] * lead, None, None), _IO, align=16)
+        self.Hk, self.Dk = Hk, Dk = q.shape[-2:]
+        tensor("k", k, (*q.shape,), (q.dtype,), q.device, align=16)
+        tensor("v", v, (*q.shape[:-2], None, None), (q.dtype,), q.device, align=16)
+        self.Hv, self.Dv = Hv, Dv = v.shape[-2:]
+        if Hk == 0 or Hv == 0 or Hv % Hk:
+            fail("v", f"{Hv} value heads are no multiple of {Hk} key heads")
+        for name, d in (("q", Dk), ("v", Dv)):
+            if d == 0 or d % 8 or d > 128:
+                fail(name, f"a head width that is a multiple of 8 up to 128 is expected, got {d}")
+        for name, t in (("g", g), ("beta", beta)):
+            if not isinstance(t, torch.Tensor) or t.dim() != lead + 1:
+                fail(name, f"a tensor of shape {(*q.shape[:-2], Hv)} is expected")
+            tensor(name, t[..., None], (*q.shape[:-2], Hv, 1), (torch.float32,), q.device)   # any strides
+        self.B, self.T = q.shape[0], q.shape[1] if lead == 2 else 1
+        self.device, self.dtype, self.type, self.scale = q.device, q.dtype, TYPES[q.dtype], Dk ** -0.5
+        self.state = (self.B, Hv, Dk, Dv)
+        self.sizes = (self.B, self.T, Hk, Hv, Dk, Dv)
+        self.empty = self.B == 0 or self.T == 0
+        self.rows = [[stride(t, d) for d in range(lead)] for t in (q, k, v, g, beta)]
+        self.rows = [(r if lead == 2 else [r[0], 0]) + [stride(t, lead)] for r, t in zip(self.rows, (q, k, v, g, beta))]
+        self.strides = _strides(*self.rows)
 
 
-def _scalars(g, beta, shape, device):
-    for name, t in (("g", g), ("beta", beta)):
-        if not isinstance(t, torch.Tensor) or t.dim() != len(shape):
-            fail(name, f"a tensor of shape {tuple(shape)} is expected")
-        tensor(name, t[..., None], (*shape, 1), (torch.float32,), device)   # any strides
+def _aligned(**tensors):
+    for name, t in tensors.items():
+        if t is not None and t.data_ptr() & 15:
+            fail(name, "has to start at a multiple of 16 bytes")
+
+
+def _plan(q, k, v, g, beta, lens, state):
+    p = _Plan(q, k, v, g, beta, 2)
+    if lens is not None:
+        whole("lens", lens, (p.B,), (torch.int64,), p.device)
+    if state is not None:
+        whole("state", state, p.state, (torch.float32,), p.device)
+    p.forward, p.backward = entry("rg_delta_fwd"), entry("rg_delta_bwd")
+    p.chunks = call("rg_delta_chunk_floats", p.B, p.T, p.Hv, p.Dk, p.Dv)
+    return p
 
 
 def delta_rule(q, k, v, g, beta, scale=None, lens=None, state=None, save=False):
     """-> o (B, T, Hv, Dv) of q's type, final state (B, Hv, Dk, Dv) fp32, and with save=True what
     delta_rule_backward() takes.  state: initial state (not written), zeros if None; scale: Dk ** -0.5 if None."""
-    Hk, Hv, Dk, Dv = _heads(q, k, v, (None, None))
-    B, T = q.shape[:2]
-    _scalars(g, beta, (B, T, Hv), q.device)
-    if lens is not None:
-        whole("lens", lens, (B,), (torch.int64,), q.device)
-    if state is not None:
-        whole("state", state, (B, Hv, Dk, Dv), (torch.float32,), q.device)
-        if state.data_ptr() % 16:
-            fail("state", "has to start at a multiple of 16 bytes")
-    scale = Dk ** -0.5 if scale is None else float(scale)
-    o = torch.empty(B, T, Hv, Dv, dtype=q.dtype, device=q.device)
-    final = torch.empty(B, Hv, Dk, Dv, dtype=torch.float32, device=q.device)
+    operands = (q, k, v, g, beta, lens, state)
+    key = tuple(map(layout, operands)) if isinstance(q, torch.Tensor) else None
+    p = _plans.get(key) or _plans.put(key, _plan(*operands))
+    at = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), ptr(lens), ptr(state)
+    if (at[0] | at[1] | at[2] | (at[6] or 0)) & 15 and not p.empty:
+        _aligned(q=q, k=k, v=v, state=state)
+    scale = p.scale if scale is None else float(scale)
+    o = torch.empty(p.B, p.T, p.Hv, p.Dv, dtype=p.dtype, device=p.device)
+    final = torch.empty(p.state, dtype=torch.float32, device=p.device)
     U = S0 = None
-    with launch(q) as st:
-        if B == 0 or T == 0:
-            final.copy_(state) if state is not None else final.zero_()
-        else:
-            if save:
-                U = torch.empty(B, Hv, T, Dv, dtype=torch.float32, device=q.device)
-                S0 = torch.empty(call("rg_delta_chunk_floats", B, T, Hv, Dk, Dv), dtype=torch.float32, device=q.device)
-            call("rg_delta_fwd", ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta),
-                 _strides(*([stride(t, 0), stride(t, 1), stride(t, 2)] for t in (q, k, v, g, beta))), ptr(lens),
-                 ptr(state), TYPES[q.dtype], B, T, Hk, Hv, Dk, Dv, scale, ptr(o), ptr(final), ptr(U),
-                 None if S0 is None or not S0.numel() else ptr(S0), st)
-    return (o, final, Saved(q, k, v, g, beta, scale, lens, state, U, S0)) if save else (o, final)
+    if p.empty:
+        final.copy_(state) if state is not None else final.zero_()
+    else:
+        if save:
+            U = torch.empty(p.B, p.Hv, p.T, p.Dv, dtype=torch.float32, device=p.device)
+            S0 = torch.empty(p.chunks, dtype=torch.float32, device=p.device) if p.chunks else None
+        run(p.forward, p.device, *at[:5], p.strides, *at[5:], p.type, *p.sizes, scale, o.data_ptr(), final.data_ptr(),
+            ptr(U), ptr(S0))
+    return (o, final, Saved(p, operands, scale, U, S0)) if save else (o, final)
+
+
+def _back_plan(p, do, dstate):
+    tensor("do", do, (p.B, p.T, p.Hv, p.Dv), (p.dtype,), p.device, align=16)
+    if dstate is not None:
+        whole("dstate", dstate, p.state, (torch.float32,), p.device)
+    return _strides(*p.rows, [stride(do, d) for d in range(3)])
 
 
 def delta_rule_backward(saved, do, dstate=None):
@@ -103,52 +130,53 @@ def delta_rule_backward(saved, do, dstate=None):
     heads in a fixed order.  Can be called again with other gradients."""
     if not isinstance(saved, Saved):
         fail("saved", "what delta_rule(..., save=True) returned is expected")
-    q, k, v, g, beta, lens, state = saved.operands
-    for t, at in zip(saved.operands, saved.versions):
-        if t is not None and t._version != at:
-            raise RuntimeError("delta_rule_backward: an operand of the forward call was changed in place since")
-    B, T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[2:]
-    tensor("do", do, (B, T, Hv, Dv), (q.dtype,), q.device, align=16)
-    if dstate is not None:
-        whole("dstate", dstate, (B, Hv, Dk, Dv), (torch.float32,), q.device)
-        if dstate.data_ptr() % 16:
-            fail("dstate", "has to start at a multiple of 16 bytes")
-    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    dq, dk, dv = new(q), new(k), new(v)
-    dg, dbeta = (torch.empty(B, T, Hv, dtype=torch.float32, device=q.device) for _ in range(2))
-    dstate0 = None if state is None else new(state)
-    with launch(q) as st:
-        if B == 0 or T == 0:
-            if dstate0 is not None:
-                dstate0.copy_(dstate) if dstate is not None else dstate0.zero_()
-        else:
-            dX, dS = torch.empty_like(saved.U), torch.empty_like(saved.S0)
-            there = dS.numel() > 0
-            call("rg_delta_bwd", ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(do),
-                 _strides(*([stride(t, 0), stride(t, 1), stride(t, 2)] for t in (q, k, v, g, beta, do))), ptr(lens),
-                 ptr(state), ptr(dstate), ptr(saved.U), ptr(saved.S0) if there else None, TYPES[q.dtype], B, T, Hk, Hv,
-                 Dk, Dv, saved.scale, ptr(dX), ptr(dS) if there else None, ptr(dq), ptr(dk), ptr(dv), ptr(dg),
-                 ptr(dbeta), ptr(dstate0), st)
+    p, (q, k, v, g, beta, lens, state) = saved.plan, saved.operands
+    if [version(t) for t in saved.operands] != saved.versions:
+        raise RuntimeError("delta_rule_backward: an operand of the forward call was changed in place since")
+    key = (p, layout(do), layout(dstate)) if isinstance(do, torch.Tensor) else None
+    strides = _plans_back.get(key) or _plans_back.put(key, _back_plan(p, do, dstate))
+    if (do.data_ptr() | (ptr(dstate) or 0)) & 15 and not p.empty:
+        _aligned(do=do, dstate=dstate)
+    half = {"dtype": p.dtype, "device": p.device}
+    full = {"dtype": torch.float32, "device": p.device}
+    dq, dk = (torch.empty(p.B, p.T, p.Hk, p.Dk, **half) for _ in range(2))
+    dv = torch.empty(p.B, p.T, p.Hv, p.Dv, **half)
+    dg, dbeta = (torch.empty(p.B, p.T, p.Hv, **full) for _ in range(2))
+    dstate0 = None if state is None else torch.empty(p.state, **full)
+    if p.empty:
+        if dstate0 is not None:
+            dstate0.copy_(dstate) if dstate is not None else dstate0.zero_()
+    else:
+        dX = torch.empty(p.B, p.Hv, p.T, p.Dv, **full)
+        dS = torch.empty(p.chunks, **full) if p.chunks else None
+        run(p.backward, p.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), do.data_ptr(),
+            strides, ptr(lens), ptr(state), ptr(dstate), saved.U.data_ptr(), ptr(saved.S0), p.type, *p.sizes,
+            saved.scale, dX.data_ptr(), ptr(dS), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+            dbeta.data_ptr(), ptr(dstate0))
     return dq, dk, dv, dg, dbeta, dstate0
+
+
+def _step_plan(q, k, v, g, beta, state):
+    p = _Plan(q, k, v, g, beta, 1)
+    tensor("state", state, p.state, (torch.float32,), p.device, align=16)
+    if p.B and not state[0].is_contiguous():
+        fail("state", f"each row's (Hv, Dk, Dv) has to be contiguous, strides are {state.stride()}")
+    if p.B > 1 and state.stride(0) < p.Hv * p.Dk * p.Dv:
+        fail("state", f"rows overlap: stride {state.stride(0)}")
+    p.step, p.apart, p.sizes = entry("rg_delta_step"), stride(state, 0), (p.B, p.Hk, p.Hv, p.Dk, p.Dv)
+    return p
 
 
 def delta_rule_step(q, k, v, g, beta, state, scale=None):
     """One token of every row: q, k (B, Hk, Dk), v (B, Hv, Dv), g, beta (B, Hv); state (B, Hv, Dk, Dv) fp32 is updated
     in place (its rows may lie apart, as in a larger pool, but not overlap).  -> o (B, Hv, Dv) of q's type."""
-    Hk, Hv, Dk, Dv = _heads(q, k, v, (None,))
-    B = q.shape[0]
-    _scalars(g, beta, (B, Hv), q.device)
-    tensor("state", state, (B, Hv, Dk, Dv), (torch.float32,), q.device, align=16)
-    if B and not state[0].is_contiguous():
-        fail("state", f"each row's (Hv, Dk, Dv) has to be contiguous, strides are {state.stride()}")
-    if B > 1 and state.stride(0) < Hv * Dk * Dv:
-        fail("state", f"rows overlap: stride {state.stride(0)}")
-    scale = Dk ** -0.5 if scale is None else float(scale)
-    o = torch.empty(B, Hv, Dv, dtype=q.dtype, device=q.device)
-    if B:
-        with launch(q) as st:
-            call("rg_delta_step", ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta),
-                 _strides(*([stride(t, 0), 0, stride(t, 1)] for t in (q, k, v, g, beta))), TYPES[q.dtype], B, Hk, Hv, Dk,
-                 Dv, scale, ptr(state), stride(state, 0), ptr(o), st)
+    key = tuple(map(layout, (q, k, v, g, beta, state))) if isinstance(q, torch.Tensor) else None
+    p = _plans_step.get(key) or _plans_step.put(key, _step_plan(q, k, v, g, beta, state))
+    o = torch.empty(p.B, p.Hv, p.Dv, dtype=p.dtype, device=p.device)
+    if p.B:
+        at = state.data_ptr()
+        if at & 15:
+            _aligned(state=state)
+        run(p.step, p.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), p.strides, p.type,
+            *p.sizes, p.scale if scale is None else float(scale), at, p.apart, o.data_ptr())
     return o

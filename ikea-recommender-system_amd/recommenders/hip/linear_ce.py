@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import call, ptr
-from .operands import TYPES, fail, launch, stride, tensor, whole
+from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole
 
 _HALF = (torch.bfloat16, torch.float16)
 _I64 = (torch.int64,)
@@ -29,63 +29,88 @@ _I64 = (torch.int64,)
 class Saved:
     """What the backward pass needs of a forward call; W and bias are not copied and have to keep their values."""
 
-    def __init__(self, h, W, bias, buffer):
-        self.shape, self.W, self.bias, self.buffer = h.shape, W, bias, buffer
-        self.versions = (W._version, None if bias is None else bias._version)
+    def __init__(self, plan, W, bias, buffer):
+        self.plan, self.W, self.bias, self.buffer = plan, W, bias, buffer
+        self.versions = version(W), version(bias)
+
+
+_plans, _plans_back = Plans(), Plans()
+
+
+class _Plan:
+    def __init__(self, h, W, target, bias):
+        tensor("h", h, (None, None), _HALF, align=16)
+        self.N, self.D = N, D = h.shape
+        tensor("W", W, (None, D), (h.dtype,), h.device, align=16)
+        self.V = V = W.shape[0]
+        if D == 0 or D % 8 or D > 256:
+            fail("h", f"a width that is a multiple of 8 up to 256 is expected, got {D}")
+        if V == 0:
+            fail("W", "has no rows")
+        if N > 1 << 24:
+            fail("h", f"at most 2^24 rows are expected, got {N}")
+        for name, t in (("h", h), ("W", W)):
+            if t.shape[0] > 1 and not D <= t.stride(0) < 1 << 23:
+                fail(name, f"rows overlap or lie too far apart: stride {t.stride(0)}")
+        if not isinstance(target, torch.Tensor) or target.dim() != 1:
+            fail("target", "a tensor of shape (N,) is expected")
+        tensor("target", target[:, None], (N, 1), _I64, h.device)
+        if bias is not None:
+            whole("bias", bias, (V,), (torch.float32,), h.device)
+        self.device, self.dtype, self.type = h.device, h.dtype, TYPES[h.dtype]
+        self.ldh, self.ldw, self.st = stride(h, 0) or D, stride(W, 0) or D, stride(target, 0)
+        if N:
+            self.forward, self.backward = entry("rg_linear_ce_fwd"), entry("rg_linear_ce_bwd")
+            self.saved = call("rg_linear_ce_saved_bytes", N, V, D)
+            self.work = [call("rg_linear_ce_work_floats", N, V, D, k) for k in range(3)]
+
+
+def _aligned(**tensors):
+    for name, t in tensors.items():
+        if t.data_ptr() & 15:
+            fail(name, "has to start at a multiple of 16 bytes")
 
 
 def linear_ce(h, W, target, bias=None, save=False):
     """Losses (N,) fp32 and, with save=True, what linear_ce_backward() takes (the forward then also sums dh)."""
-    tensor("h", h, (None, None), _HALF, align=16)
-    N, D = h.shape
-    tensor("W", W, (None, D), (h.dtype,), h.device, align=16)
-    V = W.shape[0]
-    if D == 0 or D % 8 or D > 256:
-        fail("h", f"a width that is a multiple of 8 up to 256 is expected, got {D}")
-    if V == 0:
-        fail("W", "has no rows")
-    if N > 1 << 24:
-        fail("h", f"at most 2^24 rows are expected, got {N}")
-    for name, t in (("h", h), ("W", W)):
-        if t.shape[0] > 1 and not D <= t.stride(0) < 1 << 23:
-            fail(name, f"rows overlap or lie too far apart: stride {t.stride(0)}")
-    if not isinstance(target, torch.Tensor) or target.dim() != 1:
-        fail("target", "a tensor of shape (N,) is expected")
-    tensor("target", target[:, None], (N, 1), _I64, h.device)
-    if bias is not None:
-        whole("bias", bias, (V,), (torch.float32,), h.device)
-    loss = torch.empty(N, dtype=torch.float32, device=h.device)
+    key = (layout(h), layout(W), layout(target), layout(bias)) if isinstance(h, torch.Tensor) else None
+    p = _plans.get(key) or _plans.put(key, _Plan(h, W, target, bias))
+    loss = torch.empty(p.N, dtype=torch.float32, device=p.device)
     buffer = None
-    if N:
-        with launch(h) as st:
-            buffer = torch.empty(call("rg_linear_ce_saved_bytes", N, V, D), dtype=torch.uint8, device=h.device)
-            work = torch.empty(call("rg_linear_ce_work_floats", N, V, D, int(save)), dtype=torch.float32, device=h.device)
-            call("rg_linear_ce_fwd", ptr(h), stride(h, 0) or D, ptr(W), stride(W, 0) or D, ptr(bias), ptr(target),
-                 stride(target, 0), TYPES[h.dtype], N, V, D, int(save), ptr(work), ptr(buffer), ptr(loss), st)
-    return (loss, Saved(h, W, bias, buffer)) if save else loss
+    if p.N:
+        if (h.data_ptr() | W.data_ptr()) & 15:
+            _aligned(h=h, W=W)
+        save = bool(save)
+        buffer = torch.empty(p.saved, dtype=torch.uint8, device=p.device)
+        work = torch.empty(p.work[save], dtype=torch.float32, device=p.device)
+        run(p.forward, p.device, h.data_ptr(), p.ldh, W.data_ptr(), p.ldw, ptr(bias), target.data_ptr(), p.st, p.type, p.N,
+            p.V, p.D, save, work.data_ptr(), buffer.data_ptr(), loss.data_ptr())
+    return (loss, Saved(p, W, bias, buffer)) if save else loss
 
 
 def linear_ce_backward(saved, dloss):
     """dh (N, D), dW (V, D), db (V) or None of sum(loss·dloss).  Can be called again with another dloss."""
     if not isinstance(saved, Saved):
         fail("saved", "what linear_ce(..., save=True) returned is expected")
-    W, bias, (N, D) = saved.W, saved.bias, saved.shape
-    if (W._version, None if bias is None else bias._version) != saved.versions:
+    p, W, bias = saved.plan, saved.W, saved.bias
+    if (version(W), version(bias)) != saved.versions:
         raise RuntimeError("linear_ce_backward: W or bias was changed in place since the forward call")
-    V = W.shape[0]
-    if not isinstance(dloss, torch.Tensor) or dloss.dim() != 1:
-        fail("dloss", "a tensor of shape (N,) is expected")
-    tensor("dloss", dloss[:, None], (N, 1), (torch.float32,), W.device)
-    dh = torch.empty(N, D, dtype=W.dtype, device=W.device)
-    dW = torch.empty(V, D, dtype=W.dtype, device=W.device)
-    db = None if bias is None else torch.empty(V, dtype=torch.float32, device=W.device)
-    with launch(W) as st:
-        if N == 0:
-            dW.zero_()
-            if db is not None:
-                db.zero_()
-        else:
-            work = torch.empty(call("rg_linear_ce_work_floats", N, V, D, 2), dtype=torch.float32, device=W.device)
-            call("rg_linear_ce_bwd", ptr(W), stride(W, 0) or D, ptr(bias), ptr(dloss), stride(dloss, 0), TYPES[W.dtype],
-                 N, V, D, ptr(saved.buffer), ptr(work), ptr(dh), ptr(dW), ptr(db), st)
+    key = (p.N, layout(dloss), p.device) if isinstance(dloss, torch.Tensor) else None
+    step = _plans_back.get(key)
+    if step is None:
+        if not isinstance(dloss, torch.Tensor) or dloss.dim() != 1:
+            fail("dloss", "a tensor of shape (N,) is expected")
+        tensor("dloss", dloss[:, None], (p.N, 1), (torch.float32,), p.device)
+        step = _plans_back.put(key, (stride(dloss, 0),))
+    dh = torch.empty(p.N, p.D, dtype=p.dtype, device=p.device)
+    dW = torch.empty(p.V, p.D, dtype=p.dtype, device=p.device)
+    db = None if bias is None else torch.empty(p.V, dtype=torch.float32, device=p.device)
+    if p.N == 0:
+        dW.zero_()
+        if db is not None:
+            db.zero_()
+    else:
+        work = torch.empty(p.work[2], dtype=torch.float32, device=p.device)
+        run(p.backward, p.device, W.data_ptr(), p.ldw, ptr(bias), dloss.data_ptr(), *step, p.type, p.N, p.V, p.D,
+            saved.buffer.data_ptr(), work.data_ptr(), dh.data_ptr(), dW.data_ptr(), ptr(db))
     return dh, dW, db

@@ -52,17 +52,39 @@ def stride(t, dim):
     return 0 if t.shape[dim] == 1 else t.stride(dim)
 
 
-class launch:
-    """The device of `t` made current for the calls inside; the stream they use."""
+def layout(t):
+    """What the checks of a tensor argument look at, apart from its address: calls with known layouts skip them."""
+    return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else None if t is None else type(t)
 
-    def __init__(self, t):
-        load_library()
-        self._guard = torch.cuda.device(t.device)
-        self._device = t.device
 
-    def __enter__(self):
-        self._guard.__enter__()
-        return torch.cuda.current_stream(self._device).cuda_stream
+def version(t):
+    """Changes with every write in place (None: not known, as for inference tensors)."""
+    return None if t is None or t.is_inference() else t._version
 
-    def __exit__(self, *exc):
-        return self._guard.__exit__(*exc)
+
+class Plans(dict):
+    """Checked argument layouts -> what a call needs of them.  Bounded: a program has few layouts; one that keeps making
+    new ones starts over now and then."""
+
+    def put(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+def entry(name):
+    """The C function of an entry point; use run() to call it."""
+    return getattr(load_library(), name)
+
+
+def run(fn, device, *args):
+    """Launch on `device`'s current stream, with `device` current (it usually is already)."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc < 0:
+        raise RuntimeError(f"{fn.__name__} failed with status {rc}")

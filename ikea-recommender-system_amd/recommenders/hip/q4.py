@@ -16,8 +16,8 @@ from __future__ import annotations
 
 import torch
 
-from . import call, ptr
-from .operands import TYPES, fail, launch, stride, tensor, whole
+from . import ptr
+from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, whole
 
 GROUPS = (32, 64, 128)
 K_MAX = 1024
@@ -39,13 +39,14 @@ def q4_pack(W, group=32):
     codes = torch.empty(N, K // 2, dtype=torch.uint8, device=W.device)
     scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=W.device)
     if N:
-        with launch(W) as st:
-            call("rg_q4_pack", ptr(W), TYPES[W.dtype], stride(W, 0) or K, N, K, group, ptr(codes), ptr(scales), st)
+        run(entry("rg_q4_pack"), W.device, ptr(W), TYPES[W.dtype], stride(W, 0) or K, N, K, group, ptr(codes), ptr(scales))
     return codes, scales
 
 
-def q4_scores(x, codes, scales, bias=None, out=None):
-    """x (M, K) · table (N, K)ᵀ + bias -> (M, N) fp32.  out: written instead of a new tensor; its rows may be strided."""
+_plans = Plans()
+
+
+def _plan(x, codes, scales, bias):
     tensor("x", x, (None, None), (torch.float32, torch.bfloat16))
     M, K = x.shape
     whole("codes", codes, (None, K // 2), (torch.uint8,), x.device)
@@ -55,19 +56,26 @@ def q4_scores(x, codes, scales, bias=None, out=None):
     if groups == 0 or K % groups:
         fail("scales", f"{groups} groups do not divide {K} columns")
     _table(K, K // groups)
-    for name, t in (("codes", codes), ("scales", scales)):
-        if N and t.data_ptr() % 16:
-            fail(name, "has to start at a multiple of 16 bytes")
     if bias is not None:
         whole("bias", bias, (N,), (torch.float32,), x.device)
+    return entry("rg_q4_scores"), x.device, M, N, K, K // groups, TYPES[x.dtype], stride(x, 0) or K
+
+
+def q4_scores(x, codes, scales, bias=None, out=None):
+    """x (M, K) · table (N, K)ᵀ + bias -> (M, N) fp32.  out: written instead of a new tensor; its rows may be strided."""
+    key = (layout(x), layout(codes), layout(scales), layout(bias)) if isinstance(x, torch.Tensor) else None
+    fn, device, M, N, K, group, kind, ldx = _plans.get(key) or _plans.put(key, _plan(x, codes, scales, bias))
+    at = codes.data_ptr(), scales.data_ptr()
+    if (at[0] | at[1]) & 15 and N:
+        fail("codes" if at[0] & 15 else "scales", "has to start at a multiple of 16 bytes")
     if out is None:
-        out = torch.empty(M, N, dtype=torch.float32, device=x.device)
+        out = torch.empty(M, N, dtype=torch.float32, device=device)
+        ldy = N
     else:
-        tensor("out", out, (M, N), (torch.float32,), x.device)
+        tensor("out", out, (M, N), (torch.float32,), device)
         if M > 1 and out.stride(0) < N:
             fail("out", f"rows overlap: stride {out.stride(0)}, {N} items")
+        ldy = stride(out, 0) or N
     if M and N:
-        with launch(x) as st:
-            call("rg_q4_scores", ptr(x), TYPES[x.dtype], stride(x, 0) or K, ptr(codes), ptr(scales), ptr(bias), M, N, K,
-                 K // groups, ptr(out), stride(out, 0) or N, st)
+        run(fn, device, x.data_ptr(), kind, ldx, *at, ptr(bias), M, N, K, group, out.data_ptr(), ldy)
     return out
