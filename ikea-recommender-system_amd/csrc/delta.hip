@@ -1,7 +1,7 @@
 // Gated delta rule: a linear-attention recurrence beside the GRU (csrc/gru.hip), per value head with a Dk x Dv state
 //     S_t = a_t S_{t-1} + b_t k_t (v_t − a_t S_{t-1}ᵀ k_t)ᵀ,   o_t = scale · S_tᵀ q_t,   a_t = exp(g_t)
 //
-// Chunks of 64 positions.  With G_i the running sum of g inside a chunk, D_ij = exp(G_i − G_j), S the state before it:
+// Chunks of 32 positions.  With G_i the running sum of g inside a chunk, D_ij = exp(G_i − G_j), S the state before it:
 //     A_ij = b_i D_ij k_i·k_j (j < i),  P_ij = scale · D_ij q_i·k_j (j <= i),  T = (1 + A)^-1   (unit lower triangular)
 //     X = diag(b)(V − diag(e^G) K S),   U = T X,   O = scale · diag(e^G) Q S + P U
 //     S' = e^{G_end} S + Kᵀ diag(D_end) U
@@ -10,13 +10,28 @@
 //     dS_prev = e^{G_end} dS + Qᵀ diag(scale · e^G) dO − Kᵀ diag(b e^G) dX
 // and, per chunk and independent of the others, dP = dO Uᵀ, dA = −dX Uᵀ and the rest (k_delta_grads).
 //
+// One wave owns 16·CT value columns of one (row, value head) and their part of the state, in accumulators; it makes the
+// chunk's P and T itself and never waits for another wave.  What bounds these kernels is the chain of dependent steps
+// inside a chunk (about 20 products and a triangular solve of 16 steps), not bandwidth or MFMAs: sessions are
+// short, so the answer is many independent waves with little LDS, and each step small.  (Workgroups of four waves with
+// 64-position chunks, K, Q, P and T shared through LDS and a barrier between steps: two workgroups fit a CU, 20 us each;
+// 8192 sessions x heads of width 64 took 320 us forwards.)  A long row is cut into segments whose
+// waves run side by side (below).
+//
 // The state, G and every sum are fp32 or wider (G in fp64: differences of long sums enter an exponential).  Products run
-// on bf16 MFMA with fp32 operands split into planes (planes.h): three planes (six products) for fp32 inputs; bf16
-// inputs are one exact plane.  Positions at or behind a sequence's length are read as k = v = q = 0, b = 0, g = 0,
-// which leaves the state as it is; nothing is read there.
+// on bf16 MFMA with fp32 operands split into three planes (planes.h); bf16 inputs are one exact plane.  Two planes
+// would halve the products, but leave the fp32 outputs (state, dg, dbeta) at 2^-18 instead of fp32's own rounding.
+// Positions at or behind a sequence's length are read as k = v = q = 0, b = 0, g = 0, which leaves the state as it is;
+// nothing is read there.
+//
+// Accumulator tiles feed the next product from their registers: a tile of rows i and columns n packs (with the next 16
+// rows) into an operand with n as its free index and i contracted, whichever side it stands on.  So P and T are made in
+// the orientation in which they are used and never pass through LDS; T's blocks come from forward substitution in
+// registers, by columns or by rows as the use wants.
 #include "planes.h"
 
-#define DL_C 64
+#define DL_C 32
+#define DL_NP 3
 #define DL_G_MIN (-1000.0)   // exp of anything below is 0 in fp32; keeps −inf (a full reset) out of differences
 
 struct DeltaArgs {
@@ -30,22 +45,75 @@ struct DeltaArgs {
   float *state, *dstate0, *dg, *dbeta;
   float *U, *dX;                            // (B, Hv, T, Dv)
   float *S0, *dS;                           // (B, Hv, chunks - 1, Dk, Dv): states before chunk c + 1, gradients after chunk c
+  // segments of `per` chunks; nseg = 1: none.  trans (B, Hv, nseg, Dk, Dk): what a segment does to the state it starts
+  // with; local (B, Hv, nseg, Dk, Dv): the state (or its gradient) it leaves when it starts from zero, then, joined,
+  // the one it really starts from
+  int nseg, per;
+  float *trans, *local;
 };
+
+typedef uint32_t dl_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t dl_u2 __attribute__((ext_vector_type(2)));
+
+// Memory through buffer resources.  A lane's part of an offset is one register, the rest (row, tile) is uniform and goes
+// into the scalar offset; rows behind the last one lie behind the resource's end and a lane whose column does not exist
+// has an offset behind any end: such loads give 0 and such stores do nothing, without a branch or a mask per access.
+// (All elements of a vector load have to be used: narrowed to its last elements, this compiler reads the first.)
+typedef __amdgpu_buffer_rsrc_t DlBuf;
+// rows of `cols` elements, `st` apart (st >= cols, or one row)
+__device__ __forceinline__ DlBuf dl_buf(const void* p, int rows, int64_t st, int cols, int size) {
+  const int64_t bytes = rows > 0 ? ((rows - 1) * st + cols) * size : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ int dl_lane(bool on, int bytes) { return on ? bytes : (int)0x80000000; }
 
 template <typename IO>
 struct DlIO;
 template <>
 struct DlIO<float> {
-  static constexpr int N = 3;
-  static __device__ __forceinline__ void load8(const float* p, bf16x8* f) {
-    pl_split<3>(*reinterpret_cast<const f4*>(p), *reinterpret_cast<const f4*>(p + 4), f);
+  static constexpr int N = 3, SIZE = 4;
+  static __device__ __forceinline__ float load1(DlBuf b, int v, int s) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, v, s, 0));
+  }
+  static __device__ __forceinline__ f4 load4(DlBuf b, int v, int s) {
+    return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(b, v, s, 0));
+  }
+  static __device__ __forceinline__ void load44(DlBuf b, int v, int s, int v2, int s2, bf16x8* f) {
+    pl_split<3>(load4(b, v, s), load4(b, v2, s2), f);
+  }
+  struct Raw8 {
+    f4 a, b;
+  };
+  static __device__ __forceinline__ Raw8 load8(DlBuf b, int v, int s) { return {load4(b, v, s), load4(b, v + 16, s)}; }
+  static __device__ __forceinline__ void planes(const Raw8& x, bf16x8* f) { pl_split<3>(x.a, x.b, f); }
+  static __device__ __forceinline__ void store1(DlBuf b, int v, int s, float x) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), b, v, s, 0);
+  }
+  static __device__ __forceinline__ void store4(DlBuf b, int v, int s, f4 x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dl_u4, x), b, v, s, 0);
   }
 };
 template <>
 struct DlIO<__bf16> {
-  static constexpr int N = 1;
-  static __device__ __forceinline__ void load8(const __bf16* p, bf16x8* f) {
-    f[0] = *reinterpret_cast<const bf16x8*>(p);
+  static constexpr int N = 1, SIZE = 2;
+  static __device__ __forceinline__ float load1(DlBuf b, int v, int s) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b, v, s, 0) << 16);
+  }
+  static __device__ __forceinline__ void load44(DlBuf b, int v, int s, int v2, int s2, bf16x8* f) {
+    const dl_u2 x = __builtin_amdgcn_raw_buffer_load_b64(b, v, s, 0), y = __builtin_amdgcn_raw_buffer_load_b64(b, v2, s2, 0);
+    f[0] = __builtin_bit_cast(bf16x8, (dl_u4){x[0], x[1], y[0], y[1]});
+  }
+  typedef bf16x8 Raw8;
+  static __device__ __forceinline__ Raw8 load8(DlBuf b, int v, int s) {
+    return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, v, s, 0));
+  }
+  static __device__ __forceinline__ void planes(const Raw8& x, bf16x8* f) { f[0] = x; }
+  static __device__ __forceinline__ void store1(DlBuf b, int v, int s, float x) {
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)x), b, v, s, 0);
+  }
+  static __device__ __forceinline__ void store4(DlBuf b, int v, int s, f4 x) {
+    typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(dl_u2, __builtin_convertvector(x, bf4)), b, v, s, 0);
   }
 };
 
@@ -55,521 +123,580 @@ __device__ __forceinline__ int dl_len(const DeltaArgs& a, int b) {
   return n < 0 ? 0 : n > a.T ? a.T : (int)n;
 }
 
-// rows t0 .. t0 + 63 of a (T, D) operand into planes; zeros behind `len` and behind column D
-template <typename IO, int DP>
-__device__ __forceinline__ void dl_load(const PlaneMat<DL_C, DP, DlIO<IO>::N>& m, const IO* base, int64_t st, int t0,
-                                        int len, int D, int tid, int nthreads) {
-  constexpr int N = DlIO<IO>::N;
-  for (int e = tid; e < DL_C * (DP / 8); e += nthreads) {
-    const int r = e / (DP / 8), c = (e % (DP / 8)) * 8;
-    bf16x8 f[N] = {};
-    if (t0 + r < len && c < D) DlIO<IO>::load8(base + (int64_t)(t0 + r) * st + c, f);
-    m.put8(r, c, f);
+// 32 rows of a (.., D) operand into planes (zeros behind the buffer's rows and behind column D)
+template <typename IO, int DP, int THREADS>
+__device__ __forceinline__ void dl_load(const PlaneMat<DL_C, DP, DlIO<IO>::N>& m, DlBuf buf, int64_t st, int D, int tid) {
+  constexpr int N = DlIO<IO>::N, W = DP / 8, ALL = DL_C * W, PER = ALL / THREADS > 0 ? ALL / THREADS : 1;
+  const int r = tid / W, c = tid % W * 8, v = dl_lane(c < D && tid < ALL, (int)(r * st + c) * DlIO<IO>::SIZE);
+  const int step = (int)(THREADS / W * st) * DlIO<IO>::SIZE;
+  typename DlIO<IO>::Raw8 x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = DlIO<IO>::load8(buf, v, i * step);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    bf16x8 f[N];
+    DlIO<IO>::planes(x[i], f);
+    if (ALL >= THREADS || tid < ALL) m.put8(r + i * (THREADS / W), c, f);
   }
+}
+// operand straight from memory: rows `row` + n, columns c0 + 4·kg .. and 16 further on
+template <typename IO>
+__device__ __forceinline__ void dl_operand(bf16x8* f, DlBuf buf, int row, int64_t st, int c0, int D) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, v = (int)(n * st + 4 * kg) * DlIO<IO>::SIZE;
+  const int s = (int)(row * st + c0) * DlIO<IO>::SIZE;
+  DlIO<IO>::load44(buf, dl_lane(c0 + 4 * kg < D, v), s, dl_lane(c0 + 16 + 4 * kg < D, v), s + 16 * DlIO<IO>::SIZE, f);
 }
 
 // per-position scalars of a chunk
 struct DlGates {
-  double G[DL_C];        // running sum of g
-  float gam[DL_C];       // exp(G_i)
-  float rest[DL_C];      // exp(G_end − G_i)
+  double G[DL_C];        // running sum of g · log2 e
+  float gam[DL_C];       // 2^G_i
+  float rest[DL_C];      // 2^(G_end − G_i)
   float beta[DL_C];
 };
+__device__ __forceinline__ float dl_exp2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 // one wave
 __device__ __forceinline__ void dl_gates(DlGates& s, const DeltaArgs& a, int b, int h, int t0, int len) {
-  const int i = threadIdx.x & 63, t = t0 + i;
-  double g = 0.0;
-  float be = 0.f;
-  if (t < len) {
-    g = a.g[b * a.gs[0] + t * a.gs[1] + h * a.gs[2]];
-    g = g < DL_G_MIN ? DL_G_MIN : g;   // NaN stays
-    be = a.beta[b * a.bs[0] + t * a.bs[1] + h * a.bs[2]];
-  }
+  const int i = threadIdx.x & 31, t = t0 + i;
+  const DlBuf gbuf = dl_buf(a.g + b * a.gs[0] + t0 * a.gs[1] + h * a.gs[2], 32, a.gs[1], 1, 4),
+              bbuf = dl_buf(a.beta + b * a.bs[0] + t0 * a.bs[1] + h * a.bs[2], 32, a.bs[1], 1, 4);
+  const float gi = DlIO<float>::load1(gbuf, dl_lane(t < len, (int)(i * a.gs[1]) * 4), 0);
+  const float be = DlIO<float>::load1(bbuf, dl_lane(t < len, (int)(i * a.bs[1]) * 4), 0);
+  double g = (gi < DL_G_MIN ? DL_G_MIN : (double)gi) * 1.4426950408889634;   // NaN stays
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(g, o);
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up(g, o, 32);
     if (i >= o) g += up;
   }
-  const double end = __shfl(g, 63);
-  s.G[i] = g;
-  s.gam[i] = expf((float)g);
-  s.rest[i] = expf((float)(end - g));
-  s.beta[i] = be;
+  const double end = __shfl(g, 31, 32);
+  if ((threadIdx.x & 63) < 32) {
+    s.G[i] = g;
+    s.gam[i] = dl_exp2(g);
+    s.rest[i] = dl_exp2(end - g);
+    s.beta[i] = be;
+  }
 }
 
-// T and P of a chunk in planes, from K and Q in planes and the gates.  P's place holds A first: its off-diagonal blocks
-// in planes, its diagonal 16 x 16 blocks in fp32 in the quadrant of rows 0 .. 31 and columns 32 .. 63, which no product
-// reads.  The other upper tiles must be zero before and stay so.  All waves call it; ends with every wave's writes visible.
-template <int NP>
-__device__ __forceinline__ float* dl_diag(const PlaneMat<DL_C, 64, NP>& P, int r) {   // row r of 64: 16 floats
-  using M = PlaneMat<DL_C, 64, NP>;
-  return reinterpret_cast<float*>(P.p + (r >> 5) * M::PLANE + (r & 31) * M::LD + 32);
-}
-template <int DP, int NI, int NP>
-__device__ __forceinline__ void dl_prep(const PlaneMat<DL_C, DP, NI>& K, const PlaneMat<DL_C, DP, NI>& Q,
-                                        const PlaneMat<DL_C, 64, NP>& P, const PlaneMat<DL_C, 64, NP>& T,
-                                        const DlGates& s, float scale, int nt, int wave, int nw) {
-  static_assert(NP >= 2, "the diagonal blocks need two planes' room");
-  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  auto lower = [&](const PlaneMat<DL_C, DP, NI>& X, auto use) {   // the lower tiles of X Kᵀ times D
-    for (int job = wave; job < 10; job += nw) {
-      const int it = job < 1 ? 0 : job < 3 ? 1 : job < 6 ? 2 : 3, jt = job - it * (it + 1) / 2;
-      if (it >= nt) break;
-      f4 x = {0.f, 0.f, 0.f, 0.f};
+#define DL_ZERO ((f4){0.f, 0.f, 0.f, 0.f})
+
+// Forward substitution: column n of (1 + A)^-1, A strictly lower, 16 x 16 in LDS (rows of 20 floats, read by many lanes at
+// once).  The next row is read while this one's sum runs; left to itself the compiler reads all of A first (120 registers).
+__device__ __forceinline__ void dl_solve(const float* A, int n, float* t) {
+  f4 row[4], next[4];
+  t[0] = n == 0 ? 1.f : 0.f;
+  next[0] = *reinterpret_cast<const f4*>(A + 20);
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
-        bf16x8 xi[NI], kj[NI];
-        X.row(xi, 16 * it, t);
-        K.row(kj, 16 * jt, t);
-        x = pl_mm<NI, NI>(xi, kj, x);
-      }
-      const int j = 16 * jt + n;
-      const double gj = s.G[j];
+  for (int i = 1; i < 16; ++i) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * it + 4 * kg + r;
-        use(i, j, it == jt, expf((float)(s.G[i] - gj)) * x[r]);
-      }
+    for (int q = 0; q < 4; ++q) row[q] = next[q];
+    if (i < 15) {
+#pragma unroll
+      for (int q = 0; q < (i + 4) / 4; ++q) next[q] = *reinterpret_cast<const f4*>(A + (i + 1) * 20 + 4 * q);
     }
-  };
-  lower(K, [&](int i, int j, bool diag, float x) {
-    x = j < i ? s.beta[i] * x : 0.f;
-    if (diag)
-      dl_diag(P, i)[j & 15] = x;
-    else
-      P.put(i, j, x);
-  });
-  __syncthreads();
-  // T of the diagonal blocks: lane (kg, n) solves column n of block kg forwards
-  if (wave == 0 && kg < nt) {
-    float t[16];
+    float x = i == n ? 1.f : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const f4* row = reinterpret_cast<const f4*>(dl_diag(P, 16 * kg + i));
-      float x = i == n ? 1.f : 0.f;
-#pragma unroll
-      for (int j = 0; j < i; ++j) x = __builtin_fmaf(-row[j >> 2][j & 3], t[j], x);
-      t[i] = x;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) T.put(16 * kg + i, 16 * kg + n, t[i]);
+    for (int j = 0; j < i; ++j) x = __builtin_fmaf(-row[j >> 2][j & 3], t[j], x);
+    t[i] = x;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   }
-  __syncthreads();
-  // T_10 = −T_11 (A_10 T_00) inside each 32 x 32 diagonal block; the operands' other halves are zeroed
-  const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  if (nt > 1) {
-    for (int p = wave; 2 * p + 1 < nt; p += nw) {
-      bf16x8 x[NP], y[NP];
-      P.row(x, 16 * (2 * p + 1), p);
-      T.col(y, p, 32 * p);
-#pragma unroll
-      for (int q = 0; q < NP; ++q)
-#pragma unroll
-        for (int e = 4; e < 8; ++e) y[q][e] = (__bf16)0.f, x[q][e] = (__bf16)0.f;
-      const f4 m1 = pl_mm<NP, NP>(x, y, zero);
-      T.row(x, 16 * (2 * p + 1), p);
-#pragma unroll
-      for (int q = 0; q < NP; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[q][e] = (__bf16)0.f;
-      pl_split<NP>(zero, m1, y);
-      const f4 m2 = pl_mm<NP, NP>(x, y, zero);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) T.put(32 * p + 16 + 4 * kg + r, 32 * p + n, -m2[r]);
-    }
-    __syncthreads();
-  }
-  if (nt > 2) {   // and of the 64 x 64 block
-    for (int jt = wave; jt < 2; jt += nw) {
-      bf16x8 x[NP], y[NP];
-      T.col(y, 0, 16 * jt);
-      f4 m[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        P.row(x, 32 + 16 * r, 0);
-        m[r] = pl_mm<NP, NP>(x, y, zero);
-      }
-      if (nt < 4) m[1] = zero;
-      pl_split<NP>(m[0], m[1], y);
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        if (2 + r < nt) {
-          T.row(x, 32 + 16 * r, 1);
-          const f4 m2 = pl_mm<NP, NP>(x, y, zero);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) T.put(32 + 16 * r + 4 * kg + i, 16 * jt + n, -m2[i]);
-        }
-    }
-    __syncthreads();
-  }
-  lower(Q, [&](int i, int j, bool diag, float x) { P.put(i, j, j <= i ? scale * x : 0.f); });
-  __syncthreads();
 }
 
-template <int DP, int NI, int NP>
+// LDS of one wave: K (and Q) in planes, the gates, the diagonal blocks of A, then of T
+template <int DP, int NI, bool Q>
 struct DlLds {
-  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, M = PlaneMat<DL_C, 64, NP>::BYTES;
-  static constexpr int BYTES = 2 * KQ + 2 * M + (int)sizeof(DlGates);
-  static_assert(BYTES <= 160 * 1024, "LDS of a CU");
+  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES;
+  static constexpr int BYTES = (Q ? 2 : 1) * KQ + (int)sizeof(DlGates) + 2 * 16 * 20 * 4;
 };
 
-// clear the planes of P and T: their upper triangles (and the parts behind a short sequence) stay zero
-__device__ __forceinline__ void dl_clear(void* p, int bytes) {
-  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-    *reinterpret_cast<f4*>(reinterpret_cast<uint8_t*>(p) + i) = (f4){0.f, 0.f, 0.f, 0.f};
+// T of a chunk as operands: FWD: T (free index i), two per 32 rows; else its transpose (free index j).
+//   FWD  t[0] = {T00, 0}, t[1] = {T10, T11}      else  t[0] = {T00ᵀ, T10ᵀ}, t[1] = {0, T11ᵀ}
+// Rows behind the length are zero in K, so A is zero and T the identity there.
+template <int DP, int NI, bool FWD>
+__device__ __forceinline__ void dl_inverse(const PlaneMat<DL_C, DP, NI>& K, const DlGates& s, float* Ad,
+                                           bf16x8 (*t)[DL_NP]) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  f4 d0 = DL_ZERO, d1 = DL_ZERO, off = DL_ZERO;   // off: rows j of block 0, columns i of block 1
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) {
+    bf16x8 k0[NI], k1[NI];
+    K.row(k0, 0, x);
+    K.row(k1, 16, x);
+    d0 = pl_mm<NI, NI>(k0, k0, d0);
+    d1 = pl_mm<NI, NI>(k1, k1, d1);
+    off = pl_mm<NI, NI>(k0, k1, off);
+  }
+  const double gn0 = s.G[n], gn1 = s.G[16 + n];
+  const float bn1 = s.beta[16 + n];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = 4 * kg + r;
+    const double g0 = s.G[i], g1 = s.G[16 + i];
+    Ad[i * 20 + n] = n < i ? s.beta[i] * dl_exp2(g0 - gn0) * d0[r] : 0.f;
+    Ad[320 + i * 20 + n] = n < i ? s.beta[16 + i] * dl_exp2(g1 - gn1) * d1[r] : 0.f;
+    off[r] *= bn1 * dl_exp2(gn1 - g0);
+  }
+  __syncthreads();
+  {   // lanes of kg 0, 1 solve block 0, the others block 1; T goes where A was, each lane half a column
+    float x[16];
+    dl_solve(Ad + 320 * (kg >> 1), n, x);
+    __syncthreads();
+    float* to = Ad + 320 * (kg >> 1) + n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float lo = x[i], hi = x[8 + i];
+      to[(i + 8 * (kg & 1)) * 20] = kg & 1 ? hi : lo;
+    }
+  }
+  __syncthreads();
+  f4 c0, r1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c0[r] = Ad[(4 * kg + r) * 20 + n];   // column n of T00
+  r1 = *reinterpret_cast<const f4*>(Ad + 320 + n * 20 + 4 * kg);   // row n of T11
+  // T10 = −T11 (A10 T00)
+  bf16x8 fa[DL_NP], fb[DL_NP];
+  pl_split<DL_NP>(off, DL_ZERO, fa);
+  pl_split<DL_NP>(c0, DL_ZERO, fb);
+  const f4 m = pl_mm<DL_NP, DL_NP>(fa, fb, DL_ZERO);   // rows i of block 1, columns j of block 0
+  pl_split<DL_NP>(m, DL_ZERO, fa);
+  pl_split<DL_NP>(r1, DL_ZERO, fb);
+  if (FWD) {
+    const f4 low = -pl_mm<DL_NP, DL_NP>(fa, fb, DL_ZERO), r0 = *reinterpret_cast<const f4*>(Ad + n * 20 + 4 * kg);
+    pl_split<DL_NP>(r0, DL_ZERO, t[0]);
+    pl_split<DL_NP>(low, r1, t[1]);
+  } else {
+    const f4 low = -pl_mm<DL_NP, DL_NP>(fb, fa, DL_ZERO);
+    f4 c1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c1[r] = Ad[320 + (4 * kg + r) * 20 + n];
+    pl_split<DL_NP>(c0, low, t[0]);
+    pl_split<DL_NP>(DL_ZERO, c1, t[1]);
+  }
+}
+
+template <typename IO>
+__device__ __forceinline__ void dl_zero4(IO* p) {
+  typedef IO IO4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<IO4*>(p) = (IO4)(IO)0.f;
+}
+
+// the state of one wave: rows d = 16·u + 4·kg + r, columns col0 + 16·ct + n of a (Dk, cols) fp32 matrix
+template <int CT, int UT>
+__device__ __forceinline__ void dl_state_load(f4 (*S)[UT], const float* src, int Dk, int cols, int col0) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const DlBuf buf = dl_buf(src, src != nullptr ? Dk : 0, cols, cols, 4);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = col0 + 16 * ct + n, v = dl_lane(col < cols, (4 * kg * cols + col) * 4);
+#pragma unroll
+    for (int u = 0; u < UT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[ct][u][r] = DlIO<float>::load1(buf, v, (16 * u + r) * cols * 4);
+  }
+}
+template <int CT, int UT>
+__device__ __forceinline__ void dl_state_store(const f4 (*S)[UT], float* dst, int Dk, int cols, int col0) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const DlBuf buf = dl_buf(dst, Dk, cols, cols, 4);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = col0 + 16 * ct + n, v = dl_lane(col < cols, (4 * kg * cols + col) * 4);
+#pragma unroll
+    for (int u = 0; u < UT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) DlIO<float>::store1(buf, v, (16 * u + r) * cols * 4, S[ct][u][r]);
+  }
 }
 
 // ---------------------------------------------------------------- forward ----
-// One workgroup per (batch row, value head, group of value columns); a wave owns 16 value columns and their part of
-// the state, which stays in its accumulators from the first chunk to the last.  The chunk's K, Q, P, T are shared.
-template <typename IO, int DP, int NP>
-__global__ __launch_bounds__(512) void k_delta_fwd(DeltaArgs a) {
-  constexpr int NI = DlIO<IO>::N, KT = DP / 32;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  using L = DlLds<DP, NI, NP>;
-  const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds}, Q{(__bf16*)(lds + L::KQ)};
-  const PlaneMat<DL_C, 64, NP> P{(__bf16*)(lds + 2 * L::KQ)}, T{(__bf16*)(lds + 2 * L::KQ + L::M)};
-  DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::M);
+// TRANS: only the states a segment leaves, from zero (columns of the value) or from the identity with v = 0 (the columns
+// behind them: the segment's transition)
+template <typename IO, int DP, int CT, bool TRANS>
+__global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
+  constexpr int NI = DlIO<IO>::N, KT = DP / 32, NP = DL_NP;
+  using L = DlLds<DP, NI, false>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::BYTES];
+  const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds};
+  DlGates& s = *(DlGates*)(lds + L::KQ);
+  float* Ad = (float*)(lds + L::KQ + sizeof(DlGates));
 
-  const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = nth >> 6;
-  const int b = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int len = dl_len(a, b), col = (blockIdx.y * nw + wave) * 16 + n;
-  const bool mine = col < a.Dv;
-  const int nC = (a.T + DL_C - 1) / DL_C;
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int seg = blockIdx.x % a.nseg, bhi = blockIdx.x / a.nseg;
+  const int b = bhi / a.Hv, h = bhi % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C;
+  const int vblocks = (a.Dv + 16 * CT - 1) / (16 * CT);
+  const bool unit = TRANS && (int)blockIdx.y >= vblocks;      // columns of the transition
+  const int col0 = (unit ? blockIdx.y - vblocks : blockIdx.y) * 16 * CT, cols = unit ? a.Dk : a.Dv;
   const IO* q = (const IO*)a.q + b * a.qs[0] + hk * a.qs[2];
   const IO* k = (const IO*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const IO* v = (const IO*)a.v + b * a.vs[0] + h * a.vs[2] + col;
-  const int64_t bh = (int64_t)b * a.Hv + h;
-  IO* o = (IO*)a.o + ((int64_t)b * a.T * a.Hv + h) * a.Dv + col;   // row stride Hv * Dv
-  const int64_t os = (int64_t)a.Hv * a.Dv;
+  const IO* v = (const IO*)a.v + b * a.vs[0] + h * a.vs[2];
+  const int64_t bh = bhi, os = (int64_t)a.Hv * a.Dv, size = (int64_t)a.Dk * a.Dv;
+  IO* o = (IO*)a.o + ((int64_t)b * a.T * a.Hv + h) * a.Dv;   // row stride Hv * Dv
 
-  f4 S[2 * KT];
+  const float* init = TRANS ? nullptr : seg > 0 ? a.local + (bh * a.nseg + seg) * size : a.state0 ? a.state0 + bh * size : nullptr;
+  bool zero = init == nullptr && !unit;   // the state is still zero
+  f4 S[CT][2 * KT];
+  dl_state_load<CT, 2 * KT>(S, init, a.Dk, a.Dv, col0);
+  if (unit) {
 #pragma unroll
-  for (int u = 0; u < 2 * KT; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * u + 4 * kg + r;
-      S[u][r] = a.state0 != nullptr && mine && d < a.Dk ? a.state0[(bh * a.Dk + d) * a.Dv + col] : 0.f;
-    }
-  dl_clear(P.p, 2 * L::M);
-
-  for (int t0 = 0; t0 < len; t0 += DL_C) {
-    const int nt = min((len - t0 + 15) / 16, 4);
-    if (a.S0 != nullptr && t0 > 0 && mine) {
-      float* dst = a.S0 + ((bh * (nC - 1) + t0 / DL_C - 1) * a.Dk) * a.Dv + col;
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int u = 0; u < 2 * KT; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * u + 4 * kg + r < a.Dk) dst[(int64_t)(16 * u + 4 * kg + r) * a.Dv] = S[u][r];
-    }
-    float vv[4][4];
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * it + 4 * kg + r;
-        vv[it][r] = mine && t < len ? (float)v[t * a.vs[1]] : 0.f;
-      }
-    __syncthreads();   // the last chunk's reads are done
-    dl_load<IO, DP>(K, k, a.ks[1], t0, len, a.Dk, tid, nth);
-    dl_load<IO, DP>(Q, q, a.qs[1], t0, len, a.Dk, tid, nth);
-    if (wave == 0) dl_gates(s, a, b, h, t0, len);
-    __syncthreads();
-    dl_prep<DP, NI, NP>(K, Q, P, T, s, a.scale, nt, wave, nw);
-
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 x[4] = {zero, zero, zero, zero}, oo[4] = {zero, zero, zero, zero};
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      bf16x8 sb[NP];
-      pl_split<NP>(S[2 * t], S[2 * t + 1], sb);
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-        if (it < nt) {
-          bf16x8 f[NI];
-          K.row(f, 16 * it, t);
-          x[it] = pl_mm<NI, NP>(f, sb, x[it]);
-          Q.row(f, 16 * it, t);
-          oo[it] = pl_mm<NI, NP>(f, sb, oo[it]);
-        }
-    }
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * it + 4 * kg + r;
-        const float gam = s.gam[i];
-        x[it][r] = s.beta[i] * (vv[it][r] - gam * x[it][r]);
-        oo[it][r] *= a.scale * gam;
-      }
-    bf16x8 xb[2][NP];
-    pl_split<NP>(x[0], x[1], xb[0]);
-    pl_split<NP>(x[2], x[3], xb[1]);
-    f4 u[4] = {zero, zero, zero, zero};
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-      if (it < nt) {
-#pragma unroll
-        for (int kb = 0; kb <= it / 2; ++kb) {
-          bf16x8 f[NP];
-          T.row(f, 16 * it, kb);
-          u[it] = pl_mm<NP, NP>(f, xb[kb], u[it]);
-        }
-      }
-    pl_split<NP>(u[0], u[1], xb[0]);
-    pl_split<NP>(u[2], u[3], xb[1]);
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-      if (it < nt) {
-#pragma unroll
-        for (int kb = 0; kb <= it / 2; ++kb) {
-          bf16x8 f[NP];
-          P.row(f, 16 * it, kb);
-          oo[it] = pl_mm<NP, NP>(f, xb[kb], oo[it]);
-        }
-      }
-    if (mine) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = t0 + 16 * it + 4 * kg + r;
-          if (t < a.T) o[t * os] = (IO)oo[it][r];
-          if (a.U != nullptr && t < len) a.U[(bh * a.T + t) * a.Dv + col] = u[it][r];
-        }
-    }
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) u[it][r] *= s.rest[16 * it + 4 * kg + r];
-    pl_split<NP>(u[0], u[1], xb[0]);
-    pl_split<NP>(u[2], u[3], xb[1]);
-    const float last = s.gam[DL_C - 1];
-#pragma unroll
-    for (int t = 0; t < 2 * KT; ++t) {
-      S[t] *= last;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        if (2 * kb < nt) {
-          bf16x8 f[NI];
-          K.col(f, kb, 16 * t);
-          S[t] = pl_mm<NI, NP>(f, xb[kb], S[t]);
-        }
-    }
+        for (int r = 0; r < 4; ++r) S[ct][u][r] = 16 * u + 4 * kg + r == col0 + 16 * ct + n ? 1.f : 0.f;
   }
-  if (mine) {
-    for (int t = (len + DL_C - 1) / DL_C * DL_C + kg; t < a.T; t += 4) o[t * os] = (IO)0.f;
+
+  const int tfrom = seg * a.per * DL_C, tend = a.nseg == 1 ? len : min(len, tfrom + a.per * DL_C);
+  for (int t0 = tfrom; t0 < tend; t0 += DL_C) {
+    const int left = len - t0;   // positions from here on
+    const int rows = min(left, DL_C);
+    const DlBuf vbuf = dl_buf(v + t0 * a.vs[1], unit ? 0 : rows, a.vs[1], a.Dv, DlIO<IO>::SIZE);
+    float vv[CT][8];
 #pragma unroll
-    for (int u = 0; u < 2 * KT; ++u)
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = col0 + 16 * ct + n, at = dl_lane(col < cols, (int)(4 * kg * a.vs[1] + col) * DlIO<IO>::SIZE);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        vv[ct][i] = DlIO<IO>::load1(vbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.vs[1]) * DlIO<IO>::SIZE);
+    }
+    bf16x8 qf[2][KT][NI];
+    if constexpr (!TRANS) {
+      const DlBuf qbuf = dl_buf(q + t0 * a.qs[1], rows, a.qs[1], a.Dk, DlIO<IO>::SIZE);
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) dl_operand<IO>(qf[it][t], qbuf, 16 * it, a.qs[1], 32 * t, a.Dk);
+      if (a.S0 != nullptr && t0 > 0)
+        dl_state_store<CT, 2 * KT>(S, a.S0 + (bh * (nC - 1) + t0 / DL_C - 1) * size, a.Dk, a.Dv, col0);
+    }
+    __syncthreads();
+    dl_load<IO, DP, 64>(K, dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
+    dl_gates(s, a, b, h, t0, len);
+    __syncthreads();
+    bf16x8 T[2][NP], P[2][NP];
+    dl_inverse<DP, NI, true>(K, s, Ad, T);
+    if constexpr (!TRANS) {
+      f4 p00 = DL_ZERO, p01 = DL_ZERO, p11 = DL_ZERO;   // rows j, columns i
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        bf16x8 k0[NI], k1[NI];
+        K.row(k0, 0, t);
+        K.row(k1, 16, t);
+        p00 = pl_mm<NI, NI>(k0, qf[0][t], p00);
+        p01 = pl_mm<NI, NI>(k0, qf[1][t], p01);
+        p11 = pl_mm<NI, NI>(k1, qf[1][t], p11);
+      }
+      const double g0 = s.G[n], g1 = s.G[16 + n];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = 16 * u + 4 * kg + r;
-        if (d < a.Dk) a.state[(bh * a.Dk + d) * a.Dv + col] = S[u][r];
+        const int j = 4 * kg + r;
+        const double h0 = s.G[j], h1 = s.G[16 + j];
+        p00[r] = j <= n ? a.scale * dl_exp2(g0 - h0) * p00[r] : 0.f;
+        p01[r] *= a.scale * dl_exp2(g1 - h0);
+        p11[r] = j <= n ? a.scale * dl_exp2(g1 - h1) * p11[r] : 0.f;
       }
+      pl_split<NP>(p00, DL_ZERO, P[0]);
+      pl_split<NP>(p01, p11, P[1]);
+    }
+    const float last = s.gam[DL_C - 1];
+    const DlBuf obuf = dl_buf(o + t0 * os, min(a.T - t0, DL_C), os, a.Dv, DlIO<IO>::SIZE),
+                ubuf = dl_buf(a.U + (bh * a.T + t0) * a.Dv, a.U != nullptr ? rows : 0, a.Dv, a.Dv, 4);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      f4 x[2] = {DL_ZERO, DL_ZERO}, oo[2] = {DL_ZERO, DL_ZERO};   // oo: rows v, columns i
+      if (!zero) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          bf16x8 sb[NP], f[NI];
+          pl_split<NP>(S[ct][2 * t], S[ct][2 * t + 1], sb);
+          K.row(f, 0, t);
+          x[0] = pl_mm<NI, NP>(f, sb, x[0]);
+          K.row(f, 16, t);
+          x[1] = pl_mm<NI, NP>(f, sb, x[1]);
+          if constexpr (!TRANS) {
+            oo[0] = pl_mm<NP, NI>(sb, qf[0][t], oo[0]);
+            oo[1] = pl_mm<NP, NI>(sb, qf[1][t], oo[1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f4 be = *reinterpret_cast<const f4*>(s.beta + 16 * j + 4 * kg), gam = *reinterpret_cast<const f4*>(s.gam + 16 * j + 4 * kg);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[j][r] = be[r] * (vv[ct][4 * j + r] - gam[r] * x[j][r]);
+      }
+      bf16x8 xb[NP];
+      pl_split<NP>(x[0], x[1], xb);
+      f4 u[2];
+      u[0] = pl_mm<NP, NP>(T[0], xb, DL_ZERO);
+      u[1] = pl_mm<NP, NP>(T[1], xb, DL_ZERO);
+      if constexpr (!TRANS) {
+        pl_split<NP>(u[0], u[1], xb);
+        const int row = col0 + 16 * ct + 4 * kg, at = dl_lane(row < a.Dv, (int)(n * os + row) * DlIO<IO>::SIZE);
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          oo[it] *= a.scale * s.gam[16 * it + n];
+          oo[it] = pl_mm<NP, NP>(xb, P[it], oo[it]);
+          DlIO<IO>::store4(obuf, at, (int)(16 * it * os) * DlIO<IO>::SIZE, oo[it]);
+        }
+        if (a.U != nullptr) {
+          const int col = col0 + 16 * ct + n, up = dl_lane(col < cols, (4 * kg * a.Dv + col) * 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            DlIO<float>::store1(ubuf, up, (16 * (i >> 2) + (i & 3)) * a.Dv * 4, u[i >> 2][i & 3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) u[j] *= *reinterpret_cast<const f4*>(s.rest + 16 * j + 4 * kg);
+      pl_split<NP>(u[0], u[1], xb);
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) {
+        bf16x8 f[NI];
+        K.col(f, 0, 16 * t);
+        S[ct][t] = pl_mm<NI, NP>(f, xb, S[ct][t] * last);
+      }
+    }
+    zero = false;
+  }
+  if constexpr (TRANS) {
+    float* dst = unit ? a.trans + (bh * a.nseg + seg) * a.Dk * a.Dk : a.local + (bh * a.nseg + seg) * size;
+    dl_state_store<CT, 2 * KT>(S, dst, a.Dk, cols, col0);
+  } else {
+    // outputs behind the length, in this segment's part
+    const int tto = seg == a.nseg - 1 ? a.T : min(a.T, tfrom + a.per * DL_C);
+    const int tdone = max(tfrom, (len + DL_C - 1) / DL_C * DL_C);
+    for (int t = tdone + n; t < tto; t += 16)
+      for (int c = col0 + 4 * kg; c < min(a.Dv, col0 + 16 * CT); c += 16) dl_zero4(o + t * os + c);
+    if (seg == a.nseg - 1) dl_state_store<CT, 2 * KT>(S, a.state + bh * size, a.Dk, a.Dv, col0);
   }
 }
 
 // ------------------------------------------------------- backward, the scan ----
-// The same split, chunks last to first; leaves dX, dV, the gradients after each chunk but the last, and dstate0.
-template <typename IO, int DP, int NP>
-__global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
-  constexpr int NI = DlIO<IO>::N, KT = DP / 32;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  using L = DlLds<DP, NI, NP>;
+// The same split, chunks last to first; leaves dX, dV, the gradients after each chunk but the last, and dstate0.  LOCAL: only
+// the gradient that a segment leaves when it starts from zero.
+template <typename IO, int DP, int CT, bool LOCAL>
+__global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
+  constexpr int NI = DlIO<IO>::N, KT = DP / 32, NP = DL_NP;
+  using L = DlLds<DP, NI, true>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::BYTES];
   const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds}, Q{(__bf16*)(lds + L::KQ)};
-  const PlaneMat<DL_C, 64, NP> P{(__bf16*)(lds + 2 * L::KQ)}, T{(__bf16*)(lds + 2 * L::KQ + L::M)};
-  DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::M);
+  DlGates& s = *(DlGates*)(lds + 2 * L::KQ);
+  float* Ad = (float*)(lds + 2 * L::KQ + sizeof(DlGates));
 
-  const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = nth >> 6;
-  const int b = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int len = dl_len(a, b), col = (blockIdx.y * nw + wave) * 16 + n;
-  const bool mine = col < a.Dv;
-  const int nC = (a.T + DL_C - 1) / DL_C;
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int seg = blockIdx.x % a.nseg, bhi = blockIdx.x / a.nseg;
+  const int b = bhi / a.Hv, h = bhi % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C, col0 = blockIdx.y * 16 * CT;
   const IO* q = (const IO*)a.q + b * a.qs[0] + hk * a.qs[2];
   const IO* k = (const IO*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const IO* d_o = (const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + col;
-  const int64_t bh = (int64_t)b * a.Hv + h;
-  IO* dv = (IO*)a.dv + ((int64_t)b * a.T * a.Hv + h) * a.Dv + col;
-  const int64_t os = (int64_t)a.Hv * a.Dv;
+  const IO* d_o = (const IO*)a.d_o + b * a.dos[0] + h * a.dos[2];
+  const int64_t bh = bhi, os = (int64_t)a.Hv * a.Dv, size = (int64_t)a.Dk * a.Dv;
+  IO* dv = (IO*)a.dv + ((int64_t)b * a.T * a.Hv + h) * a.Dv;
 
-  f4 S[2 * KT];
-#pragma unroll
-  for (int u = 0; u < 2 * KT; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * u + 4 * kg + r;
-      S[u][r] = a.dstate != nullptr && mine && d < a.Dk ? a.dstate[(bh * a.Dk + d) * a.Dv + col] : 0.f;
-    }
-  dl_clear(P.p, 2 * L::M);
+  const float* init = LOCAL                ? nullptr
+                      : seg < a.nseg - 1 ? a.local + (bh * a.nseg + seg) * size
+                      : a.dstate         ? a.dstate + bh * size
+                                         : nullptr;
+  bool zero = init == nullptr;
+  f4 S[CT][2 * KT];
+  dl_state_load<CT, 2 * KT>(S, init, a.Dk, a.Dv, col0);
 
-  const int nc = (len + DL_C - 1) / DL_C;
-  for (int c = nc - 1; c >= 0; --c) {
-    const int t0 = c * DL_C, nt = min((len - t0 + 15) / 16, 4);
-    if (c < nc - 1 && mine) {
-      float* dst = a.dS + ((bh * (nC - 1) + c) * a.Dk) * a.Dv + col;
+  const int nc = (len + DL_C - 1) / DL_C, cfrom = seg * a.per, cend = a.nseg == 1 ? nc : min(nc, cfrom + a.per);
+  for (int c = cend - 1; c >= cfrom; --c) {
+    const int t0 = c * DL_C, left = len - t0;
+    if (!LOCAL && c < nC - 1) dl_state_store<CT, 2 * KT>(S, a.dS + (bh * (nC - 1) + c) * size, a.Dk, a.Dv, col0);
+    const int rows = min(left, DL_C);
+    const DlBuf gbuf = dl_buf(d_o + t0 * a.dos[1], rows, a.dos[1], a.Dv, DlIO<IO>::SIZE);
+    f4 go[CT][2];
 #pragma unroll
-      for (int u = 0; u < 2 * KT; ++u)
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = col0 + 16 * ct + n, at = dl_lane(col < a.Dv, (int)(4 * kg * a.dos[1] + col) * DlIO<IO>::SIZE);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * u + 4 * kg + r < a.Dk) dst[(int64_t)(16 * u + 4 * kg + r) * a.Dv] = S[u][r];
+      for (int i = 0; i < 8; ++i)
+        go[ct][i >> 2][i & 3] = DlIO<IO>::load1(gbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.dos[1]) * DlIO<IO>::SIZE);
     }
-    f4 go[4];
+    __syncthreads();
+    dl_load<IO, DP, 64>(K, dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
+    dl_load<IO, DP, 64>(Q, dl_buf(q + t0 * a.qs[1], rows, a.qs[1], a.Dk, DlIO<IO>::SIZE), a.qs[1], a.Dk, lane);
+    dl_gates(s, a, b, h, t0, len);
+    __syncthreads();
+    bf16x8 T[2][NP], P[2][NP];
+    dl_inverse<DP, NI, false>(K, s, Ad, T);
+    {
+      f4 p00 = DL_ZERO, p10 = DL_ZERO, p11 = DL_ZERO;   // rows i, columns j
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+      for (int t = 0; t < KT; ++t) {
+        bf16x8 k0[NI], k1[NI], f[NI];
+        K.row(k0, 0, t);
+        K.row(k1, 16, t);
+        Q.row(f, 0, t);
+        p00 = pl_mm<NI, NI>(f, k0, p00);
+        Q.row(f, 16, t);
+        p10 = pl_mm<NI, NI>(f, k0, p10);
+        p11 = pl_mm<NI, NI>(f, k1, p11);
+      }
+      const double g0 = s.G[n], g1 = s.G[16 + n];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * it + 4 * kg + r;
-        go[it][r] = mine && t < len ? (float)d_o[t * a.dos[1]] : 0.f;
+        const int i = 4 * kg + r;
+        const double h0 = s.G[i], h1 = s.G[16 + i];
+        p00[r] = n <= i ? a.scale * dl_exp2(h0 - g0) * p00[r] : 0.f;
+        p10[r] *= a.scale * dl_exp2(h1 - g0);
+        p11[r] = n <= i ? a.scale * dl_exp2(h1 - g1) * p11[r] : 0.f;
       }
-    __syncthreads();
-    dl_load<IO, DP>(K, k, a.ks[1], t0, len, a.Dk, tid, nth);
-    dl_load<IO, DP>(Q, q, a.qs[1], t0, len, a.Dk, tid, nth);
-    if (wave == 0) dl_gates(s, a, b, h, t0, len);
-    // parts that a shorter last chunk left untouched hold no older chunk's values: it comes first
-    __syncthreads();
-    dl_prep<DP, NI, NP>(K, Q, P, T, s, a.scale, nt, wave, nw);
+      pl_split<NP>(p00, p10, P[0]);
+      pl_split<NP>(DL_ZERO, p11, P[1]);
+    }
+    const float last = s.gam[DL_C - 1];
+    const DlBuf dvbuf = dl_buf(dv + t0 * os, min(a.T - t0, DL_C), os, a.Dv, DlIO<IO>::SIZE),
+                xbuf = dl_buf(a.dX + (bh * a.T + t0) * a.Dv, rows, a.Dv, a.Dv, 4);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      f4 du[2] = {DL_ZERO, DL_ZERO};
+      if (!zero) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          bf16x8 sb[NP], f[NI];
+          pl_split<NP>(S[ct][2 * t], S[ct][2 * t + 1], sb);
+          K.row(f, 0, t);
+          du[0] = pl_mm<NI, NP>(f, sb, du[0]);
+          K.row(f, 16, t);
+          du[1] = pl_mm<NI, NP>(f, sb, du[1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) du[j] *= *reinterpret_cast<const f4*>(s.rest + 16 * j + 4 * kg);
+      }
+      bf16x8 gb[NI], xb[NP];
+      pl_split<NI>(go[ct][0], go[ct][1], gb);
+      du[0] = pl_mm<NP, NI>(P[0], gb, du[0]);
+      du[1] = pl_mm<NP, NI>(P[1], gb, du[1]);
+      pl_split<NP>(du[0], du[1], xb);
+      f4 dx[2];
+      dx[0] = pl_mm<NP, NP>(T[0], xb, DL_ZERO);
+      dx[1] = pl_mm<NP, NP>(T[1], xb, DL_ZERO);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f4 be = *reinterpret_cast<const f4*>(s.beta + 16 * j + 4 * kg), gam = *reinterpret_cast<const f4*>(s.gam + 16 * j + 4 * kg);
+        if constexpr (!LOCAL) {
+          const int col = col0 + 16 * ct + n, at = dl_lane(col < a.Dv, (int)(4 * kg * os + col) * DlIO<IO>::SIZE),
+                    up = dl_lane(col < a.Dv, (4 * kg * a.Dv + col) * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            DlIO<IO>::store1(dvbuf, at, (int)((16 * j + r) * os) * DlIO<IO>::SIZE, be[r] * dx[j][r]);
+            DlIO<float>::store1(xbuf, up, (16 * j + r) * a.Dv * 4, dx[j][r]);
+          }
+        }
+        go[ct][j] *= a.scale * gam;
+        dx[j] *= -be * gam;
+      }
+      bf16x8 hb[NP];
+      pl_split<NP>(go[ct][0], go[ct][1], hb);
+      pl_split<NP>(dx[0], dx[1], xb);
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) {
+        bf16x8 f[NI];
+        Q.col(f, 0, 16 * t);
+        S[ct][t] = pl_mm<NI, NP>(f, hb, S[ct][t] * last);
+        K.col(f, 0, 16 * t);
+        S[ct][t] = pl_mm<NI, NP>(f, xb, S[ct][t]);
+      }
+    }
+    zero = false;
+  }
+  if (!LOCAL) {
+    const int tto = seg == a.nseg - 1 ? a.T : min(a.T, (cfrom + a.per) * DL_C);
+    for (int t = max(cfrom, nc) * DL_C + kg; t < tto; t += 4)
+      for (int c = col0 + n; c < min(a.Dv, col0 + 16 * CT); c += 16) dv[t * os + c] = (IO)0.f;
+  }
+  float* dst = LOCAL ? a.local + (bh * a.nseg + seg) * size : seg == 0 && a.dstate0 ? a.dstate0 + bh * size : nullptr;
+  if (dst != nullptr) dl_state_store<CT, 2 * KT>(S, dst, a.Dk, a.Dv, col0);
+}
 
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 du[4] = {zero, zero, zero, zero};
+// ------------------------------------------------------- segments ----
+// The state a segment starts from: S_{s+1} = trans_s S_s + local_s, put in local's place; backwards the gradient it starts
+// from: dS_{s-1} = trans_sᵀ dS_s + local_s.  One workgroup per (row, head, 16 value columns), a wave per 16 rows of the
+// state: its rows of trans straight from memory (the next segment's while this one's products run), the state
+// from LDS in planes, in two buffers, so that a segment costs one barrier.
+template <int DP, bool BACK>
+__global__ __launch_bounds__(4 * DP) void k_delta_join(DeltaArgs a) {
+  constexpr int NP = DL_NP, KT = DP / 32;
+  using M = PlaneMat<16, DP, NP>;   // row: value column; columns: the state's rows
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][M::BYTES];
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d0 = 16 * wave, col = blockIdx.y * 16 + n;
+  const int64_t bh = blockIdx.x, size = (int64_t)a.Dk * a.Dv;
+  const float* first = BACK ? a.dstate : a.state0;
+  const int at = dl_lane(col < a.Dv, ((d0 + 4 * kg) * a.Dv + col) * 4);
+  auto state = [&](const float* p) { return dl_buf(p, p != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4); };
+  f4 S;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) S[r] = DlIO<float>::load1(state(first != nullptr ? first + bh * size : nullptr), at, r * a.Dv * 4);
+
+  f4 w[KT][2], loc;   // this wave's rows of trans (BACK: columns), and of local
+  auto fetch = [&](int seg) __attribute__((always_inline)) {
+    const DlBuf tb = dl_buf(a.trans + (bh * a.nseg + seg) * a.Dk * a.Dk, a.Dk, a.Dk, a.Dk, 4);
+    const int v = BACK ? dl_lane(d0 + n < a.Dk, (4 * kg * a.Dk + d0 + n) * 4) : (n * a.Dk + 4 * kg) * 4;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int e = 32 * t + 16 * q;
+        if (BACK) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[t][q][r] = DlIO<float>::load1(tb, v, (e + r) * a.Dk * 4);
+        } else {
+          w[t][q] = DlIO<float>::load4(tb, dl_lane(e + 4 * kg < a.Dk, v), (d0 * a.Dk + e) * 4);
+        }
+      }
+    const DlBuf lb = state(a.local + (bh * a.nseg + seg) * size);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) loc[r] = DlIO<float>::load1(lb, at, r * a.Dv * 4);
+  };
+  fetch(BACK ? a.nseg - 1 : 0);
+  for (int i = 0; i < a.nseg; ++i) {
+    const int seg = BACK ? a.nseg - 1 - i : i;
+    const DlBuf lb = state(a.local + (bh * a.nseg + seg) * size);
+    const f4 add = loc;
+    bf16x8 f[KT][NP];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) pl_split<NP>(w[t][0], w[t][1], f[t]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) DlIO<float>::store1(lb, at, r * a.Dv * 4, S[r]);
+    if (i == a.nseg - 1) break;
+    fetch(BACK ? seg - 1 : seg + 1);
+    const M m{(__bf16*)lds[i & 1]};
+    bf16x8 p[NP];
+    pl_split<NP>(S, DL_ZERO, p);
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const pl_s8 v = __builtin_bit_cast(pl_s8, p[q]);
+      *reinterpret_cast<pl_s4*>(m.p + q * M::PLANE + n * M::LD + pl_place(d0 + 4 * kg)) = (pl_s4){v[0], v[1], v[2], v[3]};
+    }
+    __syncthreads();
+    S = add;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      bf16x8 sb[NP];
-      pl_split<NP>(S[2 * t], S[2 * t + 1], sb);
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-        if (it < nt) {
-          bf16x8 f[NI];
-          K.row(f, 16 * it, t);
-          du[it] = pl_mm<NI, NP>(f, sb, du[it]);
-        }
-    }
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) du[it][r] *= s.rest[16 * it + 4 * kg + r];
-    {
-      bf16x8 gb[2][NI];
-      pl_split<NI>(go[0], go[1], gb[0]);
-      pl_split<NI>(go[2], go[3], gb[1]);
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-        if (it < nt) {
-#pragma unroll
-          for (int kb = it / 2; kb < 2; ++kb)
-            if (2 * kb < nt) {
-              bf16x8 f[NP];
-              P.col(f, kb, 16 * it);
-              du[it] = pl_mm<NP, NI>(f, gb[kb], du[it]);
-            }
-        }
-    }
-    bf16x8 xb[2][NP];
-    pl_split<NP>(du[0], du[1], xb[0]);
-    pl_split<NP>(du[2], du[3], xb[1]);
-    f4 dx[4] = {zero, zero, zero, zero};
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-      if (it < nt) {
-#pragma unroll
-        for (int kb = it / 2; kb < 2; ++kb)
-          if (2 * kb < nt) {
-            bf16x8 f[NP];
-            T.col(f, kb, 16 * it);
-            dx[it] = pl_mm<NP, NP>(f, xb[kb], dx[it]);
-          }
-      }
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * it + 4 * kg + r, t = t0 + i;
-        if (mine) {
-          if (t < a.T) dv[t * os] = (IO)(s.beta[i] * dx[it][r]);
-          if (t < len) a.dX[(bh * a.T + t) * a.Dv + col] = dx[it][r];
-        }
-        const float gam = s.gam[i];
-        go[it][r] *= a.scale * gam;
-        dx[it][r] *= -s.beta[i] * gam;
-      }
-    const float last = s.gam[DL_C - 1];
-    bf16x8 gb[2][NP];
-    pl_split<NP>(go[0], go[1], gb[0]);
-    pl_split<NP>(go[2], go[3], gb[1]);
-    pl_split<NP>(dx[0], dx[1], xb[0]);
-    pl_split<NP>(dx[2], dx[3], xb[1]);
-#pragma unroll
-    for (int t = 0; t < 2 * KT; ++t) {
-      S[t] *= last;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        if (2 * kb < nt) {
-          bf16x8 f[NI];
-          Q.col(f, kb, 16 * t);
-          S[t] = pl_mm<NI, NP>(f, gb[kb], S[t]);
-          K.col(f, kb, 16 * t);
-          S[t] = pl_mm<NI, NP>(f, xb[kb], S[t]);
-        }
-    }
-  }
-  if (mine) {
-    for (int t = nc * DL_C + kg; t < a.T; t += 4) dv[t * os] = (IO)0.f;
-    if (a.dstate0 != nullptr) {
-#pragma unroll
-      for (int u = 0; u < 2 * KT; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = 16 * u + 4 * kg + r;
-          if (d < a.Dk) a.dstate0[(bh * a.Dk + d) * a.Dv + col] = S[u][r];
-        }
+      m.row(p, 0, t);
+      S = pl_mm<NP, NP>(f[t], p, S);
     }
   }
 }
 
 // -------------------------------------- backward, the rest of a chunk's gradients ----
-// One workgroup of four waves per (batch row, key head, chunk), independent of the others; the value heads of a key head
-// one after the other, their dq and dk summed in registers (no atomics: the same result every time).  Wave w owns the
-// chunk's rows 16w .. 16w + 15.  First the contractions over the value columns, staged in blocks of 32,
+// One workgroup per (row, key head, chunk), independent of the others; the value heads of a key head one after the
+// other, their dq and dk summed in registers (no atomics: the same result every time).  Two waves, one per 16 rows; four
+// where there are more than 64 key columns, half of them each (wave w: rows of tile w & 1, half w >> 1).  The contractions over the value columns,
 //     dP = dO Uᵀ,  dA = −dX Uᵀ,  E1 = dO Sᵀ,  E2 = dX Sᵀ,  E3 = U dS'ᵀ,
-// then K and Q take the staging area's place for  dQ = scale e^G E1 + M1 K,  dK = M1ᵀ Q + (M2 + M2ᵀ) K − b e^G E2 +
-// D_end E3  with M1 = scale D dP, M2 = b D dA, and for the scalars' gradients.
-template <int DP, int NI, int NP>
+// read their operands straight from memory (rows of contiguous values are what an operand's lanes want); then
+//     dQ = scale e^G E1 + M1 K,  dK = M1ᵀ Q + (M2 + M2ᵀ) K − b e^G E2 + D_end E3,  M1 = scale D dP,  M2 = b D dA
+// with M1 and M2 passed through LDS, and the scalars' gradients from row and column sums.
+template <int DP, int NI>
 struct DlGradLds {
-  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, M = PlaneMat<DL_C, 64, NP>::BYTES;
-  static constexpr int GO = PlaneMat<DL_C, 32, NI>::BYTES, X = PlaneMat<DL_C, 32, NP>::BYTES,
-                       ST = PlaneMat<DP, 32, NP>::BYTES;
-  static constexpr int ONE = GO + 2 * X + 2 * ST, TWO = 2 * KQ + 2 * M;
-  static constexpr int AREA = ONE > TWO ? ONE : TWO;
-  static constexpr int SUMS = (4 * 64 + 6 * 64) * 4;
-  static constexpr int BYTES = AREA + (int)sizeof(DlGates) + SUMS;
-  static_assert(BYTES <= 160 * 1024, "LDS of a CU");
+  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, M = PlaneMat<DL_C, 32, DL_NP>::BYTES;
+  static constexpr int HALVES = DP > 64 ? 2 : 1, THREADS = 128 * HALVES;
+  static constexpr int SUMS = (2 * 32 + 3 * HALVES * 32 + 3 * 32 + 8) * 4;
+  static constexpr int BYTES = 2 * KQ + 2 * M + (int)sizeof(DlGates) + SUMS;
 };
-
-// rows r < rows of a (.., Dv) fp32 matrix, columns c0 .. c0 + 31, into planes; zeros elsewhere.  With `with`: also the
-// sum of products with that matrix.
-template <int R, int NP>
-__device__ __forceinline__ float dl_stage(const PlaneMat<R, 32, NP>& m, const float* src, int rows, int c0, int Dv,
-                                          const float* with) {
-  float sum = 0.f;
-  for (int e = threadIdx.x; e < R * 4; e += blockDim.x) {
-    const int r = e >> 2, c = (e & 3) * 8;
-    bf16x8 f[NP] = {};
-    if (r < rows && c0 + c < Dv) {
-      const float* s = src + (int64_t)r * Dv + c0 + c;
-      const f4 lo = *reinterpret_cast<const f4*>(s), hi = *reinterpret_cast<const f4*>(s + 4);
-      pl_split<NP>(lo, hi, f);
-      if (with != nullptr) {
-        const float* w = with + (int64_t)r * Dv + c0 + c;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(lo[i], w[i], __builtin_fmaf(hi[i], w[4 + i], sum));
-      }
-    }
-    m.put8(r, c, f);
-  }
-  return sum;
-}
 
 __device__ __forceinline__ float dl_sum16(float x) {   // over the 16 lanes of a group
 #pragma unroll
@@ -586,22 +713,22 @@ __device__ __forceinline__ float dl_get(const PlaneMat<R, C, N>& m, int r, int c
   return x;
 }
 
-template <typename IO, int DP, int NP>
-__global__ __launch_bounds__(256) void k_delta_grads(DeltaArgs a) {
-  constexpr int NI = DlIO<IO>::N, UT = DP / 16;
+template <typename IO, int DP>
+__global__ __launch_bounds__(DP > 64 ? 256 : 128, 2) void k_delta_grads(DeltaArgs a) {
+  using L = DlGradLds<DP, DlIO<IO>::N>;
+  constexpr int NI = DlIO<IO>::N, NP = DL_NP, HALVES = L::HALVES, THREADS = L::THREADS;
+  constexpr int UT = DP / 16 / HALVES;   // key tiles of a wave
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  using L = DlGradLds<DP, NI, NP>;
-  const PlaneMat<DL_C, 32, NI> GO{(__bf16*)lds};
-  const PlaneMat<DL_C, 32, NP> DX{(__bf16*)(lds + L::GO)}, UU{(__bf16*)(lds + L::GO + L::X)};
-  const PlaneMat<DP, 32, NP> SS{(__bf16*)(lds + L::GO + 2 * L::X)}, DS{(__bf16*)(lds + L::GO + 2 * L::X + L::ST)};
   const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds}, Q{(__bf16*)(lds + L::KQ)};
-  const PlaneMat<DL_C, 64, NP> M1{(__bf16*)(lds + 2 * L::KQ)}, M2{(__bf16*)(lds + 2 * L::KQ + L::M)};
-  DlGates& s = *(DlGates*)(lds + L::AREA);
-  float* colsum = (float*)(lds + L::AREA + sizeof(DlGates));   // [4 waves][64]
-  float* rows = colsum + 4 * 64;                               // [6][64]
+  const PlaneMat<DL_C, 32, NP> M1{(__bf16*)(lds + 2 * L::KQ)}, M2{(__bf16*)(lds + 2 * L::KQ + L::M)};
+  DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::M);
+  float* colsum = (float*)(lds + 2 * L::KQ + 2 * L::M + sizeof(DlGates));   // [2 row tiles][32]
+  float* part = colsum + 2 * 32;      // [3][halves][32]: q·E1, k·E2, k·E3
+  float* rows = part + 3 * HALVES * 32;    // [3][32]: row sums of M, of the terms of dbeta, dX·V
+  float* dots = rows + 3 * 32;        // [4] sums of S·dS'
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), it = wave & 1, half = wave >> 1;
   const int group = a.Hv / a.Hk, b = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk, c = blockIdx.y, t0 = c * DL_C;
   const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C, nc = (len + DL_C - 1) / DL_C;
   IO* dq = (IO*)a.dq + ((int64_t)b * a.T * a.Hk + hk) * a.Dk;
@@ -610,11 +737,11 @@ __global__ __launch_bounds__(256) void k_delta_grads(DeltaArgs a) {
 
   if (c >= nc) {
     const int end = min(a.T, t0 + DL_C);
-    for (int e = tid; e < (end - t0) * a.Dk; e += 256) {
+    for (int e = tid; e < (end - t0) * a.Dk; e += THREADS) {
       dq[(t0 + e / a.Dk) * ks + e % a.Dk] = (IO)0.f;
       dk[(t0 + e / a.Dk) * ks + e % a.Dk] = (IO)0.f;
     }
-    for (int e = tid; e < (end - t0) * group; e += 256) {
+    for (int e = tid; e < (end - t0) * group; e += THREADS) {
       const int64_t at = ((int64_t)b * a.T + t0 + e / group) * a.Hv + hk * group + e % group;
       a.dg[at] = 0.f;
       a.dbeta[at] = 0.f;
@@ -622,205 +749,212 @@ __global__ __launch_bounds__(256) void k_delta_grads(DeltaArgs a) {
     return;
   }
 
-  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+  const int left = min(len - t0, DL_C), d0 = half * 64;
+  dl_load<IO, DP, THREADS>(K, dl_buf((const IO*)a.k + b * a.ks[0] + hk * a.ks[2] + t0 * a.ks[1], left, a.ks[1], a.Dk, DlIO<IO>::SIZE),
+                       a.ks[1], a.Dk, tid);
+  dl_load<IO, DP, THREADS>(Q, dl_buf((const IO*)a.q + b * a.qs[0] + hk * a.qs[2] + t0 * a.qs[1], left, a.qs[1], a.Dk, DlIO<IO>::SIZE),
+                       a.qs[1], a.Dk, tid);
   f4 gq[UT], gk[UT];
 #pragma unroll
-  for (int u = 0; u < UT; ++u) gq[u] = gk[u] = zero;
+  for (int u = 0; u < UT; ++u) gq[u] = gk[u] = DL_ZERO;
+  const bool live = 16 * it < left;   // this wave's rows hold any position
 
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
-    const int64_t bh = (int64_t)b * a.Hv + h, state = (int64_t)a.Dk * a.Dv;
-    const float* S0 = c > 0 ? a.S0 + (bh * (nC - 1) + c - 1) * state : a.state0 ? a.state0 + bh * state : nullptr;
-    const float* dS = c < nc - 1 ? a.dS + (bh * (nC - 1) + c) * state : a.dstate ? a.dstate + bh * state : nullptr;
+    const int64_t bh = (int64_t)b * a.Hv + h, size = (int64_t)a.Dk * a.Dv;
+    const float* S0 = c > 0 ? a.S0 + (bh * (nC - 1) + c - 1) * size : a.state0 ? a.state0 + bh * size : nullptr;
+    const float* dS = c < nc - 1 ? a.dS + (bh * (nC - 1) + c) * size : a.dstate ? a.dstate + bh * size : nullptr;
+    // a length that ends on this chunk: what stands behind it is the gradient handed in
     const float* U = a.U + (bh * a.T + t0) * a.Dv;
     const float* dX = a.dX + (bh * a.T + t0) * a.Dv;
-    const IO* d_o = (const IO*)a.d_o + b * a.dos[0] + h * a.dos[2];
+    const DlBuf gbuf = dl_buf((const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + t0 * a.dos[1], left, a.dos[1], a.Dv,
+                              DlIO<IO>::SIZE),
+                xbuf = dl_buf(dX, left, a.Dv, a.Dv, 4), ubuf = dl_buf(U, left, a.Dv, a.Dv, 4),
+                sbuf = dl_buf(S0, a.Dk, a.Dv, a.Dv, 4), ebuf = dl_buf(dS, a.Dk, a.Dv, a.Dv, 4);
     const IO* v = (const IO*)a.v + b * a.vs[0] + h * a.vs[2];
-    const int left = min(len - t0, DL_C);
 
-    f4 dp[4] = {zero, zero, zero, zero}, da[4] = {zero, zero, zero, zero}, e1[UT], e2[UT], e3[UT];
+    if (wave == 0) dl_gates(s, a, b, h, t0, len);
+    // dP, dA: the diagonal tile, and the tile below it (of the second row tile)
+    f4 dp = DL_ZERO, da = DL_ZERO, dp0 = DL_ZERO, da0 = DL_ZERO, e1[UT], e2[UT], e3[UT];
 #pragma unroll
-    for (int u = 0; u < UT; ++u) e1[u] = e2[u] = e3[u] = zero;
-    float both = 0.f;
-    for (int c0 = 0; c0 < a.Dv; c0 += 32) {
-      __syncthreads();
-      for (int e = tid; e < DL_C * 4; e += 256) {
-        const int r = e >> 2, cc = (e & 3) * 8;
-        bf16x8 f[NI] = {};
-        if (r < left && c0 + cc < a.Dv) DlIO<IO>::load8(d_o + (int64_t)(t0 + r) * a.dos[1] + c0 + cc, f);
-        GO.put8(r, cc, f);
-      }
-      dl_stage<DL_C, NP>(DX, dX, left, c0, a.Dv, nullptr);
-      dl_stage<DL_C, NP>(UU, U, left, c0, a.Dv, nullptr);
-      if (S0 != nullptr) both += dl_stage<DP, NP>(SS, S0, a.Dk, c0, a.Dv, dS);
-      if (dS != nullptr) dl_stage<DP, NP>(DS, dS, a.Dk, c0, a.Dv, nullptr);
-      __syncthreads();
-      bf16x8 go[NI], gx[NP], y[NP];
-      GO.row(go, 16 * wave, 0);
-      DX.row(gx, 16 * wave, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= wave) {
-          UU.row(y, 16 * j, 0);
-          dp[j] = pl_mm<NI, NP>(go, y, dp[j]);
-          da[j] = pl_mm<NP, NP>(gx, y, da[j]);
+    for (int u = 0; u < UT; ++u) e1[u] = e2[u] = e3[u] = DL_ZERO;
+    if (live) {
+      for (int c0 = 0; c0 < a.Dv; c0 += 32) {
+        bf16x8 go[NI], gx[NP], uu[NP], y[NP];
+        dl_operand<IO>(go, gbuf, 16 * it, a.dos[1], c0, a.Dv);
+        dl_operand<float>(gx, xbuf, 16 * it, a.Dv, c0, a.Dv);
+        dl_operand<float>(uu, ubuf, 16 * it, a.Dv, c0, a.Dv);
+        dp = pl_mm<NI, NP>(go, uu, dp);
+        da = pl_mm<NP, NP>(gx, uu, da);
+        if (it == 1) {
+          dl_operand<float>(y, ubuf, 0, a.Dv, c0, a.Dv);
+          dp0 = pl_mm<NI, NP>(go, y, dp0);
+          da0 = pl_mm<NP, NP>(gx, y, da0);
         }
-      if (S0 != nullptr) {
+        if (S0 != nullptr) {
 #pragma unroll
-        for (int u = 0; u < UT; ++u) {
-          SS.row(y, 16 * u, 0);
-          e1[u] = pl_mm<NI, NP>(go, y, e1[u]);
-          e2[u] = pl_mm<NP, NP>(gx, y, e2[u]);
+          for (int u = 0; u < UT; ++u) {
+            dl_operand<float>(y, sbuf, d0 + 16 * u, a.Dv, c0, a.Dv);
+            e1[u] = pl_mm<NI, NP>(go, y, e1[u]);
+            e2[u] = pl_mm<NP, NP>(gx, y, e2[u]);
+          }
         }
-      }
-      if (dS != nullptr) {
-        UU.row(gx, 16 * wave, 0);
+        if (dS != nullptr) {
 #pragma unroll
-        for (int u = 0; u < UT; ++u) {
-          DS.row(y, 16 * u, 0);
-          e3[u] = pl_mm<NP, NP>(gx, y, e3[u]);
+          for (int u = 0; u < UT; ++u) {
+            dl_operand<float>(y, ebuf, d0 + 16 * u, a.Dv, c0, a.Dv);
+            e3[u] = pl_mm<NP, NP>(uu, y, e3[u]);
+          }
         }
       }
     }
-    // dX · V of each row: four lanes a row
+    // dX · V of each row: four (eight) threads a row
     {
-      const int r = tid >> 2;
+      constexpr int PER = THREADS / 32;
+      const int r = tid / PER;
       float x = 0.f;
       if (r < left)
-        for (int cc = (tid & 3) * 4; cc < a.Dv; cc += 16)
+        for (int cc = tid % PER * 4; cc < a.Dv; cc += 4 * PER)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             x = __builtin_fmaf(dX[(int64_t)r * a.Dv + cc + i], (float)v[(int64_t)(t0 + r) * a.vs[1] + cc + i], x);
-      x += __shfl_xor(x, 1);
-      x += __shfl_xor(x, 2);
-      if ((tid & 3) == 0) rows[5 * 64 + r] = x;
+#pragma unroll
+      for (int o = 1; o < PER; o <<= 1) x += __shfl_xor(x, o);
+      if (tid % PER == 0) rows[2 * 32 + r] = x;
+    }
+    float both = 0.f;
+    if (S0 != nullptr && dS != nullptr) {
+      for (int e = tid * 4; e < a.Dk * a.Dv; e += 4 * THREADS) {
+        const f4 x = *reinterpret_cast<const f4*>(S0 + e), y = *reinterpret_cast<const f4*>(dS + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) both = __builtin_fmaf(x[i], y[i], both);
+      }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) both += __shfl_xor(both, o);
     }
-    __syncthreads();   // the staged blocks are read: K and Q take their place
-    dl_load<IO, DP>(K, (const IO*)a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], t0, len, a.Dk, tid, 256);
-    dl_load<IO, DP>(Q, (const IO*)a.q + b * a.qs[0] + hk * a.qs[2], a.qs[1], t0, len, a.Dk, tid, 256);
-    if (wave == 0) dl_gates(s, a, b, h, t0, len);
-    __syncthreads();
-    float rm[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
+    if (lane == 0) dots[wave] = both;
+    __syncthreads();   // K, Q, gates
+    if (half == 0) {
+      float rm[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f4 kk = zero, qk = zero;
-      if (j <= wave) {
+      for (int j = 0; j < 2; ++j) {
+        f4 kk = DL_ZERO, qk = DL_ZERO;
+        if (j <= it && live) {
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t) {
-          bf16x8 ki[NI], qi[NI], kj[NI];
-          K.row(ki, 16 * wave, t);
-          Q.row(qi, 16 * wave, t);
-          K.row(kj, 16 * j, t);
-          kk = pl_mm<NI, NI>(ki, kj, kk);
-          qk = pl_mm<NI, NI>(qi, kj, qk);
+          for (int t = 0; t < DP / 32; ++t) {
+            bf16x8 ki[NI], qi[NI], kj[NI];
+            K.row(ki, 16 * it, t);
+            Q.row(qi, 16 * it, t);
+            K.row(kj, 16 * j, t);
+            kk = pl_mm<NI, NI>(ki, kj, kk);
+            qk = pl_mm<NI, NI>(qi, kj, qk);
+          }
         }
+        const int jj = 16 * j + n;
+        float cs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * it + 4 * kg + r;
+          const float dpr = j == it ? dp[r] : dp0[r], dar = j == it ? da[r] : da0[r];
+          float m1 = 0.f, m2 = 0.f;
+          if (jj <= i) {
+            const float d = dl_exp2(s.G[i] - s.G[jj]);
+            m1 = a.scale * d * dpr;
+            float m = m1 * qk[r];
+            if (jj < i) {
+              const float w = -d * dar;
+              m2 = s.beta[i] * w;
+              m += m2 * kk[r];
+              rb[r] += w * kk[r];
+            }
+            rm[r] += m;
+            cs += m;
+          }
+          M1.put(i, jj, m1);
+          M2.put(i, jj, m2);
+        }
+        cs += __shfl_xor(cs, 16);
+        cs += __shfl_xor(cs, 32);
+        if (kg == 0) colsum[it * 32 + jj] = cs;
       }
-      const int jj = 16 * j + n;
-      float cs = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * wave + 4 * kg + r;
-        float m1 = 0.f, m2 = 0.f;
-        if (jj <= i) {
-          const float d = expf((float)(s.G[i] - s.G[jj]));
-          m1 = a.scale * d * dp[j][r];
-          float m = m1 * qk[r];
-          if (jj < i) {
-            const float w = -d * da[j][r];
-            m2 = s.beta[i] * w;
-            m += m2 * kk[r];
-            rb[r] += w * kk[r];
-          }
-          rm[r] += m;
-          cs += m;
+        const float x0 = dl_sum16(rm[r]), x1 = dl_sum16(rb[r]);
+        if (n == 0) {
+          rows[16 * it + 4 * kg + r] = x0;
+          rows[32 + 16 * it + 4 * kg + r] = x1;
         }
-        M1.put(i, jj, m1);
-        M2.put(i, jj, m2);
       }
-      cs += __shfl_xor(cs, 16);
-      cs += __shfl_xor(cs, 32);
-      if (kg == 0) colsum[wave * 64 + jj] = cs;
     }
     float r1[4] = {0.f, 0.f, 0.f, 0.f}, r2[4] = {0.f, 0.f, 0.f, 0.f}, r3[4] = {0.f, 0.f, 0.f, 0.f};
+    if (S0 != nullptr || dS != nullptr) {
 #pragma unroll
-    for (int u = 0; u < UT; ++u)
+      for (int u = 0; u < UT; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * wave + 4 * kg + r;
-        const float gam = s.gam[i], kx = dl_get(K, i, 16 * u + n), qx = dl_get(Q, i, 16 * u + n);
-        r1[r] = __builtin_fmaf(qx, e1[u][r], r1[r]);
-        r2[r] = __builtin_fmaf(kx, e2[u][r], r2[r]);
-        r3[r] = __builtin_fmaf(kx, e3[u][r], r3[r]);
-        gq[u][r] += a.scale * gam * e1[u][r];
-        gk[u][r] += s.rest[i] * e3[u][r] - s.beta[i] * gam * e2[u][r];
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * it + 4 * kg + r, d = d0 + 16 * u + n;
+          const float gam = s.gam[i], kx = dl_get(K, i, d), qx = dl_get(Q, i, d);
+          r1[r] = __builtin_fmaf(qx, e1[u][r], r1[r]);
+          r2[r] = __builtin_fmaf(kx, e2[u][r], r2[r]);
+          r3[r] = __builtin_fmaf(kx, e3[u][r], r3[r]);
+          gq[u][r] += a.scale * gam * e1[u][r];
+          gk[u][r] += s.rest[i] * e3[u][r] - s.beta[i] * gam * e2[u][r];
+        }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * kg + r;
-      const float x0 = dl_sum16(rm[r]), x1 = dl_sum16(rb[r]), x2 = dl_sum16(r1[r]), x3 = dl_sum16(r2[r]),
-                  x4 = dl_sum16(r3[r]);
+      const int i = 16 * it + 4 * kg + r;
+      const float x2 = dl_sum16(r1[r]), x3 = dl_sum16(r2[r]), x4 = dl_sum16(r3[r]);
       if (n == 0) {
-        rows[i] = x0;
-        rows[64 + i] = x1;
-        rows[2 * 64 + i] = x2;
-        rows[3 * 64 + i] = x3;
-        rows[4 * 64 + i] = x4;
+        part[half * 32 + i] = x2;
+        part[(HALVES + half) * 32 + i] = x3;
+        part[(2 * HALVES + half) * 32 + i] = x4;
       }
     }
-    // one sum of S · dS' per wave in the gates' place of G, which is not read any more behind the barrier
-    __syncthreads();
-    if (lane == 0) s.G[wave] = both;
     __syncthreads();
     if (wave == 0) {
-      const int i = lane;
+      const int i = lane & 31;
       const float gam = s.gam[i], be = s.beta[i];
-      const double leave = (double)s.rest[i] * rows[4 * 64 + i];
-      double at = (double)rows[i] + (double)a.scale * gam * rows[2 * 64 + i] - (double)be * gam * rows[3 * 64 + i] - leave;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) at -= (double)colsum[w * 64 + i];
+      float qe = part[i], ke = part[HALVES * 32 + i], kd = part[2 * HALVES * 32 + i];
+      if (HALVES == 2) qe += part[32 + i], ke += part[3 * 32 + i], kd += part[5 * 32 + i];
+      const double leave = (double)s.rest[i] * kd;
+      double at = (double)rows[i] + (double)a.scale * gam * qe - (double)be * gam * ke - leave;
+      at -= (double)colsum[i] + (double)colsum[32 + i];
       double all = leave;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        all += __shfl_xor(all, o);
-        const double down = __shfl_down(at, o);
-        if (i + o < 64) at += down;
+      for (int o = 1; o < 32; o <<= 1) {
+        all += __shfl_xor(all, o, 32);
+        const double down = __shfl_down(at, o, 32);
+        if (i + o < 32) at += down;
       }
-      at += all + (double)s.gam[DL_C - 1] * (s.G[0] + s.G[1] + s.G[2] + s.G[3]);
+      at += all + (double)s.gam[DL_C - 1] * ((double)dots[0] + dots[1] + (HALVES == 2 ? (double)dots[2] + dots[3] : 0.0));
       const int64_t out = ((int64_t)b * a.T + t0 + i) * a.Hv + h;
-      if (t0 + i < a.T) {
+      if (lane < 32 && t0 + i < a.T) {
         a.dg[out] = t0 + i < len ? (float)at : 0.f;
-        a.dbeta[out] = t0 + i < len ? rows[5 * 64 + i] - gam * rows[3 * 64 + i] + rows[64 + i] : 0.f;
+        a.dbeta[out] = t0 + i < len ? rows[64 + i] - gam * ke + rows[32 + i] : 0.f;
       }
     }
+    bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
+    M1.row(m1, 16 * it, 0);
+    M2.row(m2, 16 * it, 0);
+    M1.col(m1t, 0, 16 * it);
+    M2.col(m2t, 0, 16 * it);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
-      M1.row(m1, 16 * wave, kb);
-      M2.row(m2, 16 * wave, kb);
-      M1.col(m1t, kb, 16 * wave);
-      M2.col(m2t, kb, 16 * wave);
-#pragma unroll
-      for (int u = 0; u < UT; ++u) {
-        bf16x8 f[NI];
-        K.col(f, kb, 16 * u);
-        if (kb <= wave / 2) {
-          gq[u] = pl_mm<NP, NI>(m1, f, gq[u]);
-          gk[u] = pl_mm<NP, NI>(m2, f, gk[u]);
-        }
-        if (kb >= wave / 2) {
-          gk[u] = pl_mm<NP, NI>(m2t, f, gk[u]);
-          Q.col(f, kb, 16 * u);
-          gk[u] = pl_mm<NP, NI>(m1t, f, gk[u]);
-        }
-      }
+    for (int u = 0; u < UT; ++u) {
+      bf16x8 f[NI];
+      K.col(f, 0, d0 + 16 * u);
+      gq[u] = pl_mm<NP, NI>(m1, f, gq[u]);
+      gk[u] = pl_mm<NP, NI>(m2, f, gk[u]);
+      gk[u] = pl_mm<NP, NI>(m2t, f, gk[u]);
+      Q.col(f, 0, d0 + 16 * u);
+      gk[u] = pl_mm<NP, NI>(m1t, f, gk[u]);
     }
+    __syncthreads();   // sums and M1, M2 are read: the next value head may write them
   }
 #pragma unroll
   for (int u = 0; u < UT; ++u)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int t = t0 + 16 * wave + 4 * kg + r, d = 16 * u + n;
+      const int t = t0 + 16 * it + 4 * kg + r, d = d0 + 16 * u + n;
       if (t < a.T && d < a.Dk) {
         dq[t * ks + d] = (IO)(t < len ? gq[u][r] : 0.f);
         dk[t * ks + d] = (IO)(t < len ? gk[u][r] : 0.f);
@@ -913,13 +1047,43 @@ static int delta_check(const DeltaArgs& a, int type) {
   if (type != 0 && type != 1) return RG_ERR_ARG;
   if (a.B <= 0 || a.T <= 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk) return RG_ERR_SHAPE;
   if (a.Dk <= 0 || a.Dk > 128 || a.Dk % 8 || a.Dv <= 0 || a.Dv > 128 || a.Dv % 8) return RG_ERR_SHAPE;
-  if ((int64_t)a.B * a.Hv > 0x7fffffff || (a.T + DL_C - 1) / DL_C > 65535) return RG_ERR_SHAPE;
+  if ((int64_t)a.B * a.Hv > (1 << 24) || (a.T + DL_C - 1) / DL_C > 65535) return RG_ERR_SHAPE;
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.g == nullptr || a.beta == nullptr) return RG_ERR_ARG;
   return RG_OK;
 }
-static bool delta_aligned(const void* p, const int64_t* s, int type) {   // 16-byte rows
+// positions at least a row apart, a chunk's 32 of them within a buffer's 2 GB
+static bool delta_apart(const int64_t* s, int T, int width) { return T == 1 || (s[1] >= width && s[1] < (1 << 23)); }
+// rows at multiples of 16 bytes
+static bool delta_aligned(const void* p, const int64_t* s, int type) {
   const int64_t e = type == 0 ? 4 : 2;
   return ((uintptr_t)p & 15) == 0 && s[0] * e % 16 == 0 && s[1] * e % 16 == 0 && s[2] * e % 16 == 0;
+}
+
+// column tiles a wave owns: as many as its registers hold (the chunk's P and T are made once for all of them), fewer
+// where that would leave CUs without work
+static int delta_ct(int64_t heads, int Dk, int Dv, int type) {
+  int ct = (Dk <= 64 ? 4 : 2) / (type == 0 ? 2 : 1);
+  while (ct > 1 && (16 * (ct / 2) >= Dv || heads * ((Dv + 16 * ct - 1) / (16 * ct)) < 1024)) ct /= 2;
+  return ct;
+}
+
+// Segments.  One pass takes about a chunk's 5 us per chunk in sequence; with segments there are two (the first also over
+// the transition's columns), each a segment long, and a join of about 2 us a segment.  2048 waves run at once.
+struct DeltaCut {
+  int nseg, per;
+};
+static DeltaCut delta_cut(int B, int T, int Hv, int Dk, int Dv) {
+  const int nC = (T + DL_C - 1) / DL_C;
+  DeltaCut best = {1, nC};
+  const int64_t heads = (int64_t)B * Hv, vw = (Dv + 31) / 32, kw = (Dk + 31) / 32;
+  auto rounds = [](int64_t waves) { return (double)((waves + 2047) / 2048); };
+  double cost = rounds(heads * vw) * nC * 5.0;
+  for (int want = 2; want <= 64 && want <= nC; want *= 2) {
+    const int per = (nC + want - 1) / want, nseg = (nC + per - 1) / per;
+    const double t = (rounds(heads * nseg * vw) + rounds(heads * nseg * (vw + kw))) * per * 5.0 + 2.0 * nseg + 10.0;
+    if (t < 0.8 * cost) cost = t, best = {nseg, per};
+  }
+  return best;
 }
 
 template <typename K>
@@ -932,38 +1096,59 @@ static int delta_go(K kern, dim3 grid, int threads, int shared, const DeltaArgs&
   return RG_OK;
 }
 
-// waves of a workgroup: all value columns together (K, Q, P and T of a chunk are then made once), fewer where that would
-// leave most of the 256 CUs without work
-static int delta_waves(const DeltaArgs& a) {
-  int w = (a.Dv + 15) / 16;
-  while (w > 2 && (int64_t)a.B * a.Hv * ((a.Dv + 16 * w - 1) / (16 * w)) < 128) w = (w + 1) / 2;
-  return w;
+template <typename IO, int DP, int CT>
+static int delta_fwd_ct(const DeltaArgs& a, hipStream_t st) {
+  const int heads = a.B * a.Hv, vb = (a.Dv + 16 * CT - 1) / (16 * CT), kb = (a.Dk + 16 * CT - 1) / (16 * CT);
+  if (a.nseg > 1) {
+    int rc = delta_go(k_delta_fwd<IO, DP, CT, true>, dim3(heads * a.nseg, vb + kb), 64, 0, a, st);
+    if (rc != RG_OK) return rc;
+    rc = delta_go(k_delta_join<DP, false>, dim3(heads, (a.Dv + 15) / 16), 4 * DP, 0, a, st);
+    if (rc != RG_OK) return rc;
+  }
+  return delta_go(k_delta_fwd<IO, DP, CT, false>, dim3(heads * a.nseg, vb), 64, 0, a, st);
 }
-
-// three planes of fp32 operands also for bf16 inputs: two would halve their products, but leave the fp32 outputs
-// (state, dg, dbeta) at 2^-18 instead of fp32's own rounding
-#define DL_NP 3
-
+template <typename IO, int DP, int CT>
+static int delta_scan_ct(const DeltaArgs& a, hipStream_t st) {
+  const int heads = a.B * a.Hv, vb = (a.Dv + 16 * CT - 1) / (16 * CT);
+  if (a.nseg > 1) {
+    int rc = delta_go(k_delta_scan<IO, DP, CT, true>, dim3(heads * a.nseg, vb), 64, 0, a, st);
+    if (rc != RG_OK) return rc;
+    rc = delta_go(k_delta_join<DP, true>, dim3(heads, (a.Dv + 15) / 16), 4 * DP, 0, a, st);
+    if (rc != RG_OK) return rc;
+  }
+  return delta_go(k_delta_scan<IO, DP, CT, false>, dim3(heads * a.nseg, vb), 64, 0, a, st);
+}
 template <typename IO, int DP>
 static int delta_fwd_t(const DeltaArgs& a, hipStream_t st) {
-  const int w = delta_waves(a);
-  return delta_go(k_delta_fwd<IO, DP, DL_NP>, dim3(a.B * a.Hv, (a.Dv + 16 * w - 1) / (16 * w)), 64 * w,
-                  DlLds<DP, DlIO<IO>::N, DL_NP>::BYTES, a, st);
+  const int ct = delta_ct((int64_t)a.B * a.Hv * a.nseg, a.Dk, a.Dv, DlIO<IO>::N == 3 ? 0 : 1);
+  if constexpr (DP <= 64 && DlIO<IO>::N == 1)
+    if (ct == 4) return delta_fwd_ct<IO, DP, 4>(a, st);
+  if constexpr (DP <= 64 || DlIO<IO>::N == 1)
+    if (ct >= 2) return delta_fwd_ct<IO, DP, 2>(a, st);
+  return delta_fwd_ct<IO, DP, 1>(a, st);
 }
 template <typename IO, int DP>
 static int delta_bwd_t(const DeltaArgs& a, hipStream_t st) {
-  const int w = delta_waves(a);
-  const int rc = delta_go(k_delta_scan<IO, DP, DL_NP>, dim3(a.B * a.Hv, (a.Dv + 16 * w - 1) / (16 * w)), 64 * w,
-                          DlLds<DP, DlIO<IO>::N, DL_NP>::BYTES, a, st);
+  const int ct = delta_ct((int64_t)a.B * a.Hv * a.nseg, a.Dk, a.Dv, DlIO<IO>::N == 3 ? 0 : 1);
+  int rc = RG_OK;
+  bool done = false;
+  if constexpr (DP <= 64 && DlIO<IO>::N == 1)
+    if (ct == 4) rc = delta_scan_ct<IO, DP, 4>(a, st), done = true;
+  if constexpr (DP <= 64 || DlIO<IO>::N == 1)
+    if (!done && ct >= 2) rc = delta_scan_ct<IO, DP, 2>(a, st), done = true;
+  if (!done) rc = delta_scan_ct<IO, DP, 1>(a, st);
   if (rc != RG_OK) return rc;
-  return delta_go(k_delta_grads<IO, DP, DL_NP>, dim3(a.B * a.Hk, (a.T + DL_C - 1) / DL_C), 256,
-                  DlGradLds<DP, DlIO<IO>::N, DL_NP>::BYTES, a, st);
+  using L = DlGradLds<DP, DlIO<IO>::N>;
+  return delta_go(k_delta_grads<IO, DP>, dim3(a.B * a.Hk, (a.T + DL_C - 1) / DL_C), L::THREADS, L::BYTES, a, st);
 }
 #define DL_DISPATCH(F)                                                                             \
   (type == 0 ? (a.Dk <= 32 ? F<float, 32>(a, st) : a.Dk <= 64 ? F<float, 64>(a, st) : F<float, 128>(a, st)) \
              : (a.Dk <= 32 ? F<__bf16, 32>(a, st) : a.Dk <= 64 ? F<__bf16, 64>(a, st) : F<__bf16, 128>(a, st)))
 
-static void delta_strides(DeltaArgs& a, const int64_t* s) {
+// (one position: its stride means nothing, but the rows behind it have to lie behind the buffer's end)
+static void delta_strides(DeltaArgs& a, const int64_t* strides, int T) {
+  int64_t s[18];
+  for (int i = 0; i < 18; ++i) s[i] = T == 1 && i % 3 == 1 ? 128 : strides[i];
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = s[i];
     a.ks[i] = s[3 + i];
@@ -973,47 +1158,67 @@ static void delta_strides(DeltaArgs& a, const int64_t* s) {
     a.dos[i] = s[15 + i];
   }
 }
+static void delta_segments(DeltaArgs& a, float* trans, float* local) {
+  const DeltaCut c = delta_cut(a.B, a.T, a.Hv, a.Dk, a.Dv);
+  a.nseg = c.nseg, a.per = c.per, a.trans = trans, a.local = local;
+}
 
 extern "C" int64_t rg_delta_chunk_floats(int B, int T, int Hv, int Dk, int Dv) {
   return T > 0 ? (int64_t)B * Hv * ((T + DL_C - 1) / DL_C - 1) * Dk * Dv : 0;
+}
+extern "C" int rg_delta_segments(int B, int T, int Hv, int Dk, int Dv) {
+  return B > 0 && T > 0 ? delta_cut(B, T, Hv, Dk, Dv).nseg : 1;
 }
 
 extern "C" int rg_delta_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta,
                             const int64_t* strides, const int64_t* lens, const float* state0, int type, int B, int T,
                             int Hk, int Hv, int Dk, int Dv, float scale, void* o, float* state, float* U, float* S0,
-                            hipStream_t st) {
+                            float* trans, float* local, hipStream_t st) {
   DeltaArgs a = {};
   if (strides == nullptr) return RG_ERR_ARG;
-  delta_strides(a, strides);
+  delta_strides(a, strides, T);
   a.q = q, a.k = k, a.v = v, a.g = g, a.beta = beta, a.lens = lens, a.state0 = state0;
   a.B = B, a.T = T, a.Hk = Hk, a.Hv = Hv, a.Dk = Dk, a.Dv = Dv, a.scale = scale, a.o = o, a.state = state, a.U = U;
-  a.S0 = T > DL_C ? S0 : nullptr;
+  a.S0 = U != nullptr && T > DL_C ? S0 : nullptr;
   const int rc = delta_check(a, type);
   if (rc != RG_OK) return rc;
-  if (o == nullptr || state == nullptr || (U != nullptr && T > DL_C && S0 == nullptr)) return RG_ERR_ARG;
-  if (!delta_aligned(q, a.qs, type) || !delta_aligned(k, a.ks, type)) return RG_ERR_ARG;
+  if (!delta_apart(a.qs, T, Dk) || !delta_apart(a.ks, T, Dk) || !delta_apart(a.vs, T, Dv) || !delta_apart(a.gs, T, 1) ||
+      !delta_apart(a.bs, T, 1))
+    return RG_ERR_ARG;
+  delta_segments(a, trans, local);
+  if (o == nullptr || state == nullptr || (U != nullptr && T > DL_C && S0 == nullptr) || (a.nseg > 1 && (trans == nullptr || local == nullptr)))
+    return RG_ERR_ARG;
+  if (!delta_aligned(q, a.qs, type) || !delta_aligned(k, a.ks, type) || (((uintptr_t)o | (uintptr_t)trans | (uintptr_t)local) & 15))
+    return RG_ERR_ARG;
   return DL_DISPATCH(delta_fwd_t);
 }
 
 extern "C" int rg_delta_bwd(const void* q, const void* k, const void* v, const float* g, const float* beta,
                             const void* d_o, const int64_t* strides, const int64_t* lens, const float* state0,
-                            const float* dstate, const float* U, const float* S0, int type, int B, int T, int Hk,
-                            int Hv, int Dk, int Dv, float scale, float* dX, float* dS, void* dq, void* dk, void* dv,
-                            float* dg, float* dbeta, float* dstate0, hipStream_t st) {
+                            const float* dstate, const float* U, const float* S0, const float* trans, int type, int B, int T,
+                            int Hk, int Hv, int Dk, int Dv, float scale, float* dX, float* dS, float* local, void* dq,
+                            void* dk, void* dv, float* dg, float* dbeta, float* dstate0, hipStream_t st) {
   DeltaArgs a = {};
   if (strides == nullptr) return RG_ERR_ARG;
-  delta_strides(a, strides);
+  delta_strides(a, strides, T);
   a.q = q, a.k = k, a.v = v, a.g = g, a.beta = beta, a.d_o = d_o, a.lens = lens, a.state0 = state0, a.dstate = dstate;
   a.B = B, a.T = T, a.Hk = Hk, a.Hv = Hv, a.Dk = Dk, a.Dv = Dv, a.scale = scale;
   a.U = const_cast<float*>(U), a.S0 = const_cast<float*>(S0), a.dX = dX, a.dS = dS;
   a.dq = dq, a.dk = dk, a.dv = dv, a.dg = dg, a.dbeta = dbeta, a.dstate0 = dstate0;
   const int rc = delta_check(a, type);
   if (rc != RG_OK) return rc;
+  if (!delta_apart(a.qs, T, Dk) || !delta_apart(a.ks, T, Dk) || !delta_apart(a.vs, T, Dv) || !delta_apart(a.gs, T, 1) ||
+      !delta_apart(a.bs, T, 1))
+    return RG_ERR_ARG;
+  delta_segments(a, const_cast<float*>(trans), local);
+  if (!delta_apart(a.dos, T, Dv)) return RG_ERR_ARG;
   if (d_o == nullptr || U == nullptr || dX == nullptr || dq == nullptr || dk == nullptr || dv == nullptr ||
-      dg == nullptr || dbeta == nullptr || (T > DL_C && (S0 == nullptr || dS == nullptr)))
+      dg == nullptr || dbeta == nullptr || (T > DL_C && (S0 == nullptr || dS == nullptr)) ||
+      (a.nseg > 1 && (trans == nullptr || local == nullptr)))
     return RG_ERR_ARG;
   if (!delta_aligned(q, a.qs, type) || !delta_aligned(k, a.ks, type) || !delta_aligned(d_o, a.dos, type) ||
-      (((uintptr_t)state0 | (uintptr_t)dstate | (uintptr_t)U | (uintptr_t)S0 | (uintptr_t)dX | (uintptr_t)dS) & 15))
+      (((uintptr_t)state0 | (uintptr_t)dstate | (uintptr_t)U | (uintptr_t)S0 | (uintptr_t)dX | (uintptr_t)dS |
+        (uintptr_t)trans | (uintptr_t)local) & 15))
     return RG_ERR_ARG;
   return DL_DISPATCH(delta_bwd_t);
 }
@@ -1023,7 +1228,7 @@ extern "C" int rg_delta_step(const void* q, const void* k, const void* v, const 
                              float* state, int64_t state_stride, void* o, hipStream_t st) {
   DeltaArgs a = {};
   if (strides == nullptr) return RG_ERR_ARG;
-  delta_strides(a, strides);
+  delta_strides(a, strides, 1);
   a.q = q, a.k = k, a.v = v, a.g = g, a.beta = beta, a.state = state, a.o = o;
   a.B = B, a.T = 1, a.Hk = Hk, a.Hv = Hv, a.Dk = Dk, a.Dv = Dv, a.scale = scale;
   const int rc = delta_check(a, type);

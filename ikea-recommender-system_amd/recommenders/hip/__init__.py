@@ -150,8 +150,9 @@ SIGNATURES = {
     "rg_lazy_catch_up": [P, P, P, I, P, P, P, P, I64, P, P, I32, I32, P, P],
     "rg_lazy_adam_rows": [P, P, P, P, I, P, P, P, P, P, I64, P, P, I32, I32, P, P, P],
     "rg_delta_chunk_floats": [I, I, I, I, I],
-    "rg_delta_fwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P],
-    "rg_delta_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P, P],
+    "rg_delta_segments": [I, I, I, I, I],
+    "rg_delta_fwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P],
+    "rg_delta_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P, P, P],
     "rg_delta_step": [P, P, P, P, P, P, I, I, I, I, I, I, F, P, I64, P, P],
     "rg_linear_ce_work_floats": [I, I, I, I],
     "rg_linear_ce_saved_bytes": [I, I, I],

@@ -8,7 +8,7 @@ q, k (B, T, Hk, Dk); v (B, T, Hv, Dv), Hv a multiple of Hk (value heads h of
 key head h // (Hv / Hk)); g, beta (B, T, Hv) fp32, g <= 0 the log of the
 decay (−inf resets).  q, k, v are fp32 or bf16; states and every sum are fp32.
 Dk and Dv are multiples of 8 up to 128.  Strides are free as long as heads'
-rows are contiguous and start at multiples of 16 bytes.
+rows are contiguous, start at multiples of 16 bytes and do not overlap along T.
 
 `lens` (B) int64 on the device: positions at or behind a row's length are not
 read, leave the state as it is and get zeros (also as gradients); a length of
@@ -32,11 +32,11 @@ _IO = (torch.float32, torch.bfloat16)
 
 
 class Saved:
-    """What the backward pass needs of a forward call: its operands (not copied: they have to keep their values) and the
-    updates and chunk states it left."""
+    """What the backward pass needs of a forward call: its operands (not copied: they have to keep their values), the
+    updates and chunk states it left, and its segments' transitions."""
 
-    def __init__(self, plan, operands, scale, U, S0):
-        self.plan, self.operands, self.scale, self.U, self.S0 = plan, operands, scale, U, S0
+    def __init__(self, plan, operands, scale, U, S0, trans):
+        self.plan, self.operands, self.scale, self.U, self.S0, self.trans = plan, operands, scale, U, S0, trans
         self.versions = [version(t) for t in operands]
 
 
@@ -46,6 +46,11 @@ _plans, _plans_back, _plans_step = Plans(), Plans(), Plans()
 def _strides(*rows):
     flat = [s for r in rows for s in r]
     return (C.c_int64 * 18)(*flat, *([0] * (18 - len(flat))))
+
+
+def _apart(name, t, width):
+    if not width <= t.stride(1) < 1 << 23:
+        fail(name, f"positions overlap or lie too far apart: stride {t.stride(1)}")
 
 
 class _Plan:
@@ -67,6 +72,9 @@ class _Plan:
                 fail(name, f"a tensor of shape {(*q.shape[:-2], Hv)} is expected")
             tensor(name, t[..., None], (*q.shape[:-2], Hv, 1), (torch.float32,), q.device)   # any strides
         self.B, self.T = q.shape[0], q.shape[1] if lead == 2 else 1
+        if self.T > 1:
+            for name, t, d in (("q", q, Dk), ("k", k, Dk), ("v", v, Dv), ("g", g, 1), ("beta", beta, 1)):
+                _apart(name, t, d)
         self.device, self.dtype, self.type, self.scale = q.device, q.dtype, TYPES[q.dtype], Dk ** -0.5
         self.state = (self.B, Hv, Dk, Dv)
         self.sizes = (self.B, self.T, Hk, Hv, Dk, Dv)
@@ -90,6 +98,8 @@ def _plan(q, k, v, g, beta, lens, state):
         whole("state", state, p.state, (torch.float32,), p.device)
     p.forward, p.backward = entry("rg_delta_fwd"), entry("rg_delta_bwd")
     p.chunks = call("rg_delta_chunk_floats", p.B, p.T, p.Hv, p.Dk, p.Dv)
+    n = call("rg_delta_segments", p.B, p.T, p.Hv, p.Dk, p.Dv)
+    p.trans, p.local = ((p.B, p.Hv, n, p.Dk, p.Dk), (p.B, p.Hv, n, p.Dk, p.Dv)) if n > 1 else (None, None)
     return p
 
 
@@ -105,20 +115,24 @@ def delta_rule(q, k, v, g, beta, scale=None, lens=None, state=None, save=False):
     scale = p.scale if scale is None else float(scale)
     o = torch.empty(p.B, p.T, p.Hv, p.Dv, dtype=p.dtype, device=p.device)
     final = torch.empty(p.state, dtype=torch.float32, device=p.device)
-    U = S0 = None
+    U = S0 = trans = local = None
     if p.empty:
         final.copy_(state) if state is not None else final.zero_()
     else:
         if save:
             U = torch.empty(p.B, p.Hv, p.T, p.Dv, dtype=torch.float32, device=p.device)
             S0 = torch.empty(p.chunks, dtype=torch.float32, device=p.device) if p.chunks else None
+        if p.trans:
+            trans, local = (torch.empty(n, dtype=torch.float32, device=p.device) for n in (p.trans, p.local))
         run(p.forward, p.device, *at[:5], p.strides, *at[5:], p.type, *p.sizes, scale, o.data_ptr(), final.data_ptr(),
-            ptr(U), ptr(S0))
-    return (o, final, Saved(p, operands, scale, U, S0)) if save else (o, final)
+            ptr(U), ptr(S0), ptr(trans), ptr(local))
+    return (o, final, Saved(p, operands, scale, U, S0, trans)) if save else (o, final)
 
 
 def _back_plan(p, do, dstate):
     tensor("do", do, (p.B, p.T, p.Hv, p.Dv), (p.dtype,), p.device, align=16)
+    if p.T > 1:
+        _apart("do", do, p.Dv)
     if dstate is not None:
         whole("dstate", dstate, p.state, (torch.float32,), p.device)
     return _strides(*p.rows, [stride(do, d) for d in range(3)])
@@ -149,9 +163,10 @@ def delta_rule_backward(saved, do, dstate=None):
     else:
         dX = torch.empty(p.B, p.Hv, p.T, p.Dv, **full)
         dS = torch.empty(p.chunks, **full) if p.chunks else None
+        local = torch.empty(p.local, **full) if p.local else None
         run(p.backward, p.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), do.data_ptr(),
-            strides, ptr(lens), ptr(state), ptr(dstate), saved.U.data_ptr(), ptr(saved.S0), p.type, *p.sizes,
-            saved.scale, dX.data_ptr(), ptr(dS), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+            strides, ptr(lens), ptr(state), ptr(dstate), saved.U.data_ptr(), ptr(saved.S0), ptr(saved.trans), p.type, *p.sizes,
+            saved.scale, dX.data_ptr(), ptr(dS), ptr(local), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
             dbeta.data_ptr(), ptr(dstate0))
     return dq, dk, dv, dg, dbeta, dstate0
 

@@ -615,20 +615,26 @@ int rg_comm_reduce_scatter(void* comm, const void* send, void* recv, int64_t n, 
  * S_t = exp(g_t) S_{t-1} + beta_t k_t (v_t - exp(g_t) S_{t-1}^T k_t)^T, o_t = scale S_t^T q_t, S a Dk x Dv matrix.
  * q, k (B, T, Hk, Dk), v and d_o (B, T, Hv, Dv) of `type` (0 fp32, 1 bf16), g, beta (B, T, Hv) fp32; Hv a multiple of
  * Hk; Dk, Dv multiples of 8 up to 128.  strides: HOST array of 18, the (B, T, H) strides in elements of q, k, v, g, beta,
- * d_o; rows (the last dimension) are contiguous, those of q, k, d_o start at multiples of 16 bytes.  lens (B) int64,
+ * d_o; rows (the last dimension) are contiguous, positions (T) at least a row and less than 2^23 elements apart, rows of
+ * q, k, d_o start at multiples of 16 bytes.  lens (B) int64,
  * optional: positions at or behind it are not read, do not change the state and get zeros.  Contiguous: o, dv
  * (B, T, Hv, Dv), dq, dk (B, T, Hk, Dk), dg, dbeta (B, T, Hv), the states (B, Hv, Dk, Dv) fp32.
- * For the backward pass the forward leaves U (B, Hv, T, Dv) and S0 (rg_delta_chunk_floats values, when T > 64); both
- * optional otherwise.  dX is of U's size, dS of S0's.  state0, dstate, dstate0 optional (NULL: zero / not wanted).
+ * For the backward pass the forward leaves U (B, Hv, T, Dv) and S0 (rg_delta_chunk_floats values, when T > 32); both
+ * NULL otherwise.  A long T is cut into n = rg_delta_segments(..) segments; when n > 1: trans (B, Hv, n, Dk, Dk) fp32,
+ * which the backward call reads again, and local (B, Hv, n, Dk, Dv) fp32, work space of one call.  dX is of U's size, dS
+ * of S0's.  state0, dstate, dstate0 optional (NULL: zero / not wanted).
  * rg_delta_step: one token, q, k (B, Hk, Dk), v (B, Hv, Dv); state updated in place, its rows state_stride apart. */
 int64_t rg_delta_chunk_floats(int B, int T, int Hv, int Dk, int Dv);
+int rg_delta_segments(int B, int T, int Hv, int Dk, int Dv);
 int rg_delta_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const int64_t* strides,
                  const int64_t* lens, const float* state0, int type, int B, int T, int Hk, int Hv, int Dk, int Dv,
-                 float scale, void* o, float* state, float* U, float* S0, rg_stream_t stream);
+                 float scale, void* o, float* state, float* U, float* S0, float* trans, float* local,
+                 rg_stream_t stream);
 int rg_delta_bwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const void* d_o,
                  const int64_t* strides, const int64_t* lens, const float* state0, const float* dstate, const float* U,
-                 const float* S0, int type, int B, int T, int Hk, int Hv, int Dk, int Dv, float scale, float* dX,
-                 float* dS, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* dstate0, rg_stream_t stream);
+                 const float* S0, const float* trans, int type, int B, int T, int Hk, int Hv, int Dk, int Dv,
+                 float scale, float* dX, float* dS, float* local, void* dq, void* dk, void* dv, float* dg,
+                 float* dbeta, float* dstate0, rg_stream_t stream);
 int rg_delta_step(const void* q, const void* k, const void* v, const float* g, const float* beta,
                   const int64_t* strides, int type, int B, int Hk, int Hv, int Dk, int Dv, float scale, float* state,
                   int64_t state_stride, void* o, rg_stream_t stream);

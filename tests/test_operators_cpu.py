@@ -52,23 +52,24 @@ def test_delta_c_entry_refusals():
     lib = load_library()
     p, s = 4096, (C.c_int64 * 18)(*[64] * 18)   # an aligned address that is never read: each call is refused first
 
-    def fwd(type=0, B=1, T=5, Hk=1, Hv=1, Dk=16, Dv=16, q=p, o=p, strides=s, U=None, S0=None):
-        return lib.rg_delta_fwd(q, p, p, p, p, strides, None, None, type, B, T, Hk, Hv, Dk, Dv, 1.0, o, p, U, S0, None)
+    def fwd(type=0, B=1, T=5, Hk=1, Hv=1, Dk=16, Dv=16, q=p, o=p, strides=s, U=None, S0=None, trans=None, local=None):
+        return lib.rg_delta_fwd(q, p, p, p, p, strides, None, None, type, B, T, Hk, Hv, Dk, Dv, 1.0, o, p, U, S0, trans, local, None)
     assert fwd(type=2) == -1 and fwd(o=None) == -1 and fwd(q=None) == -1 and fwd(strides=None) == -1
     assert fwd(B=0) == -3 and fwd(T=0) == -3 and fwd(Hk=2, Hv=3) == -3
-    assert fwd(Dk=12) == -3 and fwd(Dk=136) == -3 and fwd(Dv=0) == -3 and fwd(T=65536 * 64) == -3
+    assert fwd(Dk=12) == -3 and fwd(Dk=136) == -3 and fwd(Dv=0) == -3 and fwd(T=65536 * 32) == -3
     assert fwd(q=p + 4) == -1 and fwd(strides=(C.c_int64 * 18)(*[63] * 18)) == -1
-    assert fwd(T=65, U=p) == -1                 # the chunk states' room is missing
+    assert fwd(T=33, U=p) == -1                 # the chunk states' room is missing
+    assert lib.rg_delta_segments(1, 4000, 1, 16, 16) > 1 and fwd(T=4000) == -1 and fwd(T=4000, trans=p) == -1   # the segments' room is missing
 
     def bwd(do=p, dX=p, T=5, dS=None, state0=None):
-        return lib.rg_delta_bwd(p, p, p, p, p, do, s, None, state0, None, p, None, 0, 1, T, 1, 1, 16, 16, 1.0, dX, dS, p, p, p,
+        return lib.rg_delta_bwd(p, p, p, p, p, do, s, None, state0, None, p, None, None, 0, 1, T, 1, 1, 16, 16, 1.0, dX, dS, None, p, p, p,
                                 p, p, None, None)
     assert bwd(do=None) == -1 and bwd(dX=None) == -1 and bwd(T=65) == -1 and bwd(state0=p + 4) == -1
 
     def step(stride=256, state=p, B=2):
         return lib.rg_delta_step(p, p, p, p, p, s, 0, B, 1, 1, 16, 16, 1.0, state, stride, p, None)
     assert step(stride=255) == -1 and step(stride=252) == -1 and step(state=p + 4) == -1 and step(B=0) == -3
-    assert lib.rg_delta_chunk_floats(2, 64, 3, 8, 8) == 0 and lib.rg_delta_chunk_floats(2, 65, 3, 8, 16) == 2 * 3 * 8 * 16
+    assert lib.rg_delta_chunk_floats(2, 32, 3, 8, 8) == 0 and lib.rg_delta_chunk_floats(2, 33, 3, 8, 16) == 2 * 3 * 8 * 16
 
 
 def test_linear_ce_refuses_before_the_device():
