@@ -20,7 +20,8 @@
 //
 // The state, G and every sum are fp32 or wider (G in fp64: differences of long sums enter an exponential).  Products run
 // on bf16 MFMA with fp32 operands split into three planes (planes.h); bf16 inputs are one exact plane.  Two planes
-// would halve the products, but leave the fp32 outputs (state, dg, dbeta) at 2^-18 instead of fp32's own rounding.
+// would halve the products, but leave the fp32 outputs (state, dg, dbeta) at 2^-18 instead of fp32's own rounding; they do
+// for o where it is rounded to bf16 (2^-8) in the end.
 // Positions at or behind a sequence's length are read as k = v = q = 0, b = 0, g = 0, which leaves the state as it is;
 // nothing is read there.
 //
@@ -81,6 +82,10 @@ struct DlIO<float> {
   static __device__ __forceinline__ void load44(DlBuf b, int v, int s, int v2, int s2, bf16x8* f) {
     pl_split<3>(load4(b, v, s), load4(b, v2, s2), f);
   }
+  static __device__ __forceinline__ void load4x2(DlBuf b, int v, int s, int v2, int s2, f4& x, f4& y) {
+    x = load4(b, v, s);
+    y = load4(b, v2, s2);
+  }
   struct Raw8 {
     f4 a, b;
   };
@@ -89,8 +94,10 @@ struct DlIO<float> {
   static __device__ __forceinline__ void store1(DlBuf b, int v, int s, float x) {
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), b, v, s, 0);
   }
+  // the scalar offset stays constant here: a 16-byte store with one in a register may read its data after the next
+  // instruction has overwritten it (the compiler only waits where the offset is a constant)
   static __device__ __forceinline__ void store4(DlBuf b, int v, int s, f4 x) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dl_u4, x), b, v, s, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dl_u4, x), b, v + s, 0, 0);
   }
 };
 template <>
@@ -102,6 +109,11 @@ struct DlIO<__bf16> {
   static __device__ __forceinline__ void load44(DlBuf b, int v, int s, int v2, int s2, bf16x8* f) {
     const dl_u2 x = __builtin_amdgcn_raw_buffer_load_b64(b, v, s, 0), y = __builtin_amdgcn_raw_buffer_load_b64(b, v2, s2, 0);
     f[0] = __builtin_bit_cast(bf16x8, (dl_u4){x[0], x[1], y[0], y[1]});
+  }
+  static __device__ __forceinline__ void load4x2(DlBuf b, int v, int s, int v2, int s2, f4& x, f4& y) {
+    const dl_u2 p = __builtin_amdgcn_raw_buffer_load_b64(b, v, s, 0), q = __builtin_amdgcn_raw_buffer_load_b64(b, v2, s2, 0);
+    x = (f4){__uint_as_float(p[0] << 16), __uint_as_float(p[0] & 0xffff0000u), __uint_as_float(p[1] << 16), __uint_as_float(p[1] & 0xffff0000u)};
+    y = (f4){__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16), __uint_as_float(q[1] & 0xffff0000u)};
   }
   typedef bf16x8 Raw8;
   static __device__ __forceinline__ Raw8 load8(DlBuf b, int v, int s) {
@@ -123,22 +135,26 @@ __device__ __forceinline__ int dl_len(const DeltaArgs& a, int b) {
   return n < 0 ? 0 : n > a.T ? a.T : (int)n;
 }
 
-// 32 rows of a (.., D) operand into planes (zeros behind the buffer's rows and behind column D)
+// 32 rows of a (.., D) operand (zeros behind the buffer's rows and behind column D): from memory, then into planes
 template <typename IO, int DP, int THREADS>
-__device__ __forceinline__ void dl_load(const PlaneMat<DL_C, DP, DlIO<IO>::N>& m, DlBuf buf, int64_t st, int D, int tid) {
-  constexpr int N = DlIO<IO>::N, W = DP / 8, ALL = DL_C * W, PER = ALL / THREADS > 0 ? ALL / THREADS : 1;
-  const int r = tid / W, c = tid % W * 8, v = dl_lane(c < D && tid < ALL, (int)(r * st + c) * DlIO<IO>::SIZE);
-  const int step = (int)(THREADS / W * st) * DlIO<IO>::SIZE;
+struct DlTile {
+  static constexpr int N = DlIO<IO>::N, W = DP / 8, ALL = DL_C * W, PER = ALL / THREADS > 0 ? ALL / THREADS : 1;
   typename DlIO<IO>::Raw8 x[PER];
+  __device__ __forceinline__ void load(DlBuf buf, int64_t st, int D, int tid) {
+    const int r = tid / W, c = tid % W * 8, v = dl_lane(c < D && tid < ALL, (int)(r * st + c) * DlIO<IO>::SIZE);
+    const int step = (int)(THREADS / W * st) * DlIO<IO>::SIZE;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) x[i] = DlIO<IO>::load8(buf, v, i * step);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    bf16x8 f[N];
-    DlIO<IO>::planes(x[i], f);
-    if (ALL >= THREADS || tid < ALL) m.put8(r + i * (THREADS / W), c, f);
+    for (int i = 0; i < PER; ++i) x[i] = DlIO<IO>::load8(buf, v, i * step);
   }
-}
+  __device__ __forceinline__ void put(const PlaneMat<DL_C, DP, N>& m, int tid) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      bf16x8 f[N];
+      DlIO<IO>::planes(x[i], f);
+      if (ALL >= THREADS || tid < ALL) m.put8(tid / W + i * (THREADS / W), tid % W * 8, f);
+    }
+  }
+};
 // operand straight from memory: rows `row` + n, columns c0 + 4·kg .. and 16 further on
 template <typename IO>
 __device__ __forceinline__ void dl_operand(bf16x8* f, DlBuf buf, int row, int64_t st, int c0, int D) {
@@ -155,14 +171,17 @@ struct DlGates {
   float beta[DL_C];
 };
 __device__ __forceinline__ float dl_exp2(double x) { return __builtin_amdgcn_exp2f((float)x); }
-// one wave
-__device__ __forceinline__ void dl_gates(DlGates& s, const DeltaArgs& a, int b, int h, int t0, int len) {
-  const int i = threadIdx.x & 31, t = t0 + i;
+// one wave: g and beta of a chunk's positions from memory, then their sums and exponentials
+__device__ __forceinline__ void dl_gates_load(float* x, const DeltaArgs& a, int b, int h, int t0, int len) {
+  const int i = threadIdx.x & 31;
   const DlBuf gbuf = dl_buf(a.g + b * a.gs[0] + t0 * a.gs[1] + h * a.gs[2], 32, a.gs[1], 1, 4),
               bbuf = dl_buf(a.beta + b * a.bs[0] + t0 * a.bs[1] + h * a.bs[2], 32, a.bs[1], 1, 4);
-  const float gi = DlIO<float>::load1(gbuf, dl_lane(t < len, (int)(i * a.gs[1]) * 4), 0);
-  const float be = DlIO<float>::load1(bbuf, dl_lane(t < len, (int)(i * a.bs[1]) * 4), 0);
-  double g = (gi < DL_G_MIN ? DL_G_MIN : (double)gi) * 1.4426950408889634;   // NaN stays
+  x[0] = DlIO<float>::load1(gbuf, dl_lane(t0 + i < len, (int)(i * a.gs[1]) * 4), 0);
+  x[1] = DlIO<float>::load1(bbuf, dl_lane(t0 + i < len, (int)(i * a.bs[1]) * 4), 0);
+}
+__device__ __forceinline__ void dl_gates(DlGates& s, const float* x) {
+  const int i = threadIdx.x & 31;
+  double g = (x[0] < DL_G_MIN ? DL_G_MIN : (double)x[0]) * 1.4426950408889634;   // NaN stays
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double up = __shfl_up(g, o, 32);
@@ -173,11 +192,17 @@ __device__ __forceinline__ void dl_gates(DlGates& s, const DeltaArgs& a, int b, 
     s.G[i] = g;
     s.gam[i] = dl_exp2(g);
     s.rest[i] = dl_exp2(end - g);
-    s.beta[i] = be;
+    s.beta[i] = x[1];
   }
 }
 
 #define DL_ZERO ((f4){0.f, 0.f, 0.f, 0.f})
+
+// LDS between the lanes of one wave: its LDS instructions run in order, so only the compiler has to keep it
+__device__ __forceinline__ void dl_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+}
 
 // Forward substitution: column n of (1 + A)^-1, A strictly lower, 16 x 16 in LDS (rows of 20 floats, read by many lanes at
 // once).  The next row is read while this one's sum runs; left to itself the compiler reads all of A first (120 registers).
@@ -236,11 +261,11 @@ __device__ __forceinline__ void dl_inverse(const PlaneMat<DL_C, DP, NI>& K, cons
     Ad[320 + i * 20 + n] = n < i ? s.beta[16 + i] * dl_exp2(g1 - gn1) * d1[r] : 0.f;
     off[r] *= bn1 * dl_exp2(gn1 - g0);
   }
-  __syncthreads();
+  dl_fence();
   {   // lanes of kg 0, 1 solve block 0, the others block 1; T goes where A was, each lane half a column
     float x[16];
     dl_solve(Ad + 320 * (kg >> 1), n, x);
-    __syncthreads();
+    dl_fence();
     float* to = Ad + 320 * (kg >> 1) + n;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -248,7 +273,7 @@ __device__ __forceinline__ void dl_inverse(const PlaneMat<DL_C, DP, NI>& K, cons
       to[(i + 8 * (kg & 1)) * 20] = kg & 1 ? hi : lo;
     }
   }
-  __syncthreads();
+  dl_fence();
   f4 c0, r1;
 #pragma unroll
   for (int r = 0; r < 4; ++r) c0[r] = Ad[(4 * kg + r) * 20 + n];   // column n of T00
@@ -298,14 +323,21 @@ template <int CT, int UT>
 __device__ __forceinline__ void dl_state_store(const f4 (*S)[UT], float* dst, int Dk, int cols, int col0) {
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
   const DlBuf buf = dl_buf(dst, Dk, cols, cols, 4);
+  int row[CT], at = 0;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int col = col0 + 16 * ct + n, v = dl_lane(col < cols, (4 * kg * cols + col) * 4);
-#pragma unroll
-    for (int u = 0; u < UT; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) DlIO<float>::store1(buf, v, (16 * u + r) * cols * 4, S[ct][u][r]);
+    const int col = col0 + 16 * ct + n;
+    row[ct] = dl_lane(col < cols, (4 * kg * cols + col) * 4);
   }
+#pragma unroll
+  for (int u = 0; u < UT; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      asm volatile("" : "+s"(at));   // one running offset; the compiler would keep all of them and spill
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) DlIO<float>::store1(buf, row[ct], at, S[ct][u][r]);
+      at += (r < 3 ? 1 : 13) * cols * 4;
+    }
 }
 
 // ---------------------------------------------------------------- forward ----
@@ -313,7 +345,7 @@ __device__ __forceinline__ void dl_state_store(const f4 (*S)[UT], float* dst, in
 // behind them: the segment's transition)
 template <typename IO, int DP, int CT, bool TRANS>
 __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
-  constexpr int NI = DlIO<IO>::N, KT = DP / 32, NP = DL_NP;
+  constexpr int NI = DlIO<IO>::N, KT = DP / 32, NP = DL_NP, NO = NI == 1 ? 2 : 3;
   using L = DlLds<DP, NI, false>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::BYTES];
   const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds};
@@ -351,14 +383,18 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
     const int left = len - t0;   // positions from here on
     const int rows = min(left, DL_C);
     const DlBuf vbuf = dl_buf(v + t0 * a.vs[1], unit ? 0 : rows, a.vs[1], a.Dv, DlIO<IO>::SIZE);
-    float vv[CT][8];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
+    auto values = [&](int ct, float* x) __attribute__((always_inline)) {
       const int col = col0 + 16 * ct + n, at = dl_lane(col < cols, (int)(4 * kg * a.vs[1] + col) * DlIO<IO>::SIZE);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        vv[ct][i] = DlIO<IO>::load1(vbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.vs[1]) * DlIO<IO>::SIZE);
-    }
+        x[i] = DlIO<IO>::load1(vbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.vs[1]) * DlIO<IO>::SIZE);
+    };
+    DlTile<IO, DP, 64> kt;
+    kt.load(dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
+    float gates[2];
+    dl_gates_load(gates, a, b, h, t0, len);
+    float vv[8], vnext[8];
+    values(0, vnext);
     bf16x8 qf[2][KT][NI];
     if constexpr (!TRANS) {
       const DlBuf qbuf = dl_buf(q + t0 * a.qs[1], rows, a.qs[1], a.Dk, DlIO<IO>::SIZE);
@@ -369,11 +405,11 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
       if (a.S0 != nullptr && t0 > 0)
         dl_state_store<CT, 2 * KT>(S, a.S0 + (bh * (nC - 1) + t0 / DL_C - 1) * size, a.Dk, a.Dv, col0);
     }
-    __syncthreads();
-    dl_load<IO, DP, 64>(K, dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
-    dl_gates(s, a, b, h, t0, len);
-    __syncthreads();
-    bf16x8 T[2][NP], P[2][NP];
+    dl_fence();
+    kt.put(K, lane);
+    dl_gates(s, gates);
+    dl_fence();
+    bf16x8 T[2][NP], P[2][NO];
     dl_inverse<DP, NI, true>(K, s, Ad, T);
     if constexpr (!TRANS) {
       f4 p00 = DL_ZERO, p01 = DL_ZERO, p11 = DL_ZERO;   // rows j, columns i
@@ -395,14 +431,17 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
         p01[r] *= a.scale * dl_exp2(g1 - h0);
         p11[r] = j <= n ? a.scale * dl_exp2(g1 - h1) * p11[r] : 0.f;
       }
-      pl_split<NP>(p00, DL_ZERO, P[0]);
-      pl_split<NP>(p01, p11, P[1]);
+      pl_split<NO>(p00, DL_ZERO, P[0]);
+      pl_split<NO>(p01, p11, P[1]);
     }
     const float last = s.gam[DL_C - 1];
     const DlBuf obuf = dl_buf(o + t0 * os, min(a.T - t0, DL_C), os, a.Dv, DlIO<IO>::SIZE),
                 ubuf = dl_buf(a.U + (bh * a.T + t0) * a.Dv, a.U != nullptr ? rows : 0, a.Dv, a.Dv, 4);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vv[i] = vnext[i];
+      if (ct + 1 < CT) values(ct + 1, vnext);
       f4 x[2] = {DL_ZERO, DL_ZERO}, oo[2] = {DL_ZERO, DL_ZERO};   // oo: rows v, columns i
       if (!zero) {
 #pragma unroll
@@ -414,8 +453,8 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
           K.row(f, 16, t);
           x[1] = pl_mm<NI, NP>(f, sb, x[1]);
           if constexpr (!TRANS) {
-            oo[0] = pl_mm<NP, NI>(sb, qf[0][t], oo[0]);
-            oo[1] = pl_mm<NP, NI>(sb, qf[1][t], oo[1]);
+            oo[0] = pl_mm<NO, NI>(sb, qf[0][t], oo[0]);
+            oo[1] = pl_mm<NO, NI>(sb, qf[1][t], oo[1]);
           }
         }
       }
@@ -423,7 +462,7 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
       for (int j = 0; j < 2; ++j) {
         const f4 be = *reinterpret_cast<const f4*>(s.beta + 16 * j + 4 * kg), gam = *reinterpret_cast<const f4*>(s.gam + 16 * j + 4 * kg);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[j][r] = be[r] * (vv[ct][4 * j + r] - gam[r] * x[j][r]);
+        for (int r = 0; r < 4; ++r) x[j][r] = be[r] * (vv[4 * j + r] - gam[r] * x[j][r]);
       }
       bf16x8 xb[NP];
       pl_split<NP>(x[0], x[1], xb);
@@ -431,19 +470,24 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
       u[0] = pl_mm<NP, NP>(T[0], xb, DL_ZERO);
       u[1] = pl_mm<NP, NP>(T[1], xb, DL_ZERO);
       if constexpr (!TRANS) {
-        pl_split<NP>(u[0], u[1], xb);
+        bf16x8 ub[NO];
+        pl_split<NO>(u[0], u[1], ub);
         const int row = col0 + 16 * ct + 4 * kg, at = dl_lane(row < a.Dv, (int)(n * os + row) * DlIO<IO>::SIZE);
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
           oo[it] *= a.scale * s.gam[16 * it + n];
-          oo[it] = pl_mm<NP, NP>(xb, P[it], oo[it]);
+          oo[it] = pl_mm<NO, NO>(ub, P[it], oo[it]);
           DlIO<IO>::store4(obuf, at, (int)(16 * it * os) * DlIO<IO>::SIZE, oo[it]);
         }
         if (a.U != nullptr) {
           const int col = col0 + 16 * ct + n, up = dl_lane(col < cols, (4 * kg * a.Dv + col) * 4);
+          int to = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            DlIO<float>::store1(ubuf, up, (16 * (i >> 2) + (i & 3)) * a.Dv * 4, u[i >> 2][i & 3]);
+          for (int i = 0; i < 8; ++i) {
+            asm volatile("" : "+s"(to));
+            DlIO<float>::store1(ubuf, up, to, u[i >> 2][i & 3]);
+            to += (i == 3 ? 13 : 1) * a.Dv * 4;
+          }
         }
       }
 #pragma unroll
@@ -504,9 +548,13 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
   const int nc = (len + DL_C - 1) / DL_C, cfrom = seg * a.per, cend = a.nseg == 1 ? nc : min(nc, cfrom + a.per);
   for (int c = cend - 1; c >= cfrom; --c) {
     const int t0 = c * DL_C, left = len - t0;
-    if (!LOCAL && c < nC - 1) dl_state_store<CT, 2 * KT>(S, a.dS + (bh * (nC - 1) + c) * size, a.Dk, a.Dv, col0);
     const int rows = min(left, DL_C);
     const DlBuf gbuf = dl_buf(d_o + t0 * a.dos[1], rows, a.dos[1], a.Dv, DlIO<IO>::SIZE);
+    DlTile<IO, DP, 64> kt, qt;
+    kt.load(dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
+    qt.load(dl_buf(q + t0 * a.qs[1], rows, a.qs[1], a.Dk, DlIO<IO>::SIZE), a.qs[1], a.Dk, lane);
+    float gates[2];
+    dl_gates_load(gates, a, b, h, t0, len);
     f4 go[CT][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -515,11 +563,12 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
       for (int i = 0; i < 8; ++i)
         go[ct][i >> 2][i & 3] = DlIO<IO>::load1(gbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.dos[1]) * DlIO<IO>::SIZE);
     }
-    __syncthreads();
-    dl_load<IO, DP, 64>(K, dl_buf(k + t0 * a.ks[1], rows, a.ks[1], a.Dk, DlIO<IO>::SIZE), a.ks[1], a.Dk, lane);
-    dl_load<IO, DP, 64>(Q, dl_buf(q + t0 * a.qs[1], rows, a.qs[1], a.Dk, DlIO<IO>::SIZE), a.qs[1], a.Dk, lane);
-    dl_gates(s, a, b, h, t0, len);
-    __syncthreads();
+    if (!LOCAL && c < nc - 1) dl_state_store<CT, 2 * KT>(S, a.dS + (bh * (nC - 1) + c) * size, a.Dk, a.Dv, col0);
+    dl_fence();
+    kt.put(K, lane);
+    qt.put(Q, lane);
+    dl_gates(s, gates);
+    dl_fence();
     bf16x8 T[2][NP], P[2][NP];
     dl_inverse<DP, NI, false>(K, s, Ad, T);
     {
@@ -684,12 +733,15 @@ __global__ __launch_bounds__(4 * DP) void k_delta_join(DeltaArgs a) {
 
 // -------------------------------------- backward, the rest of a chunk's gradients ----
 // One workgroup per (row, key head, chunk), independent of the others; the value heads of a key head one after the
-// other, their dq and dk summed in registers (no atomics: the same result every time).  Two waves, one per 16 rows; four
-// where there are more than 64 key columns, half of them each (wave w: rows of tile w & 1, half w >> 1).  The contractions over the value columns,
+// other, their dq and dk summed in registers (no atomics: the same result every time).  Two waves, one per 16 positions
+// i; four where there are more than 64 key columns, half of them each.  The contractions over the value columns,
 //     dP = dO Uᵀ,  dA = −dX Uᵀ,  E1 = dO Sᵀ,  E2 = dX Sᵀ,  E3 = U dS'ᵀ,
 // read their operands straight from memory (rows of contiguous values are what an operand's lanes want); then
 //     dQ = scale e^G E1 + M1 K,  dK = M1ᵀ Q + (M2 + M2ᵀ) K − b e^G E2 + D_end E3,  M1 = scale D dP,  M2 = b D dA
-// with M1 and M2 passed through LDS, and the scalars' gradients from row and column sums.
+// with M1 and M2 passed through LDS, and the scalars' gradients from their row and column sums.  Every product is made
+// with the position i as its column, so a lane's scalars are one position's and its four results lie side by side.
+// What bounds it is the chain of loads, products and sums (vector instructions are issued 40 % of the time, most of
+// them splitting operands into planes).  Three waves a SIMD spill 52 registers and cost 20 %.
 template <int DP, int NI>
 struct DlGradLds {
   static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, M = PlaneMat<DL_C, 32, DL_NP>::BYTES;
@@ -698,268 +750,313 @@ struct DlGradLds {
   static constexpr int BYTES = 2 * KQ + 2 * M + (int)sizeof(DlGates) + SUMS;
 };
 
-__device__ __forceinline__ float dl_sum16(float x) {   // over the 16 lanes of a group
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
+// sum over the 16 lanes of a group, by rotations of a row of lanes
+__device__ __forceinline__ float dl_sum16(float x) {
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xf, 0xf, true));
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xf, 0xf, true));
   return x;
+}
+// sum over the four groups
+__device__ __forceinline__ float dl_sum4(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
 }
 
+// four neighbouring columns c .. c + 3 (c a multiple of 4) of a matrix in planes
 template <int R, int C, int N>
-__device__ __forceinline__ float dl_get(const PlaneMat<R, C, N>& m, int r, int c) {
+__device__ __forceinline__ f4 dl_get4(const PlaneMat<R, C, N>& m, int r, int c) {
   const __bf16* p = m.p + r * PlaneMat<R, C, N>::LD + pl_place(c);
-  float x = 0.f;
+  f4 x = DL_ZERO;
 #pragma unroll
-  for (int q = N - 1; q >= 0; --q) x += (float)p[q * PlaneMat<R, C, N>::PLANE];
+  for (int q = N - 1; q >= 0; --q) {
+    const dl_u2 u = *reinterpret_cast<const dl_u2*>(p + q * PlaneMat<R, C, N>::PLANE);
+    x += (f4){__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16),
+              __uint_as_float(u[1] & 0xffff0000u)};
+  }
   return x;
 }
+template <int R, int C, int N>
+__device__ __forceinline__ void dl_put4(const PlaneMat<R, C, N>& m, int r, int c, const f4& x) {
+  bf16x8 f[N];
+  pl_split<N>(x, DL_ZERO, f);
+  __bf16* p = m.p + r * PlaneMat<R, C, N>::LD + pl_place(c);
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const pl_s8 v = __builtin_bit_cast(pl_s8, f[q]);
+    *reinterpret_cast<pl_s4*>(p + q * PlaneMat<R, C, N>::PLANE) = (pl_s4){v[0], v[1], v[2], v[3]};
+  }
+}
+
+// 8 values of an operand as fp32, and their products' sum with another's
+struct DlRow {
+  f4 a, b;
+  __device__ __forceinline__ void load(DlBuf buf, int row, int64_t st, int c0, int D) {
+    const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, v = (int)(n * st + 4 * kg) * 4;
+    a = DlIO<float>::load4(buf, dl_lane(c0 + 4 * kg < D, v), (int)(row * st + c0) * 4);
+    b = DlIO<float>::load4(buf, dl_lane(c0 + 16 + 4 * kg < D, v), (int)(row * st + c0 + 16) * 4);
+  }
+  __device__ __forceinline__ void planes(bf16x8* f) const { pl_split<DL_NP>(a, b, f); }
+  __device__ __forceinline__ float dot(const f4& x, const f4& y, float s) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = __builtin_fmaf(a[i], x[i], __builtin_fmaf(b[i], y[i], s));
+    return s;
+  }
+};
 
 template <typename IO, int DP>
 __global__ __launch_bounds__(DP > 64 ? 256 : 128, 2) void k_delta_grads(DeltaArgs a) {
   using L = DlGradLds<DP, DlIO<IO>::N>;
-  constexpr int NI = DlIO<IO>::N, NP = DL_NP, HALVES = L::HALVES, THREADS = L::THREADS;
-  constexpr int UT = DP / 16 / HALVES;   // key tiles of a wave
+  constexpr int NI = DlIO<IO>::N, NP = DL_NP, HALVES = L::HALVES, THREADS = L::THREADS, SIZE = DlIO<IO>::SIZE;
+  constexpr int UT = DP / 16 / HALVES;   // key tiles of a wave, taken in pairs
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds}, Q{(__bf16*)(lds + L::KQ)};
   const PlaneMat<DL_C, 32, NP> M1{(__bf16*)(lds + 2 * L::KQ)}, M2{(__bf16*)(lds + 2 * L::KQ + L::M)};
   DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::M);
-  float* colsum = (float*)(lds + 2 * L::KQ + 2 * L::M + sizeof(DlGates));   // [2 row tiles][32]
-  float* part = colsum + 2 * 32;      // [3][halves][32]: q·E1, k·E2, k·E3
-  float* rows = part + 3 * HALVES * 32;    // [3][32]: row sums of M, of the terms of dbeta, dX·V
-  float* dots = rows + 3 * 32;        // [4] sums of S·dS'
+  float* colsum = (float*)(lds + 2 * L::KQ + 2 * L::M + sizeof(DlGates));   // [2 tiles of i][32]
+  float* part = colsum + 2 * 32;               // [3][halves][32]: q·E1, k·E2, k·E3
+  float* rows = part + 3 * HALVES * 32;        // [3][32]: row sums of M, of the terms of dbeta, dX·V
+  float* dots = rows + 3 * 32;                 // [2] sums of S·dS' by halves
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), it = wave & 1, half = wave >> 1;
   const int group = a.Hv / a.Hk, b = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk, c = blockIdx.y, t0 = c * DL_C;
   const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C, nc = (len + DL_C - 1) / DL_C;
-  IO* dq = (IO*)a.dq + ((int64_t)b * a.T * a.Hk + hk) * a.Dk;
-  IO* dk = (IO*)a.dk + ((int64_t)b * a.T * a.Hk + hk) * a.Dk;
   const int64_t ks = (int64_t)a.Hk * a.Dk;
-
-  if (c >= nc) {
-    const int end = min(a.T, t0 + DL_C);
-    for (int e = tid; e < (end - t0) * a.Dk; e += THREADS) {
-      dq[(t0 + e / a.Dk) * ks + e % a.Dk] = (IO)0.f;
-      dk[(t0 + e / a.Dk) * ks + e % a.Dk] = (IO)0.f;
+  const int i = 16 * it + n, d0 = half * 64;   // this lane's position, this wave's key columns
+  const int outrows = min(a.T - t0, DL_C);
+  const DlBuf dqbuf = dl_buf((IO*)a.dq + (((int64_t)b * a.T + t0) * a.Hk + hk) * a.Dk, outrows, ks, a.Dk, SIZE),
+              dkbuf = dl_buf((IO*)a.dk + (((int64_t)b * a.T + t0) * a.Hk + hk) * a.Dk, outrows, ks, a.Dk, SIZE);
+  auto store = [&](const f4* gq, const f4* gk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < UT; ++u) {
+      const int at = dl_lane(d0 + 16 * u + 4 * kg < a.Dk, (int)(i * ks + 4 * kg) * SIZE);
+      DlIO<IO>::store4(dqbuf, at, (d0 + 16 * u) * SIZE, gq[u]);
+      DlIO<IO>::store4(dkbuf, at, (d0 + 16 * u) * SIZE, gk[u]);
     }
-    for (int e = tid; e < (end - t0) * group; e += THREADS) {
-      const int64_t at = ((int64_t)b * a.T + t0 + e / group) * a.Hv + hk * group + e % group;
-      a.dg[at] = 0.f;
-      a.dbeta[at] = 0.f;
-    }
-    return;
-  }
-
-  const int left = min(len - t0, DL_C), d0 = half * 64;
-  dl_load<IO, DP, THREADS>(K, dl_buf((const IO*)a.k + b * a.ks[0] + hk * a.ks[2] + t0 * a.ks[1], left, a.ks[1], a.Dk, DlIO<IO>::SIZE),
-                       a.ks[1], a.Dk, tid);
-  dl_load<IO, DP, THREADS>(Q, dl_buf((const IO*)a.q + b * a.qs[0] + hk * a.qs[2] + t0 * a.qs[1], left, a.qs[1], a.Dk, DlIO<IO>::SIZE),
-                       a.qs[1], a.Dk, tid);
-  f4 gq[UT], gk[UT];
+  };
+  f4 gq[UT], gk[UT];   // rows: key columns, columns: positions
 #pragma unroll
   for (int u = 0; u < UT; ++u) gq[u] = gk[u] = DL_ZERO;
-  const bool live = 16 * it < left;   // this wave's rows hold any position
+  if (c >= nc) {   // behind the row's length
+    store(gq, gk);
+    if (tid < outrows)
+      for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        const int64_t at = ((int64_t)b * a.T + t0 + tid) * a.Hv + h;
+        a.dg[at] = 0.f;
+        a.dbeta[at] = 0.f;
+      }
+    return;
+  }
+  const int left = min(len - t0, DL_C);
+
+  // K and Q are on their way while the first value head's contractions run
+  DlTile<IO, DP, THREADS> kt, qt;
+  kt.load(dl_buf((const IO*)a.k + b * a.ks[0] + hk * a.ks[2] + t0 * a.ks[1], left, a.ks[1], a.Dk, SIZE), a.ks[1], a.Dk, tid);
+  qt.load(dl_buf((const IO*)a.q + b * a.qs[0] + hk * a.qs[2] + t0 * a.qs[1], left, a.qs[1], a.Dk, SIZE), a.qs[1], a.Dk, tid);
 
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     const int64_t bh = (int64_t)b * a.Hv + h, size = (int64_t)a.Dk * a.Dv;
     const float* S0 = c > 0 ? a.S0 + (bh * (nC - 1) + c - 1) * size : a.state0 ? a.state0 + bh * size : nullptr;
+    // (after the last chunk of the row's length: the gradient handed in)
     const float* dS = c < nc - 1 ? a.dS + (bh * (nC - 1) + c) * size : a.dstate ? a.dstate + bh * size : nullptr;
-    // a length that ends on this chunk: what stands behind it is the gradient handed in
-    const float* U = a.U + (bh * a.T + t0) * a.Dv;
-    const float* dX = a.dX + (bh * a.T + t0) * a.Dv;
-    const DlBuf gbuf = dl_buf((const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + t0 * a.dos[1], left, a.dos[1], a.Dv,
-                              DlIO<IO>::SIZE),
-                xbuf = dl_buf(dX, left, a.Dv, a.Dv, 4), ubuf = dl_buf(U, left, a.Dv, a.Dv, 4),
-                sbuf = dl_buf(S0, a.Dk, a.Dv, a.Dv, 4), ebuf = dl_buf(dS, a.Dk, a.Dv, a.Dv, 4);
-    const IO* v = (const IO*)a.v + b * a.vs[0] + h * a.vs[2];
+    const DlBuf gbuf = dl_buf((const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + t0 * a.dos[1], left, a.dos[1], a.Dv, SIZE),
+                vbuf = dl_buf((const IO*)a.v + b * a.vs[0] + h * a.vs[2] + t0 * a.vs[1], left, a.vs[1], a.Dv, SIZE),
+                xbuf = dl_buf(a.dX + (bh * a.T + t0) * a.Dv, left, a.Dv, a.Dv, 4),
+                ubuf = dl_buf(a.U + (bh * a.T + t0) * a.Dv, left, a.Dv, a.Dv, 4),
+                sbuf = dl_buf(S0, S0 != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4),
+                ebuf = dl_buf(dS, dS != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4);
+    float gates[2];
+    if (wave == 0) dl_gates_load(gates, a, b, h, t0, len);
 
-    if (wave == 0) dl_gates(s, a, b, h, t0, len);
-    // dP, dA: the diagonal tile, and the tile below it (of the second row tile)
-    f4 dp = DL_ZERO, da = DL_ZERO, dp0 = DL_ZERO, da0 = DL_ZERO, e1[UT], e2[UT], e3[UT];
-#pragma unroll
-    for (int u = 0; u < UT; ++u) e1[u] = e2[u] = e3[u] = DL_ZERO;
-    if (live) {
+    // dP, dA: the diagonal tile, and (second tile of positions) the one with the first tile of j
+    f4 dp = DL_ZERO, da = DL_ZERO, dp0 = DL_ZERO, da0 = DL_ZERO;
+    float dot = 0.f;
+    if (half == 0) {
       for (int c0 = 0; c0 < a.Dv; c0 += 32) {
         bf16x8 go[NI], gx[NP], uu[NP], y[NP];
+        DlRow rx, ru, ry;
         dl_operand<IO>(go, gbuf, 16 * it, a.dos[1], c0, a.Dv);
-        dl_operand<float>(gx, xbuf, 16 * it, a.Dv, c0, a.Dv);
-        dl_operand<float>(uu, ubuf, 16 * it, a.Dv, c0, a.Dv);
-        dp = pl_mm<NI, NP>(go, uu, dp);
-        da = pl_mm<NP, NP>(gx, uu, da);
+        rx.load(xbuf, 16 * it, a.Dv, c0, a.Dv);
+        ru.load(ubuf, 16 * it, a.Dv, c0, a.Dv);
+        ry.load(ubuf, 0, a.Dv, c0, a.Dv);
+        f4 v0, v1;
+        {
+          const int v = (int)(n * a.vs[1] + 4 * kg) * SIZE, sv = (int)(16 * it * a.vs[1] + c0) * SIZE;
+          DlIO<IO>::load4x2(vbuf, dl_lane(c0 + 4 * kg < a.Dv, v), sv, dl_lane(c0 + 16 + 4 * kg < a.Dv, v), sv + 16 * SIZE, v0, v1);
+        }
+        rx.planes(gx);
+        ru.planes(uu);
+        dp = pl_mm<NP, NI>(uu, go, dp);
+        da = pl_mm<NP, NP>(uu, gx, da);
         if (it == 1) {
-          dl_operand<float>(y, ubuf, 0, a.Dv, c0, a.Dv);
-          dp0 = pl_mm<NI, NP>(go, y, dp0);
-          da0 = pl_mm<NP, NP>(gx, y, da0);
+          ry.planes(y);
+          dp0 = pl_mm<NP, NI>(y, go, dp0);
+          da0 = pl_mm<NP, NP>(y, gx, da0);
         }
-        if (S0 != nullptr) {
-#pragma unroll
-          for (int u = 0; u < UT; ++u) {
-            dl_operand<float>(y, sbuf, d0 + 16 * u, a.Dv, c0, a.Dv);
-            e1[u] = pl_mm<NI, NP>(go, y, e1[u]);
-            e2[u] = pl_mm<NP, NP>(gx, y, e2[u]);
-          }
-        }
-        if (dS != nullptr) {
-#pragma unroll
-          for (int u = 0; u < UT; ++u) {
-            dl_operand<float>(y, ebuf, d0 + 16 * u, a.Dv, c0, a.Dv);
-            e3[u] = pl_mm<NP, NP>(uu, y, e3[u]);
-          }
-        }
+        dot = rx.dot(v0, v1, dot);
       }
+      dot = dl_sum4(dot);
+      if (kg == 0) rows[2 * 32 + i] = dot;
     }
-    // dX · V of each row: four (eight) threads a row
-    {
-      constexpr int PER = THREADS / 32;
-      const int r = tid / PER;
-      float x = 0.f;
-      if (r < left)
-        for (int cc = tid % PER * 4; cc < a.Dv; cc += 4 * PER)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x = __builtin_fmaf(dX[(int64_t)r * a.Dv + cc + i], (float)v[(int64_t)(t0 + r) * a.vs[1] + cc + i], x);
-#pragma unroll
-      for (int o = 1; o < PER; o <<= 1) x += __shfl_xor(x, o);
-      if (tid % PER == 0) rows[2 * 32 + r] = x;
+    if (wave == 0) dl_gates(s, gates);
+    if (h == hk * group) {
+      kt.put(K, tid);
+      qt.put(Q, tid);
     }
-    float both = 0.f;
-    if (S0 != nullptr && dS != nullptr) {
-      for (int e = tid * 4; e < a.Dk * a.Dv; e += 4 * THREADS) {
-        const f4 x = *reinterpret_cast<const f4*>(S0 + e), y = *reinterpret_cast<const f4*>(dS + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) both = __builtin_fmaf(x[i], y[i], both);
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) both += __shfl_xor(both, o);
-    }
-    if (lane == 0) dots[wave] = both;
-    __syncthreads();   // K, Q, gates
+    __syncthreads();
+    const float gam = s.gam[i], be = s.beta[i], rest = s.rest[i];
     if (half == 0) {
-      float rm[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
+      float rm = 0.f, rb = 0.f;
+      const double gi = s.G[i];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        f4 kk = DL_ZERO, qk = DL_ZERO;
-        if (j <= it && live) {
+        f4 kk = DL_ZERO, qk = DL_ZERO, m1 = DL_ZERO, m2 = DL_ZERO, cs = DL_ZERO;
+        if (j <= it) {
 #pragma unroll
           for (int t = 0; t < DP / 32; ++t) {
             bf16x8 ki[NI], qi[NI], kj[NI];
             K.row(ki, 16 * it, t);
             Q.row(qi, 16 * it, t);
             K.row(kj, 16 * j, t);
-            kk = pl_mm<NI, NI>(ki, kj, kk);
-            qk = pl_mm<NI, NI>(qi, kj, qk);
+            kk = pl_mm<NI, NI>(kj, ki, kk);
+            qk = pl_mm<NI, NI>(kj, qi, qk);
           }
-        }
-        const int jj = 16 * j + n;
-        float cs = 0.f;
+          const f4 dpj = j == it ? dp : dp0, daj = j == it ? da : da0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * it + 4 * kg + r;
-          const float dpr = j == it ? dp[r] : dp0[r], dar = j == it ? da[r] : da0[r];
-          float m1 = 0.f, m2 = 0.f;
-          if (jj <= i) {
-            const float d = dl_exp2(s.G[i] - s.G[jj]);
-            m1 = a.scale * d * dpr;
-            float m = m1 * qk[r];
-            if (jj < i) {
-              const float w = -d * dar;
-              m2 = s.beta[i] * w;
-              m += m2 * kk[r];
-              rb[r] += w * kk[r];
-            }
-            rm[r] += m;
-            cs += m;
+          for (int r = 0; r < 4; ++r) {
+            const int jj = 16 * j + 4 * kg + r;
+            const float d = jj <= i ? dl_exp2(gi - s.G[jj]) : 0.f;
+            const float w = jj < i ? -d * daj[r] : 0.f;
+            m1[r] = jj <= i ? a.scale * d * dpj[r] : 0.f;
+            m2[r] = be * w;
+            cs[r] = m1[r] * qk[r] + m2[r] * kk[r];
+            rm += cs[r];
+            rb += w * kk[r];
           }
-          M1.put(i, jj, m1);
-          M2.put(i, jj, m2);
         }
-        cs += __shfl_xor(cs, 16);
-        cs += __shfl_xor(cs, 32);
-        if (kg == 0) colsum[it * 32 + jj] = cs;
+        dl_put4(M1, i, 16 * j + 4 * kg, m1);
+        dl_put4(M2, i, 16 * j + 4 * kg, m2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) cs[r] = dl_sum16(cs[r]);
+        if (n == 0) *reinterpret_cast<f4*>(colsum + it * 32 + 16 * j + 4 * kg) = cs;
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x0 = dl_sum16(rm[r]), x1 = dl_sum16(rb[r]);
-        if (n == 0) {
-          rows[16 * it + 4 * kg + r] = x0;
-          rows[32 + 16 * it + 4 * kg + r] = x1;
-        }
+      rm = dl_sum4(rm);
+      rb = dl_sum4(rb);
+      if (kg == 0) {
+        rows[i] = rm;
+        rows[32 + i] = rb;
       }
     }
-    float r1[4] = {0.f, 0.f, 0.f, 0.f}, r2[4] = {0.f, 0.f, 0.f, 0.f}, r3[4] = {0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    // the states' part, two key tiles at a time
+    float r1 = 0.f, r2 = 0.f, r3 = 0.f, both = 0.f;
     if (S0 != nullptr || dS != nullptr) {
 #pragma unroll
-      for (int u = 0; u < UT; ++u)
+      for (int u0 = 0; u0 < UT; u0 += 2) {
+        f4 e1[2] = {DL_ZERO, DL_ZERO}, e2[2] = {DL_ZERO, DL_ZERO}, e3[2] = {DL_ZERO, DL_ZERO};
+        for (int c0 = 0; c0 < a.Dv; c0 += 32) {
+          bf16x8 go[NI], gx[NP], uu[NP], y[NP];
+          DlRow rx, ru, rs[2], re[2];   // (a state that is not there has no rows: nothing is read)
+          dl_operand<IO>(go, gbuf, 16 * it, a.dos[1], c0, a.Dv);
+          rx.load(xbuf, 16 * it, a.Dv, c0, a.Dv);
+          ru.load(ubuf, 16 * it, a.Dv, c0, a.Dv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * it + 4 * kg + r, d = d0 + 16 * u + n;
-          const float gam = s.gam[i], kx = dl_get(K, i, d), qx = dl_get(Q, i, d);
-          r1[r] = __builtin_fmaf(qx, e1[u][r], r1[r]);
-          r2[r] = __builtin_fmaf(kx, e2[u][r], r2[r]);
-          r3[r] = __builtin_fmaf(kx, e3[u][r], r3[r]);
-          gq[u][r] += a.scale * gam * e1[u][r];
-          gk[u][r] += s.rest[i] * e3[u][r] - s.beta[i] * gam * e2[u][r];
+          for (int u = 0; u < 2; ++u) {
+            rs[u].load(sbuf, d0 + 16 * (u0 + u), a.Dv, c0, a.Dv);
+            re[u].load(ebuf, d0 + 16 * (u0 + u), a.Dv, c0, a.Dv);
+          }
+          if (S0 != nullptr) {
+            rx.planes(gx);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              rs[u].planes(y);
+              e1[u] = pl_mm<NP, NI>(y, go, e1[u]);
+              e2[u] = pl_mm<NP, NP>(y, gx, e2[u]);
+            }
+          }
+          if (dS != nullptr) {
+            ru.planes(uu);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              re[u].planes(y);
+              e3[u] = pl_mm<NP, NP>(y, uu, e3[u]);
+              both = rs[u].dot(re[u].a, re[u].b, both);
+            }
+          }
         }
-    }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * it + 4 * kg + r;
-      const float x2 = dl_sum16(r1[r]), x3 = dl_sum16(r2[r]), x4 = dl_sum16(r3[r]);
-      if (n == 0) {
-        part[half * 32 + i] = x2;
-        part[(HALVES + half) * 32 + i] = x3;
-        part[(2 * HALVES + half) * 32 + i] = x4;
+        for (int u = 0; u < 2; ++u) {
+          const f4 kx = dl_get4(K, i, d0 + 16 * (u0 + u) + 4 * kg), qx = dl_get4(Q, i, d0 + 16 * (u0 + u) + 4 * kg);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            r1 = __builtin_fmaf(qx[r], e1[u][r], r1);
+            r2 = __builtin_fmaf(kx[r], e2[u][r], r2);
+            r3 = __builtin_fmaf(kx[r], e3[u][r], r3);
+          }
+          gq[u0 + u] += (a.scale * gam) * e1[u];
+          gk[u0 + u] += rest * e3[u] - (be * gam) * e2[u];
+        }
+      }
+      r1 = dl_sum4(r1);
+      r2 = dl_sum4(r2);
+      r3 = dl_sum4(r3);
+      both = dl_sum4(dl_sum16(both));
+    }
+    if (kg == 0) {
+      part[half * 32 + i] = r1;
+      part[(HALVES + half) * 32 + i] = r2;
+      part[(2 * HALVES + half) * 32 + i] = r3;
+    }
+    if (it == 0 && lane == 0) dots[half] = both;
+    {
+      bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
+      M1.row(m1, 16 * it, 0);
+      M2.row(m2, 16 * it, 0);
+      M1.col(m1t, 0, 16 * it);
+      M2.col(m2t, 0, 16 * it);
+#pragma unroll
+      for (int u = 0; u < UT; ++u) {
+        bf16x8 f[NI];
+        K.col(f, 0, d0 + 16 * u);
+        gq[u] = pl_mm<NI, NP>(f, m1, gq[u]);
+        gk[u] = pl_mm<NI, NP>(f, m2, gk[u]);
+        gk[u] = pl_mm<NI, NP>(f, m2t, gk[u]);
+        Q.col(f, 0, d0 + 16 * u);
+        gk[u] = pl_mm<NI, NP>(f, m1t, gk[u]);
       }
     }
     __syncthreads();
     if (wave == 0) {
-      const int i = lane & 31;
-      const float gam = s.gam[i], be = s.beta[i];
-      float qe = part[i], ke = part[HALVES * 32 + i], kd = part[2 * HALVES * 32 + i];
-      if (HALVES == 2) qe += part[32 + i], ke += part[3 * 32 + i], kd += part[5 * 32 + i];
-      const double leave = (double)s.rest[i] * kd;
-      double at = (double)rows[i] + (double)a.scale * gam * qe - (double)be * gam * ke - leave;
-      at -= (double)colsum[i] + (double)colsum[32 + i];
+      const int j = lane & 31;
+      const float gj = s.gam[j];
+      float qe = part[j], ke = part[HALVES * 32 + j], kd = part[2 * HALVES * 32 + j];
+      if (HALVES == 2) qe += part[32 + j], ke += part[3 * 32 + j], kd += part[5 * 32 + j];
+      const double leave = (double)s.rest[j] * kd;
+      double at = (double)rows[j] + (double)a.scale * gj * qe - (double)s.beta[j] * gj * ke - leave;
+      at -= (double)colsum[j] + (double)colsum[32 + j];
       double all = leave;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         all += __shfl_xor(all, o, 32);
         const double down = __shfl_down(at, o, 32);
-        if (i + o < 32) at += down;
+        if (j + o < 32) at += down;
       }
-      at += all + (double)s.gam[DL_C - 1] * ((double)dots[0] + dots[1] + (HALVES == 2 ? (double)dots[2] + dots[3] : 0.0));
-      const int64_t out = ((int64_t)b * a.T + t0 + i) * a.Hv + h;
-      if (lane < 32 && t0 + i < a.T) {
-        a.dg[out] = t0 + i < len ? (float)at : 0.f;
-        a.dbeta[out] = t0 + i < len ? rows[64 + i] - gam * ke + rows[32 + i] : 0.f;
+      at += all + (double)s.gam[DL_C - 1] * (HALVES == 2 ? (double)dots[0] + dots[1] : (double)dots[0]);
+      const int64_t out = ((int64_t)b * a.T + t0 + j) * a.Hv + h;
+      if (lane < 32 && j < outrows) {
+        a.dg[out] = j < left ? (float)at : 0.f;
+        a.dbeta[out] = j < left ? rows[64 + j] - gj * ke + rows[32 + j] : 0.f;
       }
     }
-    bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
-    M1.row(m1, 16 * it, 0);
-    M2.row(m2, 16 * it, 0);
-    M1.col(m1t, 0, 16 * it);
-    M2.col(m2t, 0, 16 * it);
-#pragma unroll
-    for (int u = 0; u < UT; ++u) {
-      bf16x8 f[NI];
-      K.col(f, 0, d0 + 16 * u);
-      gq[u] = pl_mm<NP, NI>(m1, f, gq[u]);
-      gk[u] = pl_mm<NP, NI>(m2, f, gk[u]);
-      gk[u] = pl_mm<NP, NI>(m2t, f, gk[u]);
-      Q.col(f, 0, d0 + 16 * u);
-      gk[u] = pl_mm<NP, NI>(m1t, f, gk[u]);
-    }
-    __syncthreads();   // sums and M1, M2 are read: the next value head may write them
+    if (h + 1 < (hk + 1) * group) __syncthreads();   // the sums are read: the next value head may write them
   }
+  if (i >= left) {
 #pragma unroll
-  for (int u = 0; u < UT; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = t0 + 16 * it + 4 * kg + r, d = d0 + 16 * u + n;
-      if (t < a.T && d < a.Dk) {
-        dq[t * ks + d] = (IO)(t < len ? gq[u][r] : 0.f);
-        dk[t * ks + d] = (IO)(t < len ? gk[u][r] : 0.f);
-      }
-    }
+    for (int u = 0; u < UT; ++u) gq[u] = gk[u] = DL_ZERO;
+  }
+  store(gq, gk);
 }
 
 // ------------------------------------------------------------- one token ----
@@ -1067,21 +1164,28 @@ static int delta_ct(int64_t heads, int Dk, int Dv, int type) {
   return ct;
 }
 
-// Segments.  One pass takes about a chunk's 5 us per chunk in sequence; with segments there are two (the first also over
-// the transition's columns), each a segment long, and a join of about 2 us a segment.  2048 waves run at once.
+// Segments.  A chunk takes a wave of 1, 2, 4 column tiles about 4.5, 7.5, 12 us with a SIMD of its own (1024 of them), 1.75
+// times that beside another (2048 at once); with segments there are two passes, the first over the transition's
+// columns too but without outputs, each a segment long, and a join of about 1 us a segment.  Measured at width 128,
+// 4 x 8 heads x 4096 positions, forward and backward: 8 segments 819 us, 16 749, 32 808, 64 960; 8 heads x 8191
+// positions, forward: 8 segments 269 us, 16 188, 32 192, 37 (a wave too many for the SIMDs in either pass) 225, 64 241.
 struct DeltaCut {
   int nseg, per;
 };
 static DeltaCut delta_cut(int B, int T, int Hv, int Dk, int Dv) {
   const int nC = (T + DL_C - 1) / DL_C;
+  const int64_t heads = (int64_t)B * Hv;
+  auto chunk = [&](int nseg, int cols) {
+    const int ct = delta_ct(heads * nseg, Dk, Dv, 1);
+    const int64_t waves = heads * nseg * ((cols + 16 * ct - 1) / (16 * ct));
+    return (ct == 1 ? 4.5 : ct == 2 ? 7.5 : 12.0) * (waves > 1024 ? 1.75 : 1.0) * (double)((waves + 2047) / 2048);
+  };
   DeltaCut best = {1, nC};
-  const int64_t heads = (int64_t)B * Hv, vw = (Dv + 31) / 32, kw = (Dk + 31) / 32;
-  auto rounds = [](int64_t waves) { return (double)((waves + 2047) / 2048); };
-  double cost = rounds(heads * vw) * nC * 5.0;
-  for (int want = 2; want <= 64 && want <= nC; want *= 2) {
+  double cost = nC * chunk(1, Dv);
+  for (int want = 2; want <= 64 && want <= nC; ++want) {
     const int per = (nC + want - 1) / want, nseg = (nC + per - 1) / per;
-    const double t = (rounds(heads * nseg * vw) + rounds(heads * nseg * (vw + kw))) * per * 5.0 + 2.0 * nseg + 10.0;
-    if (t < 0.8 * cost) cost = t, best = {nseg, per};
+    const double t = per * (chunk(nseg, Dv) + 0.7 * chunk(nseg, Dv + Dk)) + 1.06 * nseg + 15.0;
+    if (t < cost) cost = t, best = {nseg, per};
   }
   return best;
 }

@@ -86,10 +86,12 @@ CASES = [
     (3, 193, 2, 2, 24, 40, [193, 128, 70], True),
     (1, 700, 1, 2, 64, 128, None, True),
     (300, 33, 1, 1, 64, 64, list(range(33)) * 9 + [3, 33, 0], False),
+    (900, 50, 1, 2, 64, 64, [1 + 50 * i // 900 for i in range(900)], False),
+    (2, 1100, 2, 2, 128, 96, [1100, 517], True),
 ]
 
 
-@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:6])))
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_forward_and_backward(case, dtype):
     from recommenders.hip.delta import delta_rule, delta_rule_backward
