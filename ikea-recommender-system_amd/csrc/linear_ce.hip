@@ -63,8 +63,8 @@ struct CeArgs {
   const int* count;        // packed rows
   const float* bias;       // (V) or null
   const float* recs;       // backward: [chunk][3][64] log2 |g| − lse · log2 e, g, target (as int bits)
-  int nsplit, nblock;
-  float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][V][D], pl slabs [split][V]
+  int nsplit, nblock, block0;   // blocks of X: nblock of them, from block0 on
+  float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][items from block0 on][D], pl likewise
   void* dW;
   float* db;
   const float* scale;      // backward: {factor on g, its inverse}; null: 1
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     split = blockIdx.x / a.nblock;
     block = blockIdx.x % a.nblock;
   }
+  block += a.block0;
   const int rows = *a.count;
   const int nx = FWD ? rows : a.nx, ny = FWD ? a.ny : rows;
   const int x0 = block * 16 * NX * NW + wave * 16 * NX;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     } else {
       const float back = (a.scale != nullptr ? a.scale[1] : 1.f) * (BIAS && whole ? __builtin_amdgcn_exp2f(xb[t]) : 1.f);
       if (a.nsplit > 1) {
-        const int64_t at = (int64_t)split * a.nx + x;
+        const int64_t first = (int64_t)a.block0 * 16 * NX * NW, at = split * (a.nx - first) + x - first;
         if (a.db != nullptr && kg == 0) a.pl[at] = sum[t] * back;
 #pragma unroll
         for (int f = 0; f < FB; ++f)
@@ -342,42 +343,57 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 }
 
 // Rows with a target >= 0, in order: tc (their targets, −1 for one that is no item), rows (their places), inv (the way
-// back, −1: ignored), count; the losses of ignored rows.  One workgroup, a run of rows per thread.
-__global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ tgt, int64_t st, int N, int npad, int V,
-                                                  int* __restrict__ count, int* __restrict__ rows,
-                                                  int* __restrict__ tc, int* __restrict__ inv,
-                                                  float* __restrict__ loss) {
+// back, −1: ignored), count; the losses of ignored rows.  A workgroup lists 1024 rows; with more than one the
+// groups' counts come first.
+__global__ __launch_bounds__(1024) void k_ce_count(const int64_t* __restrict__ tgt, int64_t st, int N, int* __restrict__ counts) {
   __shared__ int part[16];
-  const int tid = threadIdx.x, per = (N + 1023) / 1024, lo = min(N, tid * per), hi = min(N, lo + per);
-  int k = 0;
-  for (int r = lo; r < hi; ++r) k += tgt[r * st] >= 0;
-  int up = k;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(up, o);
-    if ((tid & 63) >= o) up += x;
-  }
-  if ((tid & 63) == 63) part[tid >> 6] = up;
+  const int r = blockIdx.x * 1024 + threadIdx.x;
+  const uint64_t on = __ballot(r < N && tgt[r < N ? r * st : 0] >= 0);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = __popcll(on);
   __syncthreads();
-  int all = 0;
+  if (threadIdx.x == 0) {
+    int k = 0;
+    for (int w = 0; w < 16; ++w) k += part[w];
+    counts[blockIdx.x] = k;
+  }
+}
+__global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ tgt, int64_t st, int N, int npad, int V,
+                                                  const int* __restrict__ counts, int* __restrict__ count,
+                                                  int* __restrict__ rows, int* __restrict__ tc, int* __restrict__ inv,
+                                                  float* __restrict__ loss) {
+  __shared__ int part[16], before[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x * 1024 + tid;
+  const int64_t t = tgt[r < N ? r * st : 0];
+  const bool on = r < N && t >= 0;
+  const uint64_t mask = __ballot(on);
+  int base = 0;
+  for (int i = tid; i < (int)blockIdx.x; i += 1024) base += counts[i];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) base += __shfl_xor(base, o);
+  if (lane == 0) {
+    part[wave] = __popcll(mask);
+    before[wave] = base;
+  }
+  __syncthreads();
+  int at = 0, all = 0;
   for (int w = 0; w < 16; ++w) {
-    if (w < (tid >> 6)) up += part[w];
-    all += part[w];
+    at += before[w];
+    all += before[w] + part[w];
+    if (w < wave) at += part[w];
   }
-  int at = up - k;
-  for (int r = lo; r < hi; ++r) {
-    const int64_t t = tgt[r * st];
-    if (t >= 0) {
-      rows[at] = r;
-      tc[at] = t < V ? (int)t : -1;
-      inv[r] = at++;
-    } else {
-      inv[r] = -1;
-      loss[r] = 0.f;
-    }
+  at += __popcll(mask & ((1ull << lane) - 1));
+  if (on) {
+    rows[at] = r;
+    tc[at] = t < V ? (int)t : -1;
+    inv[r] = at;
+  } else if (r < N) {
+    inv[r] = -1;
+    loss[r] = 0.f;
   }
-  if (tid == 0) *count = all;
-  for (int c = all + tid; c < npad; c += 1024) rows[c] = -1;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (tid == 0) *count = all;
+    for (int c = all + tid; c < npad; c += 1024) rows[c] = -1;
+  }
 }
 
 // packed copy of the listed rows, zeros behind column D and behind the last row
@@ -424,12 +440,21 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
     lse[c] = all;
   }
   if constexpr (GRAD) {
+    // DP / 4 lanes per split, several splits at once
     const float one = 1.f / l;
-    for (int f = lane; f < D; f += 64) {
-      float o = 0.f;
-      for (int s = 0; s < nsplit; ++s)
-        o = __builtin_fmaf(pO[((int64_t)s * N + c) * DP + f], __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m), o);
-      dh[(int64_t)c * D + f] = t < 0 ? __builtin_nanf("") : __builtin_fmaf(o, one, -(float)w[f]);
+    const int per = DP / 4, f = lane % per * 4;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = lane / per; s < nsplit; s += 64 / per)
+      o += *reinterpret_cast<const f4*>(pO + ((int64_t)s * N + c) * DP + f) * __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m);
+    for (int x = per; x < 64; x <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
+    if (lane < per && f < D) {
+      f4 d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = t < 0 ? __builtin_nanf("") : __builtin_fmaf(o[i], one, -(float)w[f + i]);
+      *reinterpret_cast<f4*>(dh + (int64_t)c * D + f) = d;
     }
   }
 }
@@ -439,8 +464,11 @@ __global__ __launch_bounds__(1024) void k_ce_scale(const float* __restrict__ g, 
                                                    int N, float* __restrict__ scale) {
   __shared__ float part[16];
   float m = 0.f;
-  for (int r = threadIdx.x; r < N; r += 1024)
-    if (inv[r] >= 0) m = fmaxf(m, fabsf(g[r * sg]));
+#pragma unroll 8
+  for (int r = threadIdx.x; r < N; r += 1024) {
+    const float x = fabsf(g[r * sg]);
+    m = inv[r] >= 0 ? fmaxf(m, x) : m;
+  }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
@@ -513,26 +541,29 @@ static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // a workgroup holds CE_NW · CE_NX · 16 = 256 rows of X: eight waves, two on a SIMD, so that one's exponentials run beside
 // the other's MFMAs, and two tiles a wave.  Measured (4096 x 1M x 128 bf16 / 7867 rows x 78K x 256 fp16, whole
 // step): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
-// two to six tiles each 5.2 ms and more (nothing beside the exponentials).
+// two to six tiles each 5.2 ms and more (nothing beside the exponentials).  Exponentials woven between the MFMAs of the tiles
+// before and after by hand (three buffers, sched_group_barrier): 116 to 800 registers spilled, 14.9 / 9.5 ms.
 #define CE_NX 2
 #define CE_NW 8
 
-// splits of the streamed axis: fewest rounds of 256 workgroups times a split's chunks (and about 8 chunks' worth of
-// start and end); `most` bounds the partial results
-static int ce_splits(int64_t nblock, int64_t nch, int64_t most) {
+// splits of the streamed axis: fewest rounds of 256 workgroups times a split's chunks (and two chunks' worth of start
+// and end), a chunk of 64 rows taking a CU about `chunk` us; every split's partial results are written and read
+static int ce_splits(int64_t nblock, int64_t nch, double chunk, double bytes, int64_t most) {
   if (most > nch) most = nch;
   int best = 1;
   double cost = 1e30;
   for (int64_t s = 1; s <= most && s <= 512; ++s) {
     if (s > 8 && s % 8) continue;
-    const double c = (double)((nblock * s + 255) / 256) * ((nch + s - 1) / s + 8);
+    const double c = (double)((nblock * s + 255) / 256) * ((nch + s - 1) / s + 2) * chunk + (s > 1 ? s * bytes / 4e6 : 0.0);
     if (c < cost * 0.999) cost = c, best = (int)s;
   }
   return best;
 }
 
 struct CePlan {
-  int DP, xw, npad, fblocks, fsplits, bblocks, bsplits;
+  int DP, xw, npad, fblocks, fsplits;
+  int bwhole, brest, bsplits;   // backward: blocks done whole (rounds of 256 workgroups), and the rest in splits
+  int64_t items;                // of the rest
 };
 static CePlan ce_plan(int N, int V, int D) {
   CePlan p;
@@ -541,9 +572,16 @@ static CePlan ce_plan(int N, int V, int D) {
   p.npad = (int)ce_up(N, CE_PAD);
   p.fblocks = (N + p.xw - 1) / p.xw;
   // partial results: at most 2^28 values
-  p.fsplits = ce_splits(p.fblocks, (V + CE_CH - 1) / CE_CH, ((int64_t)1 << 28) / ((int64_t)p.npad * p.DP) + 1);
-  p.bblocks = (V + p.xw - 1) / p.xw;
-  p.bsplits = p.bblocks >= 2048 ? 1 : ce_splits(p.bblocks, (N + CE_CH - 1) / CE_CH, ((int64_t)1 << 28) / ((int64_t)V * D) + 1);
+  const double chunk = p.xw * (p.DP / 64) * 0.006;
+  p.fsplits = ce_splits(p.fblocks, (V + CE_CH - 1) / CE_CH, chunk, 8.0 * N * p.DP,
+                        ((int64_t)1 << 28) / ((int64_t)p.npad * p.DP) + 1);
+  // backwards full rounds of 256 blocks go whole, the last, partial one is split over the rows to fill the CUs
+  const int blocks = (V + p.xw - 1) / p.xw;
+  p.bwhole = blocks / 256 * 256;
+  p.brest = blocks - p.bwhole;
+  p.items = V - (int64_t)p.bwhole * p.xw;
+  p.bsplits = p.brest == 0 ? 1 : ce_splits(p.brest, (N + CE_CH - 1) / CE_CH, chunk, 8.0 * p.items * D,
+                                           ((int64_t)1 << 28) / (p.items * D) + 1);
   return p;
 }
 
@@ -559,7 +597,7 @@ extern "C" int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass) {
   const CePlan p = ce_plan(N, V, D);
   if (pass == 0) return 2 * (int64_t)p.fsplits * N + 64;
   if (pass == 1) return 2 * (int64_t)p.fsplits * N + 64 + (int64_t)p.fsplits * N * p.DP;
-  return 64 + 3 * (int64_t)p.npad + (p.bsplits > 1 ? (int64_t)p.bsplits * V * (D + 1) + 64 : 0);
+  return 64 + 3 * (int64_t)p.npad + (p.bsplits > 1 ? p.bsplits * p.items * (D + 1) + 64 : 0);
 }
 // what the backward pass needs of the forward (bytes): packed h, lists, lse, dh for g = 1
 extern "C" int64_t rg_linear_ce_saved_bytes(int N, int V, int D) {
@@ -607,7 +645,11 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
                   int64_t st_t, int N, int V, int D, bool grad, float* work, void* saved, float* loss, hipStream_t st) {
   const CePlan p = ce_plan(N, V, D);
   const CeSaved s = ce_saved(saved, N, D);
-  hipLaunchKernelGGL(k_ce_rows, dim3(1), dim3(1024), 0, st, tgt, st_t, N, p.npad, V, s.count, s.rows, s.tc, s.inv, loss);
+  const int groups = (N + 1023) / 1024;
+  int* counts = (int*)s.lse;   // not written before the join
+  if (groups > 1) hipLaunchKernelGGL(k_ce_count, dim3(groups), dim3(1024), 0, st, tgt, st_t, N, counts);
+  hipLaunchKernelGGL(k_ce_rows, dim3(groups), dim3(1024), 0, st, tgt, st_t, N, p.npad, V, counts, s.count, s.rows, s.tc,
+                     s.inv, loss);
   hipLaunchKernelGGL(k_ce_pack, dim3((p.npad * (p.DP / 8) + 255) / 256), dim3(256), 0, st, (const uint16_t*)h, ldh, D,
                      p.DP, p.npad, s.rows, (uint16_t*)s.hp);
   RG_LAUNCH_CHECK();
@@ -645,14 +687,25 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
   RG_LAUNCH_CHECK();
   CeArgs a = {};
   a.X = W, a.ldx = ldw, a.nx = V, a.Y = s.hp, a.ldy = p.DP, a.ny = N, a.D = D, a.count = s.count, a.bias = bias;
-  a.recs = recs, a.nsplit = p.bsplits, a.nblock = p.bblocks, a.dW = dW, a.db = db, a.scale = scale;
-  a.pO = recs + 3 * (int64_t)p.npad, a.pl = a.pO + ce_up((int64_t)p.bsplits * V * D, 64);
-  const int rc = bias != nullptr ? ce_pass<T, false, true, true>(p.DP, a, st) : ce_pass<T, false, true, false>(p.DP, a, st);
-  if (rc != RG_OK) return rc;
+  a.recs = recs, a.dW = dW, a.db = db, a.scale = scale;
+  auto pass = [&]() {
+    return bias != nullptr ? ce_pass<T, false, true, true>(p.DP, a, st) : ce_pass<T, false, true, false>(p.DP, a, st);
+  };
+  if (p.bwhole > 0) {
+    a.nsplit = 1, a.nblock = p.bwhole, a.block0 = 0;
+    const int rc = pass();
+    if (rc != RG_OK) return rc;
+  }
+  if (p.brest > 0) {
+    a.nsplit = p.bsplits, a.nblock = p.brest, a.block0 = p.bwhole;
+    a.pO = recs + 3 * (int64_t)p.npad, a.pl = a.pO + ce_up(p.bsplits * p.items * D, 64);
+    const int rc = pass();
+    if (rc != RG_OK) return rc;
+  }
   if (p.bsplits > 1) {
-    const int64_t blocks = ((int64_t)V * D / 4 + 255) / 256;
+    const int64_t first = V - p.items, blocks = (p.items * D / 4 + 255) / 256;
     hipLaunchKernelGGL(k_ce_slabs<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, a.pO, a.pl,
-                       p.bsplits, V, D, (T*)dW, db);
+                       p.bsplits, (int)p.items, D, (T*)dW + first * D, db != nullptr ? db + first : nullptr);
     RG_LAUNCH_CHECK();
   }
   return RG_OK;
