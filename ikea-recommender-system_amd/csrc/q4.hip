@@ -12,15 +12,22 @@
 // end: in one chain their low bits would be rounded at the size of 24·Σ x (1.3e-6 of the result instead of 1e-7).
 //
 // A lane's share of an item's group is G/4 consecutive codes; reading those straight from HBM makes 16 rows' short
-// pieces per instruction (64 lanes, 8 cache lines of which 4 B to 16 B are used), so a wave first copies whole
-// 16·T-item pieces (contiguous in memory, about 4 KB) to LDS with 16-byte buffer -> LDS loads and reads them from there.
-// One buffer per wave: 16 waves a CU keep enough bytes in flight.
+// pieces per instruction (64 lanes, 8 cache lines of which 4 B to 16 B are used), so a wave first copies the 16·U
+// items of a job, contiguous in memory, to LDS with 16-byte buffer -> LDS loads and reads them from there.  One buffer a
+// wave; the next job's copy starts when the last code has been read, before this job's scores are stored.  A second
+// buffer a wave halves the waves that fit and measured 36 us against 30 on 1M x 128.
+//
+// Measured: 1M x 128 for one fp32 session, G = 32: 28 us, 76 MB, 2.7 TB/s with the launch (the vector instructions take
+// 18 of the 28: 44 a step of 16 items x 32 codes, of which 8 expand the codes); 5M x 256 for 16 bf16 sessions,
+// G = 64: 250 us, 0.68 GB read and 0.32 GB written, 4.0 TB/s, 78 % of a large copy's rate: the scores of 16 rows end
+// anywhere in a cache line.  10K x 64: 3.5 us of kernel, less than a launch costs.
 #include "common.h"
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 #define Q4_WAVES 4
 #define Q4_K_MAX 1024
+#define Q4_GRID 2048   // 5M x 256: 250 us; 1024 305, 1280 257, 4096 259
 
 // two bf16 values (16 + c) of the codes at bits 4j .. and 16 + 4j .. of w
 template <int J>
@@ -39,14 +46,16 @@ __device__ __forceinline__ float q4_x(const float* x, int64_t i) { return x[i]; 
 __device__ __forceinline__ float q4_x(const __bf16* x, int64_t i) { return (float)x[i]; }
 
 // LDS: x fragments [K / 32][NP][64 lanes] of 16 B, then per wave `cbytes` of codes and `sbytes` of scales (both
-// multiples of 1 KB).  units: 16-item units a wave takes at once.
-template <typename XT, int NP, int G>
-__global__ __launch_bounds__(64 * Q4_WAVES) void k_q4_scores(const XT* __restrict__ x, int64_t ldx,
+// multiples of 1 KB) of the 16·U items that it has in hand.  A granule (16 B of codes) l of a job lies at
+// l ^ (l >> shift & 7): 2^shift granules or fewer make a row, so 16 rows' granules of one group spread over the banks
+// (a row of 128 B would put them all on eight).  Four waves a SIMD keep the accumulators in vector registers.
+template <typename XT, int NP, int G, int U>
+__global__ __launch_bounds__(64 * Q4_WAVES, 4) void k_q4_scores(const XT* __restrict__ x, int64_t ldx,
                                                              const uint8_t* __restrict__ codes,
                                                              const uint16_t* __restrict__ scales,
                                                              const float* __restrict__ bias, int M, int64_t N, int K,
-                                                             int units, int cbytes, int sbytes, float* __restrict__ y,
-                                                             int64_t ldy) {
+                                                             int cbytes, int sbytes, int shift,
+                                                             float* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   constexpr int SG = G / 32;   // MFMA steps of a group; a lane's codes of a group: 4·SG bytes
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15,
@@ -57,8 +66,10 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void k_q4_scores(const XT* __restric
   uint8_t* cl = lds + (size_t)steps * NP * 1024 + (size_t)wave * (cbytes + sbytes);
   const uint8_t* sl = cl + cbytes;
 
-  const int64_t per = 16 * units, jobs = (N + per - 1) / per, stride = (int64_t)gridDim.x * Q4_WAVES;
+  constexpr int per = 16 * U;
+  const int64_t jobs = (N + per - 1) / per, stride = (int64_t)gridDim.x * Q4_WAVES;
   int64_t job = (int64_t)blockIdx.x * Q4_WAVES + wave;
+  auto slot = [&](int l) { return l ^ ((l >> shift) & 7); };   // its own inverse: shift >= 3
   // 16-byte loads of a job's codes and scales; behind the table's end the buffer's bound makes them zero
   auto fetch = [&](int64_t j) {
     const int64_t i0 = j * per;
@@ -68,7 +79,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void k_q4_scores(const XT* __restric
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(scales)) + i0 * groups * 2, 0,
         (int)min((sleft + 3) & ~(int64_t)3, (int64_t)sbytes), 0x00020000);
-    for (int o = 0; o < cbytes; o += 1024) rg_blds16(rc, cl + o, o + 16 * lane, 0);
+    for (int o = 0; o < cbytes; o += 1024) rg_blds16(rc, cl + o, 16 * slot((o >> 4) + lane), 0);
     for (int o = 0; o < sbytes; o += 1024) rg_blds16(rs, cl + cbytes + o, o + 16 * lane, 0);
   };
   if (job < jobs) fetch(job);
@@ -90,56 +101,58 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void k_q4_scores(const XT* __restric
                           (__bf16)-24.f, (__bf16)-24.f, (__bf16)-24.f, (__bf16)-24.f};
   for (; job < jobs; job += stride) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    for (int u0 = 0; u0 < units; u0 += 4) {
-      f4 acc[4];
+    f4 acc[U];
+    float b[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) acc[u] = (f4){0.f, 0.f, 0.f, 0.f};
-      for (int g = 0; g < groups; ++g) {
-        bf16x8 a[SG][NP];
-        f4 start[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int u = 0; u < U; ++u) {
+      const int64_t item = job * per + 16 * u + n;
+      acc[u] = (f4){0.f, 0.f, 0.f, 0.f};
+      b[u] = bias != nullptr && item < N ? bias[item] : 0.f;
+    }
+    for (int g = 0; g < groups; ++g) {
+      bf16x8 a[SG][NP];
+      f4 start[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int s = 0; s < SG; ++s)
+      for (int s = 0; s < SG; ++s)
 #pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            a[s][q] = xf[((g * SG + s) * NP + q) * 64 + lane];
-            start[q > 0] = mfma16bf(a[s][q], minus24, start[q > 0]);
-          }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (u0 + u >= units) break;
-          const int row = 16 * (u0 + u) + n;
-          const uint32_t* c = reinterpret_cast<const uint32_t*>(cl + row * (K / 2) + g * (G / 2) + kg * (G / 8));
-          f4 d = start[0], rest = start[1];
-#pragma unroll
-          for (int s = 0; s < SG; ++s) {
-            const bf16x8 b = q4_codes(c[s]);
-            d = mfma16bf(a[s][0], b, d);
-#pragma unroll
-            for (int q = NP - 1; q >= 1; --q) rest = mfma16bf(a[s][q], b, rest);
-          }
-          if constexpr (NP > 1) d += rest;
-          const float sc = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(sl)[row * groups + g] << 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[u][i] = __builtin_fmaf(sc, d[i], acc[u][i]);
+        for (int q = 0; q < NP; ++q) {
+          a[s][q] = xf[((g * SG + s) * NP + q) * 64 + lane];
+          start[q > 0] = mfma16bf(a[s][q], minus24, start[q > 0]);
         }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = 16 * u + n;
+        const int off = row * (K / 2) + g * (G / 2) + kg * (G / 8);
+        const uint32_t* c = reinterpret_cast<const uint32_t*>(cl + 16 * slot(off >> 4) + (off & 15));
+        f4 d = start[0], rest = start[1];
+#pragma unroll
+        for (int s = 0; s < SG; ++s) {
+          const bf16x8 w = q4_codes(c[s]);
+          d = mfma16bf(a[s][0], w, d);
+#pragma unroll
+          for (int q = NP - 1; q >= 1; --q) rest = mfma16bf(a[s][q], w, rest);
+        }
+        if constexpr (NP > 1) d += rest;
+        const float sc = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(sl)[row * groups + g] << 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[u][i] = __builtin_fmaf(sc, d[i], acc[u][i]);
       }
+    }
+    // every LDS read of this job has returned before the next job's loads land there; they go before the stores,
+    // since the wait for them at the loop's head is one for everything in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (job + stride < jobs) fetch(job + stride);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (u0 + u >= units) break;
-        const int64_t item = job * per + 16 * (u0 + u) + n;
-        if (item < N) {
-          const float b = bias != nullptr ? bias[item] : 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int64_t item = job * per + 16 * u + n;
+      if (item < N) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int m = m0 + 4 * kg + i;
-            if (m < M) y[(int64_t)m * ldy + item] = acc[u][i] + b;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int m = m0 + 4 * kg + i;
+          if (m < M) y[(int64_t)m * ldy + item] = acc[u][i] + b[u];
         }
       }
     }
-    // every LDS read of this job has returned (its values are used above) before the next job's loads land
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (job + stride < jobs) fetch(job + stride);
   }
 }
 
@@ -190,28 +203,35 @@ extern "C" int rg_q4_pack(const void* W, int wtype, int64_t ldw, int64_t N, int 
   return RG_OK;
 }
 
-template <typename XT, int NP, int G>
+template <typename XT, int NP, int G, int U>
 static int q4_launch(const void* x, int64_t ldx, const uint8_t* codes, const uint16_t* scales, const float* bias, int M,
                      int64_t N, int K, float* y, int64_t ldy, hipStream_t stream) {
-  // about 4 KB of codes a wave and pass: fewer leave loads in flight unused, more cost waves
-  const int unit = 8 * K;
-  int units = 4096 / unit;
-  units = units < 1 ? 1 : units > 8 ? 8 : units;
-  // few items: one unit a wave, so that more CUs take part
-  if (N <= (int64_t)16 * units * Q4_WAVES * 256) units = 1;
-  const int cbytes = (units * unit + 1023) & ~1023, sbytes = (units * 32 * (K / G) + 1023) & ~1023;
+  const int cbytes = (U * 8 * K + 1023) & ~1023, sbytes = (U * 32 * (K / G) + 1023) & ~1023;
   const size_t shared = (size_t)(K / 32) * NP * 1024 + (size_t)Q4_WAVES * (cbytes + sbytes);
-  auto kern = k_q4_scores<XT, NP, G>;
+  int shift = 3;   // rows of 2^shift granules or fewer
+  while ((K >> 5) >> (shift + 1)) ++shift;
+  auto kern = k_q4_scores<XT, NP, G, U>;
   if (shared > 64 * 1024 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shared) != hipSuccess)
     return RG_ERR_LAUNCH;
-  const int64_t jobs = (N + 16 * units - 1) / (16 * units);
+  const int64_t jobs = (N + 16 * U - 1) / (16 * U);
   const int64_t wgs = (jobs + Q4_WAVES - 1) / Q4_WAVES;
-  const int gx = (int)(wgs < 2048 ? wgs : 2048);
+  const int gx = (int)(wgs < Q4_GRID ? wgs : Q4_GRID);
   hipLaunchKernelGGL(kern, dim3(gx, (M + 15) / 16), dim3(64 * Q4_WAVES), shared, stream, (const XT*)x, ldx, codes, scales,
-                     bias, M, N, K, units, cbytes, sbytes, y, ldy);
+                     bias, M, N, K, cbytes, sbytes, shift, y, ldy);
   RG_LAUNCH_CHECK();
   return RG_OK;
+}
+
+// Four units a wave read x's operands once for 64 items (5M x 256: 250 us against 276 with two); one where four would
+// hold over 8 KB of codes, or where the items are so few that CUs would stand idle (10K x 64: 39 workgroups of four
+// units, 157 of one).
+template <typename XT, int NP, int G>
+static int q4_units(const void* x, int64_t ldx, const uint8_t* codes, const uint16_t* scales, const float* bias, int M,
+                    int64_t N, int K, float* y, int64_t ldy, hipStream_t stream) {
+  return K <= 256 && N > 64 * Q4_WAVES * 256
+             ? q4_launch<XT, NP, G, 4>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)
+             : q4_launch<XT, NP, G, 1>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream);
 }
 
 extern "C" int rg_q4_scores(const void* x, int xtype, int64_t ldx, const uint8_t* codes, const uint16_t* scales,
@@ -222,9 +242,9 @@ extern "C" int rg_q4_scores(const void* x, int xtype, int64_t ldx, const uint8_t
   if (x == nullptr || codes == nullptr || scales == nullptr || y == nullptr || ldx < K || ldy < N) return RG_ERR_ARG;
   if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 15)) return RG_ERR_ARG;
 #define Q4_GO(XT, NP)                                                                                       \
-  return G == 32   ? q4_launch<XT, NP, 32>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)            \
-         : G == 64 ? q4_launch<XT, NP, 64>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)            \
-                   : q4_launch<XT, NP, 128>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)
+  return G == 32   ? q4_units<XT, NP, 32>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)            \
+         : G == 64 ? q4_units<XT, NP, 64>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)            \
+                   : q4_units<XT, NP, 128>(x, ldx, codes, scales, bias, M, N, K, y, ldy, stream)
   if (xtype == 0) Q4_GO(float, 3);
   if (xtype == 1) Q4_GO(__bf16, 1);
 #undef Q4_GO

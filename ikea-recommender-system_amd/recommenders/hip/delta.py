@@ -26,7 +26,7 @@ import ctypes as C
 import torch
 
 from . import call, ptr
-from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole
+from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole, wrote
 
 _IO = (torch.float32, torch.bfloat16)
 
@@ -194,4 +194,5 @@ def delta_rule_step(q, k, v, g, beta, state, scale=None):
             _aligned(state=state)
         run(p.step, p.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), p.strides, p.type,
             *p.sizes, p.scale if scale is None else float(scale), at, p.apart, o.data_ptr())
+        wrote(state)
     return o

@@ -62,6 +62,13 @@ def version(t):
     return None if t is None or t.is_inference() else t._version
 
 
+def wrote(t):
+    """After a kernel wrote a caller's tensor in place: counted as a write, so that a backward pass that still needs the
+    old values says so."""
+    if not t.is_inference():
+        torch._C._increment_version([t])
+
+
 class Plans(dict):
     """Checked argument layouts -> what a call needs of them.  Bounded: a program has few layouts; one that keeps making
     new ones starts over now and then."""

@@ -8,7 +8,7 @@ served model at a quarter of its bf16 bytes.
 codes  (N, K / 2) uint8, two codes a byte, the even column in the low half;
 scales (N, K / group) bfloat16; a weight is scales[n, k // group]·(code − 8).
 K is a multiple of `group` (32, 64 or 128) and at most 1024; any number of
-items N and of rows M.  Sums are kept in fp32; x may be fp32 or bf16 and
+items N, up to 1M rows M.  Sums are kept in fp32; x may be fp32 or bf16 and
 enters exactly.  Capturable; no workspace, no host synchronisation.  Weights
 have to be finite.
 """
@@ -17,10 +17,10 @@ from __future__ import annotations
 import torch
 
 from . import ptr
-from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, whole
+from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, whole, wrote
 
 GROUPS = (32, 64, 128)
-K_MAX = 1024
+K_MAX, M_MAX = 1024, 65535 * 16
 
 
 def _table(K, group):
@@ -49,6 +49,8 @@ _plans = Plans()
 def _plan(x, codes, scales, bias):
     tensor("x", x, (None, None), (torch.float32, torch.bfloat16))
     M, K = x.shape
+    if M > M_MAX:
+        fail("x", f"at most {M_MAX} rows are expected, got {M}")
     whole("codes", codes, (None, K // 2), (torch.uint8,), x.device)
     N = codes.shape[0]
     whole("scales", scales, (N, None), (torch.bfloat16,), x.device)
@@ -78,4 +80,5 @@ def q4_scores(x, codes, scales, bias=None, out=None):
         ldy = stride(out, 0) or N
     if M and N:
         run(fn, device, x.data_ptr(), kind, ldx, *at, ptr(bias), M, N, K, group, out.data_ptr(), ldy)
+        wrote(out)
     return out

@@ -38,7 +38,8 @@ def check(y, x, codes, scales, bias, G):
 
 @pytest.mark.parametrize("M,N,K,G", [(1, 1, 32, 32), (1, 15, 64, 64), (3, 17, 128, 128), (16, 1000, 96, 32),
                                      (17, 33, 192, 64), (5, 4099, 1024, 32), (2, 70001, 256, 128), (40, 515, 640, 128),
-                                     (1, 300001, 128, 32), (16, 299, 1024, 64)])
+                                     (1, 300001, 128, 32), (16, 299, 1024, 64),
+                                     (17, 66001, 192, 64), (3, 80003, 96, 32), (1, 70000, 32, 32), (18, 65553, 512, 128)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_scores(M, N, K, G, dtype):
     from recommenders.hip.q4 import q4_scores

@@ -16,6 +16,12 @@ def test_q4_refuses_before_the_device():
         q4_scores(W, torch.zeros(5, 32, dtype=torch.uint8), torch.zeros(5, 2, dtype=torch.bfloat16))
 
 
+def test_q4_c_entry_refuses_more_rows_than_a_grid():
+    from recommenders.hip import load_library
+    one = 4096
+    assert load_library().rg_q4_scores(one, 0, 64, one, one, None, 65535 * 16 + 1, 5, 64, 32, one, 5, None) == -3
+
+
 def test_q4_c_entry_refusals():
     from recommenders.hip import load_library
     lib = load_library()
