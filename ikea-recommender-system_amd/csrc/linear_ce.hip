@@ -23,8 +23,10 @@
 // Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
 // packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
 // P is rounded to bf16 / fp16 for the second product (half a step of the type, once, as its other operand is held); sums
-// of P, lse, O and the gradients are fp32, and each output is rounded once.  fp16 keeps small probabilities out of its
-// subnormals by a power of two: forwards P <= 2^15, backwards g is scaled to [2^13, 2^14] at its largest.
+// of P, lse, O and the gradients are fp32, and each output is rounded once.  Backwards g is scaled so that the largest
+// |g| is 2^13, and back in fp32: a mean's g is one number for every row and most of a target item's gradient, and
+// rounded as it stands it moved all of dW the same way (2.2 times the error of the output's own rounding; scaled it
+// enters exactly).  It also keeps fp16's small probabilities out of its subnormals; forwards P <= 2^15 does.
 #include "common.h"
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
@@ -36,7 +38,6 @@ typedef short ce_s8 __attribute__((ext_vector_type(8)));
 #define CE_L2E 1.4426950408889634f
 #define CE_LN2 0.6931471805599453f
 #define CE_LOW (-3.0e38f)  // the running reference before any logit
-#define CE_BIG 30.f        // |bias| · log2 e up to which an item's bias is taken out of its probabilities' exponents
 
 template <typename T>
 struct CeT;
@@ -67,7 +68,7 @@ struct CeArgs {
   float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][items from block0 on][D], pl likewise
   void* dW;
   float* db;
-  const float* scale;      // backward: {factor on g, its inverse}; null: 1
+  const float* scale;      // backward: what g's scaling left out
 };
 
 // 16-byte chunk c of row r sits at place c ^ swz(r): 16 rows' reads of one column spread over all banks
@@ -150,14 +151,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     }
     ref[t] = CE_LOW;
     sum[t] = 0.f;
-    xb[t] = BIAS && x < nx ? a.bias[x] * CE_L2E : 0.f;
-  }
-  // bf16 has fp32's range: an item's bias factor 2^xb is left out of P and multiplied into its sums at the end
-  bool whole = true;
-  if constexpr (BIAS) {
-#pragma unroll
-    for (int t = 0; t < NX; ++t) whole &= fabsf(xb[t]) <= CE_BIG;
-    whole = CeT<T>::OFF == 0.f && __all(whole);
+    xb[t] = BIAS && x < nx ? a.bias[x] : 0.f;
   }
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   f4 O[FB][NX];
@@ -185,7 +179,8 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int t = 0; t < NX; ++t) S[j][t] = FWD ? *reinterpret_cast<const f4*>(r + at + 16 * j) : zero;
+        for (int t = 0; t < NX; ++t)
+          S[j][t] = FWD ? *reinterpret_cast<const f4*>(r + at + 16 * j) : BIAS ? (f4){xb[t], xb[t], xb[t], xb[t]} : zero;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const uint8_t* p = y + (32 * h + nn) * RB + (((4 * s + kg) ^ ce_swz<DP>(nn)) << 4);
@@ -242,19 +237,11 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) e[j] = *reinterpret_cast<const f4*>(r + at + 16 * j);
         float p[NX][8];
-        if (whole) {
 #pragma unroll
-          for (int t = 0; t < NX; ++t)
+        for (int t = 0; t < NX; ++t)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, e[i >> 2][i & 3]));
-        } else {
-#pragma unroll
-          for (int t = 0; t < NX; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, e[i >> 2][i & 3] + xb[t]));
-        }
+          for (int i = 0; i < 8; ++i)
+            p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, e[i >> 2][i & 3]));
         if (mine || sign) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -263,7 +250,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 #pragma unroll
             for (int t = 0; t < NX; ++t) {
               if (g < 0.f) p[t][i] = -p[t][i];
-              if (tg == x0 + 16 * t + n) p[t][i] -= whole ? g * __builtin_amdgcn_exp2f(-xb[t]) : g;
+              if (tg == x0 + 16 * t + n) p[t][i] -= g;
             }
           }
         }
@@ -322,7 +309,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
         for (int f = 0; f < FB; ++f) *reinterpret_cast<f4*>(a.pO + at * DP + 16 * f + 4 * kg) = O[f][t];
       }
     } else {
-      const float back = (a.scale != nullptr ? a.scale[1] : 1.f) * (BIAS && whole ? __builtin_amdgcn_exp2f(xb[t]) : 1.f);
+      const float back = *a.scale;
       if (a.nsplit > 1) {
         const int64_t first = (int64_t)a.block0 * 16 * NX * NW, at = split * (a.nx - first) + x - first;
         if (a.db != nullptr && kg == 0) a.pl[at] = sum[t] * back;
@@ -459,39 +446,41 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
   }
 }
 
-// fp16: the power of two that brings the largest |g| of the listed rows to [2^13, 2^14), and its inverse
-__global__ __launch_bounds__(1024) void k_ce_scale(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
-                                                   int N, float* __restrict__ scale) {
+// the largest |g| of 1024 rows that are not ignored
+__global__ __launch_bounds__(1024) void k_ce_largest(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
+                                                     int N, float* __restrict__ largest) {
   __shared__ float part[16];
-  float m = 0.f;
-#pragma unroll 8
-  for (int r = threadIdx.x; r < N; r += 1024) {
-    const float x = fabsf(g[r * sg]);
-    m = inv[r] >= 0 ? fmaxf(m, x) : m;
-  }
+  const int r = blockIdx.x * 1024 + threadIdx.x;
+  float m = r < N && inv[r] >= 0 ? fabsf(g[r * sg]) : 0.f;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 0; w < 16; ++w) m = fmaxf(m, part[w]);
-    int e = 0;
-    if (m > 0.f && m < __builtin_inff()) (void)frexpf(m, &e);   // m in [2^(e−1), 2^e)
-    e = min(max(14 - e, -120), 120);
-    scale[0] = ldexpf(1.f, e);
-    scale[1] = ldexpf(1.f, -e);
+    largest[blockIdx.x] = m;
   }
 }
 
-// dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows
+// dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows, and the
+// factor that their scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
                                                const int* __restrict__ count, const int* __restrict__ tc,
                                                const float* __restrict__ lse, const float* __restrict__ dh0, int N,
-                                               int npad, int D, const float* __restrict__ scale, T* __restrict__ dh,
-                                               float* __restrict__ recs) {
+                                               int npad, int D, const float* __restrict__ largest, T* __restrict__ dh,
+                                               float* __restrict__ recs, float* __restrict__ scale) {
   const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= npad) return;
+  float top = 0.f;
+  if (largest != nullptr)
+    for (int i = lane; i < (N + 1023) / 1024; i += 64) top = fmaxf(top, largest[i]);
+  else
+    for (int i = lane; i < N; i += 64) top = fmaxf(top, inv[i] >= 0 ? fabsf(g[i * sg]) : 0.f);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = top < __builtin_inff() ? fmaxf(top, 0x1p-100f) : 1.f;
+  if (r == 0 && lane == 0) *scale = top * 0x1p-13f;
   if (lane == 0 && r >= *count) {   // behind the last packed row
     float* rec = recs + (int64_t)(r / CE_CH) * 3 * CE_CH + r % CE_CH;
     rec[0] = -__builtin_inff();
@@ -508,7 +497,7 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
   }
   if (lane == 0 && c >= 0) {
     float* rec = recs + (int64_t)(c / CE_CH) * 3 * CE_CH + c % CE_CH;
-    const float w = scale != nullptr ? gr * scale[0] : gr;
+    const float w = gr / top * 0x1p13f;
     rec[0] = __log2f(fabsf(w)) - lse[c] * CE_L2E;
     rec[CE_CH] = w;
     rec[2 * CE_CH] = __int_as_float(tc[c]);
@@ -540,7 +529,7 @@ static int ce_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // a workgroup holds CE_NW · CE_NX · 16 = 256 rows of X: eight waves, two on a SIMD, so that one's exponentials run beside
 // the other's MFMAs, and two tiles a wave.  Measured (4096 x 1M x 128 bf16 / 7867 rows x 78K x 256 fp16, whole
-// step): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
+// step): two tiles 3.52 / 1.31 ms (now 3.42 / 1.15), three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
 // two to six tiles each 5.2 ms and more (nothing beside the exponentials).  Exponentials woven between the MFMAs of the tiles
 // before and after by hand (three buffers, sched_group_barrier): 116 to 800 registers spilled, 14.9 / 9.5 ms.
 #define CE_NX 2
@@ -591,13 +580,14 @@ static int ce_check(int64_t N, int64_t V, int D, int type) {
   return RG_OK;
 }
 
-// forward scratch (floats): pm, pl, pO; backward: scale, recs, pO slabs, pl slabs
+// forward scratch (floats): pm, pl, pO; backward: scale, recs, pO slabs and pl slabs (before them the largest |g|s)
 extern "C" int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass) {
   if (ce_check(N, V, D, 1) != RG_OK) return 0;
   const CePlan p = ce_plan(N, V, D);
   if (pass == 0) return 2 * (int64_t)p.fsplits * N + 64;
   if (pass == 1) return 2 * (int64_t)p.fsplits * N + 64 + (int64_t)p.fsplits * N * p.DP;
-  return 64 + 3 * (int64_t)p.npad + (p.bsplits > 1 ? p.bsplits * p.items * (D + 1) + 64 : 0);
+  const int64_t slabs = p.bsplits > 1 ? p.bsplits * p.items * (D + 1) + 64 : 0, groups = (N + 1023) / 1024;
+  return 64 + 3 * (int64_t)p.npad + (slabs > groups ? slabs : groups);
 }
 // what the backward pass needs of the forward (bytes): packed h, lists, lse, dh for g = 1
 extern "C" int64_t rg_linear_ce_saved_bytes(int N, int V, int D) {
@@ -677,13 +667,11 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
                   const void* saved, float* work, void* dh, void* dW, float* db, hipStream_t st) {
   const CePlan p = ce_plan(N, V, D);
   const CeSaved s = ce_saved(const_cast<void*>(saved), N, D);
-  float *scale = nullptr, *recs = work + 64;
-  if (CeT<T>::OFF != 0.f) {
-    scale = work;
-    hipLaunchKernelGGL(k_ce_scale, dim3(1), dim3(1024), 0, st, g, sg, s.inv, N, scale);
-  }
+  const int groups = (N + 1023) / 1024;
+  float *scale = work, *recs = work + 64, *largest = groups > 1 ? recs + 3 * (int64_t)p.npad : nullptr;
+  if (groups > 1) hipLaunchKernelGGL(k_ce_largest, dim3(groups), dim3(1024), 0, st, g, sg, s.inv, N, largest);
   hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.dh0, N,
-                     p.npad, D, scale, (T*)dh, recs);
+                     p.npad, D, largest, (T*)dh, recs, scale);
   RG_LAUNCH_CHECK();
   CeArgs a = {};
   a.X = W, a.ldx = ldw, a.nx = V, a.Y = s.hp, a.ldy = p.DP, a.ny = N, a.D = D, a.count = s.count, a.bias = bias;

@@ -217,3 +217,24 @@ def test_changed_weights_are_refused_and_no_rows():
     loss, saved = linear_ce(h[:0], W, t[:0], bias=b, save=True)
     dh, dW, db = linear_ce_backward(saved, torch.ones(0, device="cuda"))
     assert loss.shape == (0,) and dh.shape == (0, 8) and (dW == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_targets_share_is_not_rounded_twice(dtype, bias):
+    """A mean's weight g is the same for all rows and most of a target item's gradient.  Scaled by the largest weight it
+    enters as 2^13 (p − 1), and what rounding that moves is at most p (the nearest value kept is −1) and at most u.  Beside it
+    the other items' probabilities carry u, every sum 1e-4 and the output's rounding u, once."""
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = inputs(700, 4001, 64, dtype, bias, 0.0)
+    t = torch.randperm(4001, device="cuda")[:700]
+    dloss = torch.full((700,), 1.00389 / 512, device="cuda")   # 257 / 256: halfway between bf16 values
+    loss, saved = linear_ce(h, W, t, bias=b, save=True)
+    dh, dW, db = linear_ce_backward(saved, dloss)
+    z = h.double() @ W.double().t() + (0 if b is None else b.double())
+    hit = torch.zeros_like(z).scatter_(1, t[:, None], 1.0)
+    p, g, u = z.softmax(1), dloss.double()[:, None], torch.finfo(dtype).eps / 2
+    ref = (g * (p - hit)).t() @ h.double()
+    a = h.double().abs()
+    room = u * ref.abs() + (u + 1e-4) * ((g * p).t() @ a) + ((1e-4 + p.clamp(max=u)) * g * hit).t() @ a + 2.0 ** -24
+    assert ((dW.double() - ref).abs() <= room).all()
