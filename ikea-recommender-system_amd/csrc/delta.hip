@@ -46,8 +46,8 @@ struct DeltaArgs {
   float *state, *dstate0, *dg, *dbeta;
   float *U, *dX;                            // (B, Hv, T, Dv)
   float *S0, *dS;                           // (B, Hv, chunks - 1, Dk, Dv): states before chunk c + 1, gradients after chunk c
-  // segments of `per` chunks; nseg = 1: none.  trans (B, Hv, nseg, Dk, Dk): what a segment does to the state it starts
-  // with; local (B, Hv, nseg, Dk, Dv): the state (or its gradient) it leaves when it starts from zero, then, joined,
+  // segments of `per` chunks; nseg = 1: none.  trans (B, Hv, nseg, dl_trans_floats): what a segment does to the state it
+  // starts with; local (B, Hv, nseg, Dk, Dv): the state (or its gradient) it leaves when it starts from zero, then, joined,
   // the one it really starts from
   int nseg, per;
   float *trans, *local;
@@ -82,15 +82,16 @@ struct DlIO<float> {
   static __device__ __forceinline__ void load44(DlBuf b, int v, int s, int v2, int s2, bf16x8* f) {
     pl_split<3>(load4(b, v, s), load4(b, v2, s2), f);
   }
-  static __device__ __forceinline__ void load4x2(DlBuf b, int v, int s, int v2, int s2, f4& x, f4& y) {
-    x = load4(b, v, s);
-    y = load4(b, v2, s2);
-  }
   struct Raw8 {
     f4 a, b;
   };
   static __device__ __forceinline__ Raw8 load8(DlBuf b, int v, int s) { return {load4(b, v, s), load4(b, v + 16, s)}; }
   static __device__ __forceinline__ void planes(const Raw8& x, bf16x8* f) { pl_split<3>(x.a, x.b, f); }
+  static __device__ __forceinline__ float dot(const Raw8& x, const f4& p, const f4& q, float s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = __builtin_fmaf(x.a[i], p[i], __builtin_fmaf(x.b[i], q[i], s));
+    return s;
+  }
   static __device__ __forceinline__ void store1(DlBuf b, int v, int s, float x) {
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), b, v, s, 0);
   }
@@ -110,16 +111,16 @@ struct DlIO<__bf16> {
     const dl_u2 x = __builtin_amdgcn_raw_buffer_load_b64(b, v, s, 0), y = __builtin_amdgcn_raw_buffer_load_b64(b, v2, s2, 0);
     f[0] = __builtin_bit_cast(bf16x8, (dl_u4){x[0], x[1], y[0], y[1]});
   }
-  static __device__ __forceinline__ void load4x2(DlBuf b, int v, int s, int v2, int s2, f4& x, f4& y) {
-    const dl_u2 p = __builtin_amdgcn_raw_buffer_load_b64(b, v, s, 0), q = __builtin_amdgcn_raw_buffer_load_b64(b, v2, s2, 0);
-    x = (f4){__uint_as_float(p[0] << 16), __uint_as_float(p[0] & 0xffff0000u), __uint_as_float(p[1] << 16), __uint_as_float(p[1] & 0xffff0000u)};
-    y = (f4){__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16), __uint_as_float(q[1] & 0xffff0000u)};
-  }
   typedef bf16x8 Raw8;
   static __device__ __forceinline__ Raw8 load8(DlBuf b, int v, int s) {
     return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, v, s, 0));
   }
   static __device__ __forceinline__ void planes(const Raw8& x, bf16x8* f) { f[0] = x; }
+  static __device__ __forceinline__ float dot(const Raw8& x, const f4& p, const f4& q, float s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = __builtin_fmaf((float)x[i], p[i], __builtin_fmaf((float)x[4 + i], q[i], s));
+    return s;
+  }
   static __device__ __forceinline__ void store1(DlBuf b, int v, int s, float x) {
     __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)x), b, v, s, 0);
   }
@@ -340,6 +341,31 @@ __device__ __forceinline__ void dl_state_store(const f4 (*S)[UT], float* dst, in
     }
 }
 
+// A transition is kept as its 16 x 16 tiles in the order in which the join's operands want them, so that a wave reads 1 KB
+// in one piece (from rows, half a cache line a lane: 2.2 us a segment of width 128 against 1.55): lane (kg, n), value r of
+// tile (w, t) is row 16·w + n, column 16·t + 4·kg + r, then, for the backward pass, row 16·t + 4·kg + r, column 16·w + n.
+__host__ __device__ __forceinline__ int64_t dl_trans_floats(int Dk) {
+  const int N = (Dk + 15) / 16;
+  return 2 * 256 * (int64_t)N * N;
+}
+template <int CT, int UT>
+__device__ __forceinline__ void dl_trans_store(const f4 (*S)[UT], float* dst, int Dk, int col0, bool back) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, N = (Dk + 15) / 16;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = col0 / 16 + ct;
+    if (c >= N) break;
+#pragma unroll
+    for (int u = 0; u < UT; ++u) {
+      if (u >= N) break;
+      float* p = dst + (u * N + c) * 256 + (16 * (n >> 2) + 4 * kg) * 4 + (n & 3);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[4 * r] = S[ct][u][r];
+      if (back) *reinterpret_cast<f4*>(dst + N * N * 256 + (c * N + u) * 256 + lane * 4) = S[ct][u];
+    }
+  }
+}
+
 // ---------------------------------------------------------------- forward ----
 // TRANS: only the states a segment leaves, from zero (columns of the value) or from the identity with v = 0 (the columns
 // behind them: the segment's transition)
@@ -353,7 +379,7 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
   float* Ad = (float*)(lds + L::KQ + sizeof(DlGates));
 
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int seg = blockIdx.x % a.nseg, bhi = blockIdx.x / a.nseg;
+  const int seg = blockIdx.x / (a.B * a.Hv), bhi = blockIdx.x % (a.B * a.Hv);
   const int b = bhi / a.Hv, h = bhi % a.Hv, hk = h / (a.Hv / a.Hk);
   const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C;
   const int vblocks = (a.Dv + 16 * CT - 1) / (16 * CT);
@@ -503,8 +529,10 @@ __global__ __launch_bounds__(64, 2) void k_delta_fwd(DeltaArgs a) {
     zero = false;
   }
   if constexpr (TRANS) {
-    float* dst = unit ? a.trans + (bh * a.nseg + seg) * a.Dk * a.Dk : a.local + (bh * a.nseg + seg) * size;
-    dl_state_store<CT, 2 * KT>(S, dst, a.Dk, cols, col0);
+    if (unit)
+      dl_trans_store<CT, 2 * KT>(S, a.trans + (bh * a.nseg + seg) * dl_trans_floats(a.Dk), a.Dk, col0, a.U != nullptr);
+    else
+      dl_state_store<CT, 2 * KT>(S, a.local + (bh * a.nseg + seg) * size, a.Dk, cols, col0);
   } else {
     // outputs behind the length, in this segment's part
     const int tto = seg == a.nseg - 1 ? a.T : min(a.T, tfrom + a.per * DL_C);
@@ -528,7 +556,7 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
   float* Ad = (float*)(lds + 2 * L::KQ + sizeof(DlGates));
 
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int seg = blockIdx.x % a.nseg, bhi = blockIdx.x / a.nseg;
+  const int seg = blockIdx.x / (a.B * a.Hv), bhi = blockIdx.x % (a.B * a.Hv);
   const int b = bhi / a.Hv, h = bhi % a.Hv, hk = h / (a.Hv / a.Hk);
   const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C, col0 = blockIdx.y * 16 * CT;
   const IO* q = (const IO*)a.q + b * a.qs[0] + hk * a.qs[2];
@@ -664,15 +692,16 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
 // ------------------------------------------------------- segments ----
 // The state a segment starts from: S_{s+1} = trans_s S_s + local_s, put in local's place; backwards the gradient it starts
 // from: dS_{s-1} = trans_sᵀ dS_s + local_s.  One workgroup per (row, head, 16 value columns), a wave per 16 rows of the
-// state: its rows of trans straight from memory (the next segment's while this one's products run), the state
-// from LDS in planes, in two buffers, so that a segment costs one barrier.
+// state: its rows of trans straight from memory (the next segments' while this one's products run), the state from LDS, in
+// two buffers, so that a segment costs one barrier.  On fp32 MFMA, whose four steps take a lane's four values of an
+// accumulator as they are.  What bounds it is a CU's way to the 64 KB of trans of each segment (width 128): neither the
+// products (fp32, or bf16 planes split here) nor loading one or three segments ahead move it.  (8 heads, 32 segments: 49 us.)
 template <int DP, bool BACK>
 __global__ __launch_bounds__(4 * DP) void k_delta_join(DeltaArgs a) {
-  constexpr int NP = DL_NP, KT = DP / 32;
-  using M = PlaneMat<16, DP, NP>;   // row: value column; columns: the state's rows
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][M::BYTES];
+  constexpr int NT = DP / 16, AHEAD = 3;
+  __shared__ f4 lds[2][NT][64];
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d0 = 16 * wave, col = blockIdx.y * 16 + n;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d0 = 16 * wave, col = blockIdx.y * 16 + n, N = (a.Dk + 15) / 16;
   const int64_t bh = blockIdx.x, size = (int64_t)a.Dk * a.Dv;
   const float* first = BACK ? a.dstate : a.state0;
   const int at = dl_lane(col < a.Dv, ((d0 + 4 * kg) * a.Dv + col) * 4);
@@ -681,73 +710,83 @@ __global__ __launch_bounds__(4 * DP) void k_delta_join(DeltaArgs a) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) S[r] = DlIO<float>::load1(state(first != nullptr ? first + bh * size : nullptr), at, r * a.Dv * 4);
 
-  f4 w[KT][2], loc;   // this wave's rows of trans (BACK: columns), and of local
-  auto fetch = [&](int seg) __attribute__((always_inline)) {
-    const DlBuf tb = dl_buf(a.trans + (bh * a.nseg + seg) * a.Dk * a.Dk, a.Dk, a.Dk, a.Dk, 4);
-    const int v = BACK ? dl_lane(d0 + n < a.Dk, (4 * kg * a.Dk + d0 + n) * 4) : (n * a.Dk + 4 * kg) * 4;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int e = 32 * t + 16 * q;
-        if (BACK) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w[t][q][r] = DlIO<float>::load1(tb, v, (e + r) * a.Dk * 4);
-        } else {
-          w[t][q] = DlIO<float>::load4(tb, dl_lane(e + 4 * kg < a.Dk, v), (d0 * a.Dk + e) * 4);
-        }
-      }
-    const DlBuf lb = state(a.local + (bh * a.nseg + seg) * size);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) loc[r] = DlIO<float>::load1(lb, at, r * a.Dv * 4);
-  };
-  fetch(BACK ? a.nseg - 1 : 0);
-  for (int i = 0; i < a.nseg; ++i) {
+  struct Part {
+    f4 w[NT], loc;   // this wave's rows of trans (BACK: of its transpose), and of local
+  } part[AHEAD];
+  auto fetch = [&](Part& x, int i) __attribute__((always_inline)) {
     const int seg = BACK ? a.nseg - 1 - i : i;
-    const DlBuf lb = state(a.local + (bh * a.nseg + seg) * size);
-    const f4 add = loc;
-    bf16x8 f[KT][NP];
+    const DlBuf tb = dl_buf(a.trans + (bh * a.nseg + seg) * dl_trans_floats(a.Dk) + (BACK ? N * N * 256 : 0), 1, 0, N * N * 256, 4);
 #pragma unroll
-    for (int t = 0; t < KT; ++t) pl_split<NP>(w[t][0], w[t][1], f[t]);
+    for (int t = 0; t < NT; ++t)
+      x.w[t] = DlIO<float>::load4(tb, dl_lane(wave < N && t < N, lane * 16), (wave * N + t) * 1024);
+    const DlBuf lb = state(a.local + (bh * a.nseg + seg) * size);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x.loc[r] = DlIO<float>::load1(lb, at, r * a.Dv * 4);
+  };
+  const int last = a.nseg - 1;   // (what the last segment leaves is not asked for)
+  auto put = [&](int i) __attribute__((always_inline)) {
+    const DlBuf lb = state(a.local + (bh * a.nseg + (BACK ? last - i : i)) * size);
 #pragma unroll
     for (int r = 0; r < 4; ++r) DlIO<float>::store1(lb, at, r * a.Dv * 4, S[r]);
-    if (i == a.nseg - 1) break;
-    fetch(BACK ? seg - 1 : seg + 1);
-    const M m{(__bf16*)lds[i & 1]};
-    bf16x8 p[NP];
-    pl_split<NP>(S, DL_ZERO, p);
+  };
 #pragma unroll
-    for (int q = 0; q < NP; ++q) {
-      const pl_s8 v = __builtin_bit_cast(pl_s8, p[q]);
-      *reinterpret_cast<pl_s4*>(m.p + q * M::PLANE + n * M::LD + pl_place(d0 + 4 * kg)) = (pl_s4){v[0], v[1], v[2], v[3]};
-    }
-    __syncthreads();
-    S = add;
+  for (int k = 0; k < AHEAD; ++k) {
+    fetch(part[k], min(k, last));
+    __builtin_amdgcn_sched_barrier(0);   // in this order, so that the first wait leaves the others in flight
+  }
+  int i = 0;
+  while (true) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      m.row(p, 0, t);
-      S = pl_mm<NP, NP>(f[t], p, S);
+    for (int k = 0; k < AHEAD; ++k, ++i) {
+      if (i >= last) {
+        put(i);
+        return;
+      }
+      f4 sum[4] = {part[k].loc, DL_ZERO, DL_ZERO, DL_ZERO};
+      put(i);
+      lds[i & 1][wave][lane] = S;
+      __syncthreads();
+      f4 x[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x[t] = lds[i & 1][t][lane];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = mfma16(part[k].w[t][r], x[t][r], sum[r]);
+      __builtin_amdgcn_sched_barrier(0);
+      // without a branch, so that the waits for the segments before count only what they have to
+      fetch(part[k], min(i + AHEAD, last));
+      __builtin_amdgcn_sched_barrier(0);
+      S = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
   }
 }
 
 // -------------------------------------- backward, the rest of a chunk's gradients ----
-// One workgroup per (row, key head, chunk), independent of the others; the value heads of a key head one after the
-// other, their dq and dk summed in registers (no atomics: the same result every time).  Two waves, one per 16 positions
-// i; four where there are more than 64 key columns, half of them each.  The contractions over the value columns,
+// One workgroup of four waves per (row, key head, chunk), independent of the others; the value heads of a key head one
+// after the other, their dq and dk summed in registers (no atomics: the same result every time).  The contractions over the
+// value columns,
 //     dP = dO Uᵀ,  dA = −dX Uᵀ,  E1 = dO Sᵀ,  E2 = dX Sᵀ,  E3 = U dS'ᵀ,
-// read their operands straight from memory (rows of contiguous values are what an operand's lanes want); then
+// go 32 columns at a time: dX, U and dO are split into planes once, in LDS, and shared, while each wave loads and
+// splits its own key tiles of S and dS' (rows of contiguous values are what an operand's lanes want) and multiplies them
+// with both tiles of positions; of the four tiles of dP and dA each wave has one.  Then
 //     dQ = scale e^G E1 + M1 K,  dK = M1ᵀ Q + (M2 + M2ᵀ) K − b e^G E2 + D_end E3,  M1 = scale D dP,  M2 = b D dA
-// with M1 and M2 passed through LDS, and the scalars' gradients from their row and column sums.  Every product is made
-// with the position i as its column, so a lane's scalars are one position's and its four results lie side by side.
-// What bounds it is the chain of loads, products and sums (vector instructions are issued 40 % of the time, most of
-// them splitting operands into planes).  Three waves a SIMD spill 52 registers and cost 20 %.
+// with M1 and M2 passed through LDS, in dX's and U's place, and the scalars' gradients from their row and column sums, by
+// one wave while the others load the next value head.  Every product is made with the position i as its column, so a
+// lane's scalars are one position's and its four results lie side by side.
+// What bounds it is vector instructions, most of them splitting operands into planes, and the chain of loads, products and sums.  (Two
+// waves, one per tile of positions, each splitting all of S, dS', dX and U for itself: 270 us against 157 on 4 x 8
+// heads x 4096 positions of width 128, 181 against 165 on 8192 sessions x heads of up to 50 positions of width 64.  Waves a
+// SIMD: with three, fp32 spills 23 registers, 91 us against 75 on 2048 sessions x heads; bf16 does not, 165 us against 219 with two.
+// Rows of one chunk, which have no states, in a kernel of their own with four waves a SIMD: 56 + 118 us against 165.)
 template <int DP, int NI>
 struct DlGradLds {
-  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, M = PlaneMat<DL_C, 32, DL_NP>::BYTES;
-  static constexpr int HALVES = DP > 64 ? 2 : 1, THREADS = 128 * HALVES;
-  static constexpr int SUMS = (2 * 32 + 3 * HALVES * 32 + 3 * 32 + 8) * 4;
-  static constexpr int BYTES = 2 * KQ + 2 * M + (int)sizeof(DlGates) + SUMS;
+  static constexpr int KQ = PlaneMat<DL_C, DP, NI>::BYTES, X = PlaneMat<DL_C, 32, DL_NP>::BYTES,
+                       G = PlaneMat<DL_C, 32, NI>::BYTES;
+  static constexpr int THREADS = 256, WAVES = 4;
+  static constexpr int SUMS = 2 * 32 + 3 * WAVES * 32 + 5 * 32 + WAVES;   // floats, once per parity of the value head
+  static constexpr int BYTES = 2 * KQ + 2 * X + G + (int)sizeof(DlGates) + 2 * SUMS * 4;
 };
 
 // sum over the 16 lanes of a group, by rotations of a row of lanes
@@ -806,41 +845,43 @@ struct DlRow {
 };
 
 template <typename IO, int DP>
-__global__ __launch_bounds__(DP > 64 ? 256 : 128, 2) void k_delta_grads(DeltaArgs a) {
+__global__ __launch_bounds__(256, DP > 64 || DlIO<IO>::N > 1 ? 2 : 3) void k_delta_grads(DeltaArgs a) {
   using L = DlGradLds<DP, DlIO<IO>::N>;
-  constexpr int NI = DlIO<IO>::N, NP = DL_NP, HALVES = L::HALVES, THREADS = L::THREADS, SIZE = DlIO<IO>::SIZE;
-  constexpr int UT = DP / 16 / HALVES;   // key tiles of a wave, taken in pairs
+  constexpr int NI = DlIO<IO>::N, NP = DL_NP, THREADS = L::THREADS, WAVES = L::WAVES, SIZE = DlIO<IO>::SIZE;
+  constexpr int KT = DP / 16 / WAVES;   // key tiles of a wave
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PlaneMat<DL_C, DP, NI> K{(__bf16*)lds}, Q{(__bf16*)(lds + L::KQ)};
-  const PlaneMat<DL_C, 32, NP> M1{(__bf16*)(lds + 2 * L::KQ)}, M2{(__bf16*)(lds + 2 * L::KQ + L::M)};
-  DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::M);
-  float* colsum = (float*)(lds + 2 * L::KQ + 2 * L::M + sizeof(DlGates));   // [2 tiles of i][32]
-  float* part = colsum + 2 * 32;               // [3][halves][32]: q·E1, k·E2, k·E3
-  float* rows = part + 3 * HALVES * 32;        // [3][32]: row sums of M, of the terms of dbeta, dX·V
-  float* dots = rows + 3 * 32;                 // [2] sums of S·dS' by halves
+  // 32 columns of dX, U and dO; then dX's and U's place is M1's and M2's
+  const PlaneMat<DL_C, 32, NP> X{(__bf16*)(lds + 2 * L::KQ)}, Y{(__bf16*)(lds + 2 * L::KQ + L::X)}, M1 = X, M2 = Y;
+  const PlaneMat<DL_C, 32, NI> G{(__bf16*)(lds + 2 * L::KQ + 2 * L::X)};
+  DlGates& s = *(DlGates*)(lds + 2 * L::KQ + 2 * L::X + L::G);
+  float* sums = (float*)(lds + 2 * L::KQ + 2 * L::X + L::G + sizeof(DlGates));
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), it = wave & 1, half = wave >> 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int it = wave & 1, jt = wave < 2 ? it : 1 - it;   // this wave's tile of dP and dA: positions i, j
   const int group = a.Hv / a.Hk, b = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk, c = blockIdx.y, t0 = c * DL_C;
   const int len = dl_len(a, b), nC = (a.T + DL_C - 1) / DL_C, nc = (len + DL_C - 1) / DL_C;
   const int64_t ks = (int64_t)a.Hk * a.Dk;
-  const int i = 16 * it + n, d0 = half * 64;   // this lane's position, this wave's key columns
+  const int d0 = wave * 16 * KT;   // this wave's key columns
   const int outrows = min(a.T - t0, DL_C);
   const DlBuf dqbuf = dl_buf((IO*)a.dq + (((int64_t)b * a.T + t0) * a.Hk + hk) * a.Dk, outrows, ks, a.Dk, SIZE),
               dkbuf = dl_buf((IO*)a.dk + (((int64_t)b * a.T + t0) * a.Hk + hk) * a.Dk, outrows, ks, a.Dk, SIZE);
-  auto store = [&](const f4* gq, const f4* gk) __attribute__((always_inline)) {
+  f4 gq[KT][2], gk[KT][2];   // rows: key columns, columns: positions
 #pragma unroll
-    for (int u = 0; u < UT; ++u) {
-      const int at = dl_lane(d0 + 16 * u + 4 * kg < a.Dk, (int)(i * ks + 4 * kg) * SIZE);
-      DlIO<IO>::store4(dqbuf, at, (d0 + 16 * u) * SIZE, gq[u]);
-      DlIO<IO>::store4(dkbuf, at, (d0 + 16 * u) * SIZE, gk[u]);
-    }
+  for (int u = 0; u < KT; ++u) gq[u][0] = gq[u][1] = gk[u][0] = gk[u][1] = DL_ZERO;
+  auto store = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < KT; ++u)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int at = dl_lane(d0 + 16 * u + 4 * kg < a.Dk, (int)((16 * p + n) * ks + 4 * kg) * SIZE);
+        DlIO<IO>::store4(dqbuf, at, (d0 + 16 * u) * SIZE, gq[u][p]);
+        DlIO<IO>::store4(dkbuf, at, (d0 + 16 * u) * SIZE, gk[u][p]);
+      }
   };
-  f4 gq[UT], gk[UT];   // rows: key columns, columns: positions
-#pragma unroll
-  for (int u = 0; u < UT; ++u) gq[u] = gk[u] = DL_ZERO;
   if (c >= nc) {   // behind the row's length
-    store(gq, gk);
+    store();
     if (tid < outrows)
       for (int h = hk * group; h < (hk + 1) * group; ++h) {
         const int64_t at = ((int64_t)b * a.T + t0 + tid) * a.Hv + h;
@@ -851,190 +892,227 @@ __global__ __launch_bounds__(DP > 64 ? 256 : 128, 2) void k_delta_grads(DeltaArg
   }
   const int left = min(len - t0, DL_C);
 
-  // K and Q are on their way while the first value head's contractions run
+  // 8 columns of a row: two waves take dX and V, the others U and dO
+  const int pr = (tid & 127) >> 2, pc = (tid & 3) * 8;
+  typename DlIO<float>::Raw8 rx;   // dX or U
+  typename DlIO<IO>::Raw8 rv;      // V or dO
+  auto fetch = [&](int h, int c0) __attribute__((always_inline)) {
+    const int64_t row = ((int64_t)b * a.Hv + h) * a.T + t0;
+    const bool on = c0 + pc < a.Dv;
+    const int v = dl_lane(on, (pr * a.Dv + pc) * 4);
+    const bool x = wave < 2;
+    const IO* p = x ? (const IO*)a.v + b * a.vs[0] + h * a.vs[2] + t0 * a.vs[1]
+                    : (const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + t0 * a.dos[1];
+    const int64_t st = x ? a.vs[1] : a.dos[1];
+    rx = DlIO<float>::load8(dl_buf((x ? a.dX : a.U) + row * a.Dv, left, a.Dv, a.Dv, 4), v, c0 * 4);
+    rv = DlIO<IO>::load8(dl_buf(p, left, st, a.Dv, SIZE), dl_lane(on, (int)(pr * st + pc) * SIZE), c0 * SIZE);
+  };
+  float gates[2];
+  if (wave == 0) dl_gates_load(gates, a, b, hk * group, t0, len);
+  fetch(hk * group, 0);
   DlTile<IO, DP, THREADS> kt, qt;
   kt.load(dl_buf((const IO*)a.k + b * a.ks[0] + hk * a.ks[2] + t0 * a.ks[1], left, a.ks[1], a.Dk, SIZE), a.ks[1], a.Dk, tid);
   qt.load(dl_buf((const IO*)a.q + b * a.qs[0] + hk * a.qs[2] + t0 * a.qs[1], left, a.qs[1], a.Dk, SIZE), a.qs[1], a.Dk, tid);
 
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
+    float* colsum = sums + (h & 1) * L::SUMS;    // [2 tiles of i][32]
+    float* part = colsum + 2 * 32;               // [3][waves][32]: q·E1, k·E2, k·E3
+    float* rows = part + 3 * WAVES * 32;         // [5][32]: row sums of M, of the terms of dbeta (two tiles of j each), dX·V
+    float* dots = rows + 5 * 32;                 // [waves]: sums of S·dS'
     const int64_t bh = (int64_t)b * a.Hv + h, size = (int64_t)a.Dk * a.Dv;
     const float* S0 = c > 0 ? a.S0 + (bh * (nC - 1) + c - 1) * size : a.state0 ? a.state0 + bh * size : nullptr;
     // (after the last chunk of the row's length: the gradient handed in)
     const float* dS = c < nc - 1 ? a.dS + (bh * (nC - 1) + c) * size : a.dstate ? a.dstate + bh * size : nullptr;
-    const DlBuf gbuf = dl_buf((const IO*)a.d_o + b * a.dos[0] + h * a.dos[2] + t0 * a.dos[1], left, a.dos[1], a.Dv, SIZE),
-                vbuf = dl_buf((const IO*)a.v + b * a.vs[0] + h * a.vs[2] + t0 * a.vs[1], left, a.vs[1], a.Dv, SIZE),
-                xbuf = dl_buf(a.dX + (bh * a.T + t0) * a.Dv, left, a.Dv, a.Dv, 4),
-                ubuf = dl_buf(a.U + (bh * a.T + t0) * a.Dv, left, a.Dv, a.Dv, 4),
-                sbuf = dl_buf(S0, S0 != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4),
+    const DlBuf sbuf = dl_buf(S0, S0 != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4),
                 ebuf = dl_buf(dS, dS != nullptr ? a.Dk : 0, a.Dv, a.Dv, 4);
-    float gates[2];
-    if (wave == 0) dl_gates_load(gates, a, b, h, t0, len);
+    const bool states = S0 != nullptr || dS != nullptr;
+    DlRow rs[KT], re[KT];   // (a state that is not there has no rows: nothing is read)
+    auto rows_of = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        rs[u].load(sbuf, d0 + 16 * u, a.Dv, c0, a.Dv);
+        re[u].load(ebuf, d0 + 16 * u, a.Dv, c0, a.Dv);
+      }
+    };
+    if (states) rows_of(0);
 
-    // dP, dA: the diagonal tile, and (second tile of positions) the one with the first tile of j
-    f4 dp = DL_ZERO, da = DL_ZERO, dp0 = DL_ZERO, da0 = DL_ZERO;
-    float dot = 0.f;
-    if (half == 0) {
-      for (int c0 = 0; c0 < a.Dv; c0 += 32) {
-        bf16x8 go[NI], gx[NP], uu[NP], y[NP];
-        DlRow rx, ru, ry;
-        dl_operand<IO>(go, gbuf, 16 * it, a.dos[1], c0, a.Dv);
-        rx.load(xbuf, 16 * it, a.Dv, c0, a.Dv);
-        ru.load(ubuf, 16 * it, a.Dv, c0, a.Dv);
-        ry.load(ubuf, 0, a.Dv, c0, a.Dv);
-        f4 v0, v1;
-        {
-          const int v = (int)(n * a.vs[1] + 4 * kg) * SIZE, sv = (int)(16 * it * a.vs[1] + c0) * SIZE;
-          DlIO<IO>::load4x2(vbuf, dl_lane(c0 + 4 * kg < a.Dv, v), sv, dl_lane(c0 + 16 + 4 * kg < a.Dv, v), sv + 16 * SIZE, v0, v1);
+    // dP, dA and the states' part
+    f4 dp = DL_ZERO, da = DL_ZERO;
+    f4 e1[KT][2], e2[KT][2], e3[KT][2];
+#pragma unroll
+    for (int u = 0; u < KT; ++u)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) e1[u][p] = e2[u][p] = e3[u][p] = DL_ZERO;
+    float dot = 0.f, both = 0.f;
+    for (int c0 = 0; c0 < a.Dv; c0 += 32) {
+      {
+        bf16x8 f[NP];
+        DlIO<float>::planes(rx, f);
+        (wave < 2 ? X : Y).put8(pr, pc, f);
+        if (wave < 2) {
+          dot = DlIO<IO>::dot(rv, rx.a, rx.b, dot);
+        } else {
+          DlIO<IO>::planes(rv, f);
+          G.put8(pr, pc, f);
         }
-        rx.planes(gx);
-        ru.planes(uu);
-        dp = pl_mm<NP, NI>(uu, go, dp);
-        da = pl_mm<NP, NP>(uu, gx, da);
-        if (it == 1) {
-          ry.planes(y);
-          dp0 = pl_mm<NP, NI>(y, go, dp0);
-          da0 = pl_mm<NP, NP>(y, gx, da0);
+      }
+      if (c0 == 0) {
+        if (wave == 0) dl_gates(s, gates);
+        if (h == hk * group) {
+          kt.put(K, tid);
+          qt.put(Q, tid);
         }
-        dot = rx.dot(v0, v1, dot);
       }
-      dot = dl_sum4(dot);
-      if (kg == 0) rows[2 * 32 + i] = dot;
-    }
-    if (wave == 0) dl_gates(s, gates);
-    if (h == hk * group) {
-      kt.put(K, tid);
-      qt.put(Q, tid);
-    }
-    __syncthreads();
-    const float gam = s.gam[i], be = s.beta[i], rest = s.rest[i];
-    if (half == 0) {
-      float rm = 0.f, rb = 0.f;
-      const double gi = s.G[i];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f4 kk = DL_ZERO, qk = DL_ZERO, m1 = DL_ZERO, m2 = DL_ZERO, cs = DL_ZERO;
-        if (j <= it) {
-#pragma unroll
-          for (int t = 0; t < DP / 32; ++t) {
-            bf16x8 ki[NI], qi[NI], kj[NI];
-            K.row(ki, 16 * it, t);
-            Q.row(qi, 16 * it, t);
-            K.row(kj, 16 * j, t);
-            kk = pl_mm<NI, NI>(kj, ki, kk);
-            qk = pl_mm<NI, NI>(kj, qi, qk);
-          }
-          const f4 dpj = j == it ? dp : dp0, daj = j == it ? da : da0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int jj = 16 * j + 4 * kg + r;
-            const float d = jj <= i ? dl_exp2(gi - s.G[jj]) : 0.f;
-            const float w = jj < i ? -d * daj[r] : 0.f;
-            m1[r] = jj <= i ? a.scale * d * dpj[r] : 0.f;
-            m2[r] = be * w;
-            cs[r] = m1[r] * qk[r] + m2[r] * kk[r];
-            rm += cs[r];
-            rb += w * kk[r];
-          }
-        }
-        dl_put4(M1, i, 16 * j + 4 * kg, m1);
-        dl_put4(M2, i, 16 * j + 4 * kg, m2);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) cs[r] = dl_sum16(cs[r]);
-        if (n == 0) *reinterpret_cast<f4*>(colsum + it * 32 + 16 * j + 4 * kg) = cs;
+      __syncthreads();
+      if (c0 + 32 < a.Dv) fetch(h, c0 + 32);
+      if (jt <= it) {
+        bf16x8 go[NI], gx[NP], y[NP];
+        G.row(go, 16 * it, 0);
+        X.row(gx, 16 * it, 0);
+        Y.row(y, 16 * jt, 0);
+        dp = pl_mm<NP, NI>(y, go, dp);
+        da = pl_mm<NP, NP>(y, gx, da);
       }
-      rm = dl_sum4(rm);
-      rb = dl_sum4(rb);
-      if (kg == 0) {
-        rows[i] = rm;
-        rows[32 + i] = rb;
-      }
-    }
-    __syncthreads();
-    // the states' part, two key tiles at a time
-    float r1 = 0.f, r2 = 0.f, r3 = 0.f, both = 0.f;
-    if (S0 != nullptr || dS != nullptr) {
+      if (states) {
 #pragma unroll
-      for (int u0 = 0; u0 < UT; u0 += 2) {
-        f4 e1[2] = {DL_ZERO, DL_ZERO}, e2[2] = {DL_ZERO, DL_ZERO}, e3[2] = {DL_ZERO, DL_ZERO};
-        for (int c0 = 0; c0 < a.Dv; c0 += 32) {
-          bf16x8 go[NI], gx[NP], uu[NP], y[NP];
-          DlRow rx, ru, rs[2], re[2];   // (a state that is not there has no rows: nothing is read)
-          dl_operand<IO>(go, gbuf, 16 * it, a.dos[1], c0, a.Dv);
-          rx.load(xbuf, 16 * it, a.Dv, c0, a.Dv);
-          ru.load(ubuf, 16 * it, a.Dv, c0, a.Dv);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            rs[u].load(sbuf, d0 + 16 * (u0 + u), a.Dv, c0, a.Dv);
-            re[u].load(ebuf, d0 + 16 * (u0 + u), a.Dv, c0, a.Dv);
-          }
+        for (int u = 0; u < KT; ++u) {
+          bf16x8 y[NP], f[NP];
+          both = rs[u].dot(re[u].a, re[u].b, both);
           if (S0 != nullptr) {
-            rx.planes(gx);
+            rs[u].planes(y);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              rs[u].planes(y);
-              e1[u] = pl_mm<NP, NI>(y, go, e1[u]);
-              e2[u] = pl_mm<NP, NP>(y, gx, e2[u]);
+            for (int p = 0; p < 2; ++p) {
+              bf16x8 go[NI];
+              G.row(go, 16 * p, 0);
+              X.row(f, 16 * p, 0);
+              e1[u][p] = pl_mm<NP, NI>(y, go, e1[u][p]);
+              e2[u][p] = pl_mm<NP, NP>(y, f, e2[u][p]);
             }
           }
           if (dS != nullptr) {
-            ru.planes(uu);
+            re[u].planes(y);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              re[u].planes(y);
-              e3[u] = pl_mm<NP, NP>(y, uu, e3[u]);
-              both = rs[u].dot(re[u].a, re[u].b, both);
+            for (int p = 0; p < 2; ++p) {
+              Y.row(f, 16 * p, 0);
+              e3[u][p] = pl_mm<NP, NP>(y, f, e3[u][p]);
             }
           }
         }
+        if (c0 + 32 < a.Dv) rows_of(c0 + 32);
+      }
+      __syncthreads();
+    }
+    if (wave < 2) {
+      dot += __shfl_xor(dot, 1);
+      dot += __shfl_xor(dot, 2);
+      if ((tid & 3) == 0) rows[4 * 32 + pr] = dot;
+    }
+    {
+      const int i = 16 * it + n;   // this lane's position
+      f4 kk = DL_ZERO, qk = DL_ZERO, m1 = DL_ZERO, m2 = DL_ZERO, cs = DL_ZERO;
+      float rm = 0.f, rb = 0.f;
+      if (jt <= it) {
+        const float be = s.beta[i];
+        const double gi = s.G[i];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f4 kx = dl_get4(K, i, d0 + 16 * (u0 + u) + 4 * kg), qx = dl_get4(Q, i, d0 + 16 * (u0 + u) + 4 * kg);
+        for (int t = 0; t < DP / 32; ++t) {
+          bf16x8 ki[NI], qi[NI], kj[NI];
+          K.row(ki, 16 * it, t);
+          Q.row(qi, 16 * it, t);
+          K.row(kj, 16 * jt, t);
+          kk = pl_mm<NI, NI>(kj, ki, kk);
+          qk = pl_mm<NI, NI>(kj, qi, qk);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * jt + 4 * kg + r;
+          const float d = j <= i ? dl_exp2(gi - s.G[j]) : 0.f;
+          const float w = j < i ? -d * da[r] : 0.f;
+          m1[r] = j <= i ? a.scale * d * dp[r] : 0.f;
+          m2[r] = be * w;
+          cs[r] = m1[r] * qk[r] + m2[r] * kk[r];
+          rm += cs[r];
+          rb += w * kk[r];
+          cs[r] = dl_sum16(cs[r]);
+        }
+        rm = dl_sum4(rm);
+        rb = dl_sum4(rb);
+      }
+      dl_put4(M1, i, 16 * jt + 4 * kg, m1);
+      dl_put4(M2, i, 16 * jt + 4 * kg, m2);
+      if (n == 0) *reinterpret_cast<f4*>(colsum + it * 32 + 16 * jt + 4 * kg) = cs;
+      if (kg == 0) {
+        rows[(wave >> 1) * 32 + i] = rm;
+        rows[(2 + (wave >> 1)) * 32 + i] = rb;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      float r1 = 0.f, r2 = 0.f, r3 = 0.f;
+      if (states) {
+        const float gam = s.gam[16 * p + n], be = s.beta[16 * p + n], rest = s.rest[16 * p + n];
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          const f4 kx = dl_get4(K, 16 * p + n, d0 + 16 * u + 4 * kg), qx = dl_get4(Q, 16 * p + n, d0 + 16 * u + 4 * kg);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            r1 = __builtin_fmaf(qx[r], e1[u][r], r1);
-            r2 = __builtin_fmaf(kx[r], e2[u][r], r2);
-            r3 = __builtin_fmaf(kx[r], e3[u][r], r3);
+            r1 = __builtin_fmaf(qx[r], e1[u][p][r], r1);
+            r2 = __builtin_fmaf(kx[r], e2[u][p][r], r2);
+            r3 = __builtin_fmaf(kx[r], e3[u][p][r], r3);
           }
-          gq[u0 + u] += (a.scale * gam) * e1[u];
-          gk[u0 + u] += rest * e3[u] - (be * gam) * e2[u];
+          gq[u][p] += (a.scale * gam) * e1[u][p];
+          gk[u][p] += rest * e3[u][p] - (be * gam) * e2[u][p];
         }
+        r1 = dl_sum4(r1);
+        r2 = dl_sum4(r2);
+        r3 = dl_sum4(r3);
       }
-      r1 = dl_sum4(r1);
-      r2 = dl_sum4(r2);
-      r3 = dl_sum4(r3);
-      both = dl_sum4(dl_sum16(both));
+      if (kg == 0) {
+        part[wave * 32 + 16 * p + n] = r1;
+        part[(WAVES + wave) * 32 + 16 * p + n] = r2;
+        part[(2 * WAVES + wave) * 32 + 16 * p + n] = r3;
+      }
     }
-    if (kg == 0) {
-      part[half * 32 + i] = r1;
-      part[(HALVES + half) * 32 + i] = r2;
-      part[(2 * HALVES + half) * 32 + i] = r3;
-    }
-    if (it == 0 && lane == 0) dots[half] = both;
-    {
-      bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
-      M1.row(m1, 16 * it, 0);
-      M2.row(m2, 16 * it, 0);
-      M1.col(m1t, 0, 16 * it);
-      M2.col(m2t, 0, 16 * it);
+    if (states) both = dl_sum4(dl_sum16(both));
+    if (lane == 0) dots[wave] = both;
+    __syncthreads();
 #pragma unroll
-      for (int u = 0; u < UT; ++u) {
+    for (int p = 0; p < 2; ++p) {
+      bf16x8 m1[NP], m1t[NP], m2[NP], m2t[NP];
+      M1.row(m1, 16 * p, 0);
+      M2.row(m2, 16 * p, 0);
+      M1.col(m1t, 0, 16 * p);
+      M2.col(m2t, 0, 16 * p);
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
         bf16x8 f[NI];
         K.col(f, 0, d0 + 16 * u);
-        gq[u] = pl_mm<NI, NP>(f, m1, gq[u]);
-        gk[u] = pl_mm<NI, NP>(f, m2, gk[u]);
-        gk[u] = pl_mm<NI, NP>(f, m2t, gk[u]);
+        gq[u][p] = pl_mm<NI, NP>(f, m1, gq[u][p]);
+        gk[u][p] = pl_mm<NI, NP>(f, m2, gk[u][p]);
+        gk[u][p] = pl_mm<NI, NP>(f, m2t, gk[u][p]);
         Q.col(f, 0, d0 + 16 * u);
-        gk[u] = pl_mm<NI, NP>(f, m1t, gk[u]);
+        gk[u][p] = pl_mm<NI, NP>(f, m1t, gk[u][p]);
       }
     }
-    __syncthreads();
+    const bool more = h + 1 < (hk + 1) * group;
+    if (more) {
+      fetch(h + 1, 0);
+      __syncthreads();   // M is read: the next value head's dX and U take its place
+    }
     if (wave == 0) {
       const int j = lane & 31;
       const float gj = s.gam[j];
-      float qe = part[j], ke = part[HALVES * 32 + j], kd = part[2 * HALVES * 32 + j];
-      if (HALVES == 2) qe += part[32 + j], ke += part[3 * 32 + j], kd += part[5 * 32 + j];
+      float qe = 0.f, ke = 0.f, kd = 0.f;
+      double sd = 0.0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        qe += part[w * 32 + j];
+        ke += part[(WAVES + w) * 32 + j];
+        kd += part[(2 * WAVES + w) * 32 + j];
+        sd += dots[w];
+      }
       const double leave = (double)s.rest[j] * kd;
-      double at = (double)rows[j] + (double)a.scale * gj * qe - (double)s.beta[j] * gj * ke - leave;
+      double at = (double)rows[j] + rows[32 + j] + (double)a.scale * gj * qe - (double)s.beta[j] * gj * ke - leave;
       at -= (double)colsum[j] + (double)colsum[32 + j];
       double all = leave;
 #pragma unroll
@@ -1043,20 +1121,21 @@ __global__ __launch_bounds__(DP > 64 ? 256 : 128, 2) void k_delta_grads(DeltaArg
         const double down = __shfl_down(at, o, 32);
         if (j + o < 32) at += down;
       }
-      at += all + (double)s.gam[DL_C - 1] * (HALVES == 2 ? (double)dots[0] + dots[1] : (double)dots[0]);
+      at += all + (double)s.gam[DL_C - 1] * sd;
       const int64_t out = ((int64_t)b * a.T + t0 + j) * a.Hv + h;
       if (lane < 32 && j < outrows) {
         a.dg[out] = j < left ? (float)at : 0.f;
-        a.dbeta[out] = j < left ? rows[64 + j] - gj * ke + rows[32 + j] : 0.f;
+        a.dbeta[out] = j < left ? rows[128 + j] - gj * ke + (rows[64 + j] + rows[96 + j]) : 0.f;
       }
+      if (more) dl_gates_load(gates, a, b, h + 1, t0, len);
     }
-    if (h + 1 < (hk + 1) * group) __syncthreads();   // the sums are read: the next value head may write them
   }
-  if (i >= left) {
 #pragma unroll
-    for (int u = 0; u < UT; ++u) gq[u] = gk[u] = DL_ZERO;
-  }
-  store(gq, gk);
+  for (int p = 0; p < 2; ++p)
+    if (16 * p + n >= left)
+#pragma unroll
+      for (int u = 0; u < KT; ++u) gq[u][p] = gk[u][p] = DL_ZERO;
+  store();
 }
 
 // ------------------------------------------------------------- one token ----
@@ -1166,9 +1245,10 @@ static int delta_ct(int64_t heads, int Dk, int Dv, int type) {
 
 // Segments.  A chunk takes a wave of 1, 2, 4 column tiles about 4.5, 7.5, 12 us with a SIMD of its own (1024 of them), 1.75
 // times that beside another (2048 at once); with segments there are two passes, the first over the transition's
-// columns too but without outputs, each a segment long, and a join of about 1 us a segment.  Measured at width 128,
+// columns too but without outputs, each a segment long, and a join of 1 to 1.5 us a segment.  Measured at width 128,
 // 4 x 8 heads x 4096 positions, forward and backward: 8 segments 819 us, 16 749, 32 808, 64 960; 8 heads x 8191
-// positions, forward: 8 segments 269 us, 16 188, 32 192, 37 (a wave too many for the SIMDs in either pass) 225, 64 241.
+// positions, forward: 8 segments 269 us, 16 188, 32 192, 37 (a wave too many for the SIMDs in either pass) 225, 64 241
+// (before the joins and the gradients' kernel were made faster: now 600 with 16 and 170 with 32).
 struct DeltaCut {
   int nseg, per;
 };
@@ -1242,8 +1322,9 @@ static int delta_bwd_t(const DeltaArgs& a, hipStream_t st) {
     if (!done && ct >= 2) rc = delta_scan_ct<IO, DP, 2>(a, st), done = true;
   if (!done) rc = delta_scan_ct<IO, DP, 1>(a, st);
   if (rc != RG_OK) return rc;
-  using L = DlGradLds<DP, DlIO<IO>::N>;
-  return delta_go(k_delta_grads<IO, DP>, dim3(a.B * a.Hk, (a.T + DL_C - 1) / DL_C), L::THREADS, L::BYTES, a, st);
+  constexpr int GP = DP > 64 ? 128 : 64;   // (two key tiles at least: four waves have one or two each)
+  using L = DlGradLds<GP, DlIO<IO>::N>;
+  return delta_go(k_delta_grads<IO, GP>, dim3(a.B * a.Hk, (a.T + DL_C - 1) / DL_C), L::THREADS, L::BYTES, a, st);
 }
 #define DL_DISPATCH(F)                                                                             \
   (type == 0 ? (a.Dk <= 32 ? F<float, 32>(a, st) : a.Dk <= 64 ? F<float, 64>(a, st) : F<float, 128>(a, st)) \
@@ -1272,6 +1353,11 @@ extern "C" int64_t rg_delta_chunk_floats(int B, int T, int Hv, int Dk, int Dv) {
 }
 extern "C" int rg_delta_segments(int B, int T, int Hv, int Dk, int Dv) {
   return B > 0 && T > 0 ? delta_cut(B, T, Hv, Dk, Dv).nseg : 1;
+}
+
+extern "C" int64_t rg_delta_trans_floats(int B, int T, int Hv, int Dk, int Dv) {
+  const int n = rg_delta_segments(B, T, Hv, Dk, Dv);
+  return n > 1 ? (int64_t)B * Hv * n * dl_trans_floats(Dk) : 0;
 }
 
 extern "C" int rg_delta_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta,

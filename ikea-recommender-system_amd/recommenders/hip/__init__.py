@@ -25,7 +25,7 @@ U64 = C.c_uint64
 # entry points returning int64_t (all others return int)
 RESTYPE_I64 = {"rg_sampled_work_bytes", "rg_head_work_bytes", "rg_head_plane_bytes", "rg_gru_wide_work_bytes",
                "rg_scatter_rows_work_bytes", "rg_flash_dw_work_bytes", "rg_shard_dedup_work_bytes",
-               "rg_flash_topk_work_bytes", "rg_flash_zs_bytes", "rg_delta_chunk_floats",
+               "rg_flash_topk_work_bytes", "rg_flash_zs_bytes", "rg_delta_chunk_floats", "rg_delta_trans_floats",
                "rg_linear_ce_work_floats", "rg_linear_ce_saved_bytes"}
 
 # name -> argtypes
@@ -151,6 +151,7 @@ SIGNATURES = {
     "rg_lazy_adam_rows": [P, P, P, P, I, P, P, P, P, P, I64, P, P, I32, I32, P, P, P],
     "rg_delta_chunk_floats": [I, I, I, I, I],
     "rg_delta_segments": [I, I, I, I, I],
+    "rg_delta_trans_floats": [I, I, I, I, I],
     "rg_delta_fwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P],
     "rg_delta_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P, P, P, P, P, P, P, P, P],
     "rg_delta_step": [P, P, P, P, P, P, I, I, I, I, I, I, F, P, I64, P, P],

@@ -99,7 +99,8 @@ def _plan(q, k, v, g, beta, lens, state):
     p.forward, p.backward = entry("rg_delta_fwd"), entry("rg_delta_bwd")
     p.chunks = call("rg_delta_chunk_floats", p.B, p.T, p.Hv, p.Dk, p.Dv)
     n = call("rg_delta_segments", p.B, p.T, p.Hv, p.Dk, p.Dv)
-    p.trans, p.local = ((p.B, p.Hv, n, p.Dk, p.Dk), (p.B, p.Hv, n, p.Dk, p.Dv)) if n > 1 else (None, None)
+    trans = call("rg_delta_trans_floats", p.B, p.T, p.Hv, p.Dk, p.Dv)
+    p.trans, p.local = (trans, (p.B, p.Hv, n, p.Dk, p.Dv)) if n > 1 else (None, None)
     return p
 
 

@@ -620,12 +620,13 @@ int rg_comm_reduce_scatter(void* comm, const void* send, void* recv, int64_t n, 
  * optional: positions at or behind it are not read, do not change the state and get zeros.  Contiguous: o, dv
  * (B, T, Hv, Dv), dq, dk (B, T, Hk, Dk), dg, dbeta (B, T, Hv), the states (B, Hv, Dk, Dv) fp32.
  * For the backward pass the forward leaves U (B, Hv, T, Dv) and S0 (rg_delta_chunk_floats values, when T > 32); both
- * NULL otherwise.  A long T is cut into n = rg_delta_segments(..) segments; when n > 1: trans (B, Hv, n, Dk, Dk) fp32,
- * which the backward call reads again, and local (B, Hv, n, Dk, Dv) fp32, work space of one call.  dX is of U's size, dS
+ * NULL otherwise.  A long T is cut into n = rg_delta_segments(..) segments; when n > 1: trans (rg_delta_trans_floats
+ * values), which the backward call reads again, and local (B, Hv, n, Dk, Dv) fp32, work space of one call.  dX is of U's size, dS
  * of S0's.  state0, dstate, dstate0 optional (NULL: zero / not wanted).
  * rg_delta_step: one token, q, k (B, Hk, Dk), v (B, Hv, Dv); state updated in place, its rows state_stride apart. */
 int64_t rg_delta_chunk_floats(int B, int T, int Hv, int Dk, int Dv);
 int rg_delta_segments(int B, int T, int Hv, int Dk, int Dv);
+int64_t rg_delta_trans_floats(int B, int T, int Hv, int Dk, int Dv);
 int rg_delta_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const int64_t* strides,
                  const int64_t* lens, const float* state0, int type, int B, int T, int Hk, int Hv, int Dk, int Dv,
                  float scale, void* o, float* state, float* U, float* S0, float* trans, float* local,
