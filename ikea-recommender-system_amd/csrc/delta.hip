@@ -1223,7 +1223,7 @@ static int delta_check(const DeltaArgs& a, int type) {
   if (type != 0 && type != 1) return RG_ERR_ARG;
   if (a.B <= 0 || a.T <= 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk) return RG_ERR_SHAPE;
   if (a.Dk <= 0 || a.Dk > 128 || a.Dk % 8 || a.Dv <= 0 || a.Dv > 128 || a.Dv % 8) return RG_ERR_SHAPE;
-  if ((int64_t)a.B * a.Hv > (1 << 24) || (a.T + DL_C - 1) / DL_C > 65535) return RG_ERR_SHAPE;
+  if ((int64_t)a.B * a.Hv >= (1 << 24) || (a.T + DL_C - 1) / DL_C > 65535) return RG_ERR_SHAPE;
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.g == nullptr || a.beta == nullptr) return RG_ERR_ARG;
   return RG_OK;
 }

@@ -72,6 +72,8 @@ class _Plan:
                 fail(name, f"a tensor of shape {(*q.shape[:-2], Hv)} is expected")
             tensor(name, t[..., None], (*q.shape[:-2], Hv, 1), (torch.float32,), q.device)   # any strides
         self.B, self.T = q.shape[0], q.shape[1] if lead == 2 else 1
+        if self.B * Hv >= 1 << 24 or self.T > 65535 * 32:
+            fail("q", f"less than 2^24 rows times value heads and at most 2^21 − 32 positions are expected, got {self.B}·{Hv} and {self.T}")
         if self.T > 1:
             for name, t, d in (("q", q, Dk), ("k", k, Dk), ("v", v, Dv), ("g", g, 1), ("beta", beta, 1)):
                 _apart(name, t, d)

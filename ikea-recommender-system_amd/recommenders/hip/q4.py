@@ -30,12 +30,18 @@ def _table(K, group):
         fail("columns", f"a multiple of the group size {group} up to {K_MAX} is expected, got {K}")
 
 
+def _rows(name, t):
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        fail(name, f"rows overlap: stride {t.stride(0)}, {t.shape[1]} columns")
+
+
 def q4_pack(W, group=32):
     """Quantise a (N, K) fp32 or bf16 table: (codes, scales).  Per group the scale is max |w| / 7 rounded to bf16 and a
     code is round(w / scale) + 8, ties to even, clamped to 0 .. 15."""
     tensor("W", W, (None, None), (torch.float32, torch.bfloat16))
     N, K = W.shape
     _table(K, group)
+    _rows("W", W)
     codes = torch.empty(N, K // 2, dtype=torch.uint8, device=W.device)
     scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=W.device)
     if N:
@@ -51,6 +57,7 @@ def _plan(x, codes, scales, bias):
     M, K = x.shape
     if M > M_MAX:
         fail("x", f"at most {M_MAX} rows are expected, got {M}")
+    _rows("x", x)
     whole("codes", codes, (None, K // 2), (torch.uint8,), x.device)
     N = codes.shape[0]
     whole("scales", scales, (N, None), (torch.bfloat16,), x.device)

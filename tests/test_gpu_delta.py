@@ -88,6 +88,8 @@ CASES = [
     (300, 33, 1, 1, 64, 64, list(range(33)) * 9 + [3, 33, 0], False),
     (900, 50, 1, 2, 64, 64, [1 + 50 * i // 900 for i in range(900)], False),
     (2, 1100, 2, 2, 128, 96, [1100, 517], True),
+    (1, 1500, 1, 1, 40, 24, None, True),
+    (2, 900, 1, 2, 104, 72, [411, 900], True),
 ]
 
 

@@ -128,3 +128,15 @@ def test_scores_of_a_trained_head():
     codes, scales = q4_pack(W, 32)
     h = torch.tanh(torch.randn(3, 64, device="cuda"))
     check(q4_scores(h, codes, scales, b), h, codes, scales, b, 32)
+
+
+def test_rows_that_overlap_are_refused():
+    """A row repeated by a stride of 0 is not K apart from itself: refused, not read as if it were."""
+    from recommenders.hip.q4 import q4_pack, q4_scores
+    codes, scales, g = table(20, 64, 32)
+    x = torch.randn(1, 64, generator=g, device="cuda")
+    for bad in (x.expand(5, 64), torch.as_strided(x, (2, 32), (16, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            q4_scores(bad, *q4_pack(torch.randn(9, bad.shape[1], device="cuda")))
+        with pytest.raises(ValueError, match="overlap"):
+            q4_pack(bad)

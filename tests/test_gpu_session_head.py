@@ -124,3 +124,38 @@ def test_a_step_in_place_is_a_change():
     delta_rule_step(q[:, 0], k[:, 0], v[:, 0], a[:, 0], beta[:, 0], state)
     with pytest.raises(RuntimeError, match="in place"):
         delta_rule_backward(saved, o)
+
+
+def test_two_streams_at_once():
+    """Two training steps and two scorings side by side, each on a stream of its own: nothing is shared between calls."""
+    from recommenders.hip.delta import delta_rule, delta_rule_backward
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    from recommenders.hip.q4 import q4_pack, q4_scores
+    w, W, b, g = model(3)
+    codes, scales = q4_pack(W, 64)
+    cases = []
+    for B, T in ((40, 90), (3, 1000)):
+        items = torch.randint(0, V, (B, T), generator=g, device="cuda")
+        cases.append(([t.contiguous() for t in project(w, w["E"][items])], items.flatten()))
+
+    def step(x, target):
+        o, s, saved = delta_rule(*x, save=True)
+        h = o.flatten(2).flatten(0, 1).bfloat16()
+        loss, kept = linear_ce(h, W, target, bias=b, save=True)
+        grads = linear_ce_backward(kept, torch.full_like(loss, 1 / len(loss)))
+        back = delta_rule_backward(saved, grads[0].float().view(o.shape))
+        return [o, s, loss, *grads, *back[:5], q4_scores(h[:7], codes, scales, bias=b)]
+
+    want = [step(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        got = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(step(*c))
+        torch.cuda.synchronize()
+        for a, e in zip(got, want):
+            for y, z in zip(a, e):
+                assert torch.equal(y, z)

@@ -75,6 +75,7 @@ def test_delta_c_entry_refusals():
     def step(stride=256, state=p, B=2):
         return lib.rg_delta_step(p, p, p, p, p, s, 0, B, 1, 1, 16, 16, 1.0, state, stride, p, None)
     assert step(stride=255) == -1 and step(stride=252) == -1 and step(state=p + 4) == -1 and step(B=0) == -3
+    assert fwd(B=1 << 24) == -3   # 256 threads for each would pass a grid's 2^32
     assert lib.rg_delta_chunk_floats(2, 32, 3, 8, 8) == 0 and lib.rg_delta_chunk_floats(2, 33, 3, 8, 16) == 2 * 3 * 8 * 16
 
 
