@@ -1248,7 +1248,7 @@ static int delta_ct(int64_t heads, int Dk, int Dv, int type) {
 // columns too but without outputs, each a segment long, and a join of 1 to 1.5 us a segment.  Measured at width 128,
 // 4 x 8 heads x 4096 positions, forward and backward: 8 segments 819 us, 16 749, 32 808, 64 960; 8 heads x 8191
 // positions, forward: 8 segments 269 us, 16 188, 32 192, 37 (a wave too many for the SIMDs in either pass) 225, 64 241
-// (before the joins and the gradients' kernel were made faster: now 600 with 16 and 170 with 32).
+// (before the joins and the gradients' kernel were made faster: then 16 612, 20 589, 24 651, 32 674, and 16 180, 20 190, 32 176).
 struct DeltaCut {
   int nseg, per;
 };

@@ -333,8 +333,9 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 }
 
 // Rows with a target >= 0, in order: tc (their targets, −1 for one that is no item), rows (their places), inv (the way
-// back, −1: ignored), count; the losses of ignored rows.  A workgroup lists 1024 rows; with more than one the
-// groups' counts come first.
+// back, −1: ignored), count; the losses of ignored rows.  A workgroup lists 1024 rows; with more than one the groups'
+// counts come first and the packed copy of h (zeros behind column D and behind the last row) after.  Up to 1024 rows
+// each workgroup lists them all and packs its share: two launches less.
 __global__ __launch_bounds__(1024) void k_ce_count(const int64_t* __restrict__ tgt, int64_t st, int N, int* __restrict__ counts) {
   __shared__ int part[16];
   const int r = blockIdx.x * 1024 + threadIdx.x;
@@ -347,17 +348,27 @@ __global__ __launch_bounds__(1024) void k_ce_count(const int64_t* __restrict__ t
     counts[blockIdx.x] = k;
   }
 }
+__device__ __forceinline__ void ce_pack8(const uint16_t* h, int64_t ldh, int D, int DP, int c, int r, int col, uint16_t* hp) {
+  ce_s8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (r >= 0 && col < D) v = *reinterpret_cast<const ce_s8*>(h + r * ldh + col);
+  *reinterpret_cast<ce_s8*>(hp + (int64_t)c * DP + col) = v;
+}
+template <bool PACK>
 __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ tgt, int64_t st, int N, int npad, int V,
                                                   const int* __restrict__ counts, int* __restrict__ count,
                                                   int* __restrict__ rows, int* __restrict__ tc, int* __restrict__ inv,
-                                                  float* __restrict__ loss) {
-  __shared__ int part[16], before[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x * 1024 + tid;
+                                                  float* __restrict__ loss, const uint16_t* __restrict__ h, int64_t ldh,
+                                                  int D, int DP, uint16_t* __restrict__ hp) {
+  __shared__ int part[16], before[16], list[PACK ? 1024 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = (PACK ? 0 : blockIdx.x * 1024) + tid;
   const int64_t t = tgt[r < N ? r * st : 0];
   const bool on = r < N && t >= 0;
   const uint64_t mask = __ballot(on);
   int base = 0;
-  for (int i = tid; i < (int)blockIdx.x; i += 1024) base += counts[i];
+  if constexpr (PACK)
+    list[tid] = -1;
+  else
+    for (int i = tid; i < (int)blockIdx.x; i += 1024) base += counts[i];
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) base += __shfl_xor(base, o);
   if (lane == 0) {
@@ -372,29 +383,31 @@ __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ tg
     if (w < wave) at += part[w];
   }
   at += __popcll(mask & ((1ull << lane) - 1));
-  if (on) {
-    rows[at] = r;
-    tc[at] = t < V ? (int)t : -1;
-    inv[r] = at;
-  } else if (r < N) {
-    inv[r] = -1;
-    loss[r] = 0.f;
+  if (PACK && on) list[at] = r;
+  if (!PACK || blockIdx.x == 0) {
+    if (on) {
+      rows[at] = r;
+      tc[at] = t < V ? (int)t : -1;
+      inv[r] = at;
+    } else if (r < N) {
+      inv[r] = -1;
+      loss[r] = 0.f;
+    }
   }
-  if (blockIdx.x == gridDim.x - 1) {
+  if (blockIdx.x == (PACK ? 0 : gridDim.x - 1)) {
     if (tid == 0) *count = all;
     for (int c = all + tid; c < npad; c += 1024) rows[c] = -1;
   }
+  if constexpr (PACK) {
+    __syncthreads();
+    const int e = blockIdx.x * 1024 + tid, c = e / (DP / 8);
+    if (c < npad) ce_pack8(h, ldh, D, DP, c, list[c], e % (DP / 8) * 8, hp);
+  }
 }
-
-// packed copy of the listed rows, zeros behind column D and behind the last row
 __global__ __launch_bounds__(256) void k_ce_pack(const uint16_t* __restrict__ h, int64_t ldh, int D, int DP, int npad,
                                                  const int* __restrict__ rows, uint16_t* __restrict__ hp) {
-  const int e = blockIdx.x * 256 + threadIdx.x, c = e / (DP / 8), col = (e % (DP / 8)) * 8;
-  if (c >= npad) return;
-  const int r = rows[c];
-  ce_s8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (r >= 0 && col < D) v = *reinterpret_cast<const ce_s8*>(h + r * ldh + col);
-  *reinterpret_cast<ce_s8*>(hp + (int64_t)c * DP + col) = v;
+  const int e = blockIdx.x * 256 + threadIdx.x, c = e / (DP / 8);
+  if (c < npad) ce_pack8(h, ldh, D, DP, c, rows[c], e % (DP / 8) * 8, hp);
 }
 
 // one wave per packed row: lse over the splits, the loss, and (GRAD) dh for g = 1 in fp32
@@ -640,11 +653,19 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
   const CeSaved s = ce_saved(saved, N, D);
   const int groups = (N + 1023) / 1024;
   int* counts = (int*)s.lse;   // not written before the join
-  if (groups > 1) hipLaunchKernelGGL(k_ce_count, dim3(groups), dim3(1024), 0, st, tgt, st_t, N, counts);
-  hipLaunchKernelGGL(k_ce_rows, dim3(groups), dim3(1024), 0, st, tgt, st_t, N, p.npad, V, counts, s.count, s.rows, s.tc,
-                     s.inv, loss);
-  hipLaunchKernelGGL(k_ce_pack, dim3((p.npad * (p.DP / 8) + 255) / 256), dim3(256), 0, st, (const uint16_t*)h, ldh, D,
-                     p.DP, p.npad, s.rows, (uint16_t*)s.hp);
+  const int pieces = p.npad * (p.DP / 8);
+  auto list = [&](auto kern, int grid) {
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(1024), 0, st, tgt, st_t, N, p.npad, V, counts, s.count, s.rows, s.tc, s.inv,
+                       loss, (const uint16_t*)h, ldh, D, p.DP, (uint16_t*)s.hp);
+  };
+  if (groups == 1) {
+    list(k_ce_rows<true>, (pieces + 1023) / 1024);
+  } else {
+    hipLaunchKernelGGL(k_ce_count, dim3(groups), dim3(1024), 0, st, tgt, st_t, N, counts);
+    list(k_ce_rows<false>, groups);
+    hipLaunchKernelGGL(k_ce_pack, dim3((pieces + 255) / 256), dim3(256), 0, st, (const uint16_t*)h, ldh, D, p.DP, p.npad,
+                       s.rows, (uint16_t*)s.hp);
+  }
   RG_LAUNCH_CHECK();
   CeArgs a = {};
   a.X = s.hp, a.ldx = p.DP, a.nx = N, a.Y = W, a.ldy = ldw, a.ny = V, a.D = D, a.count = s.count, a.bias = bias;
