@@ -21,7 +21,7 @@
 //
 // Measured, whole step: 4096 rows x 1M items x 128 bf16 3.42 ms, 1250 TFLOP/s of these 8 N V D (91 % of what a large
 // library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.15 ms, 1090 TFLOP/s;
-// 64 x 10001 x 32 38 us, of which the launches and the waits between its seven kernels are most.
+// 64 x 10001 x 32 34 us, of which the launches and the waits between its five kernels (3 to 8 us each) are most.
 //
 // Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
 // packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
