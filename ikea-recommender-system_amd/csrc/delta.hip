@@ -591,6 +591,9 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
       for (int i = 0; i < 8; ++i)
         go[ct][i >> 2][i & 3] = DlIO<IO>::load1(gbuf, at, (int)((16 * (i >> 2) + (i & 3)) * a.dos[1]) * DlIO<IO>::SIZE);
     }
+    // before the segment's first chunk nobody asks for the state's gradient but dstate0 (8192 sessions x heads
+    // of up to 50 positions: 86 us against 96)
+    const bool on = LOCAL || c > cfrom || (seg == 0 && a.dstate0 != nullptr);
     if (!LOCAL && c < nc - 1) dl_state_store<CT, 2 * KT>(S, a.dS + (bh * (nC - 1) + c) * size, a.Dk, a.Dv, col0);
     dl_fence();
     kt.put(K, lane);
@@ -666,6 +669,7 @@ __global__ __launch_bounds__(64, 2) void k_delta_scan(DeltaArgs a) {
         go[ct][j] *= a.scale * gam;
         dx[j] *= -be * gam;
       }
+      if (!on) continue;
       bf16x8 hb[NP];
       pl_split<NP>(go[ct][0], go[ct][1], hb);
       pl_split<NP>(dx[0], dx[1], xb);
