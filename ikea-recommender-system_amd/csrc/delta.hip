@@ -13,10 +13,11 @@
 // One wave owns 16·CT value columns of one (row, value head) and their part of the state, in accumulators; it makes the
 // chunk's P and T itself and never waits for another wave.  What bounds these kernels is the chain of dependent steps
 // inside a chunk (about 20 products and a triangular solve of 16 steps), not bandwidth or MFMAs: sessions are
-// short, so the answer is many independent waves with little LDS, and each step small.  (Workgroups of four waves with
-// 64-position chunks, K, Q, P and T shared through LDS and a barrier between steps: two workgroups fit a CU, 20 us each;
-// 8192 sessions x heads of width 64 took 320 us forwards.)  A long row is cut into segments whose
-// waves run side by side (below).
+// short, so the answer is many independent waves with little LDS, and each step small.  Forwards, 8192 sessions x
+// heads of up to 50 positions of width 64, bf16: 104 us.  (Workgroups of four waves with 64-position chunks, K, Q, P and T
+// shared through LDS and a barrier between steps, two to a CU: 320 us.  Three waves a SIMD spill: 602 us a
+// training step against 350.  A second copy of the code with half the tiles, for chunks of 16 positions or fewer,
+// spills 19 registers: 120 us.)  A long row is cut into segments whose waves run side by side (below).
 //
 // The state, G and every sum are fp32 or wider (G in fp64: differences of long sums enter an exponential).  Products run
 // on bf16 MFMA with fp32 operands split into three planes (planes.h); bf16 inputs are one exact plane.  Two planes
