@@ -16,7 +16,8 @@
 // start value of size 20 they would cost S its low bits: db was off by 1.5e-6 instead of 1e-7).  That matters because
 // the exponentials, not the MFMAs, take the longer at small D: an element costs a scaling, an exponential (four
 // issue slots), a sum and half a conversion, so there is no running maximum either: forwards the reference only
-// moves when a lane's eight powers sum to more than LIM, which needs one comparison per eight elements.  Per 32
+// moves when a lane's eight powers sum to more than LIM, which needs one comparison per eight elements.  A wave that
+// has met only masked items, or logits beyond CE_FAR, pays one subtraction more an element.  Per 32
 // rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D MFMA flops.
 //
 // Measured, whole step: 4096 rows x 1M items x 128 bf16 3.42 ms, 1250 TFLOP/s of these 8 N V D (91 % of what a large
@@ -40,7 +41,8 @@ typedef short ce_s8 __attribute__((ext_vector_type(8)));
 #define CE_PAD 512         // packed rows are allocated in multiples of this
 #define CE_L2E 1.4426950408889634f
 #define CE_LN2 0.6931471805599453f
-#define CE_LOW (-3.0e38f)  // the running reference before any logit
+#define CE_LOW (-2.0e38f)  // the running reference before any logit
+#define CE_FAR 32768.f     // references beyond it: exponents from differences of logits
 
 template <typename T>
 struct CeT;
@@ -59,6 +61,21 @@ struct CeT<_Float16> {
   }
 };
 
+// Powers are 2^(z log2 e + base) with a base per reference, one fused operation an element.  The base is rounded to half a
+// unit of its last place, which moves all powers of the reference alike and drops out as long as everything that meets
+// them uses the same base; but beyond CE_FAR that half unit grows (64 at a logit of 1e9) until the powers leave fp32's range
+// on either side, and there they are 2^((z - m) log2 e), whose difference is exact where it matters.
+template <typename T>
+__device__ __forceinline__ float ce_base(float m) {
+  return __builtin_fmaf(-m, CE_L2E, CeT<T>::OFF);
+}
+__device__ __forceinline__ bool ce_near(float m) { return fabsf(m) <= CE_FAR; }
+// what sums taken with the reference m count beside sums with the reference top >= m
+template <typename T>
+__device__ __forceinline__ float ce_weight(float m, float top) {
+  return __builtin_amdgcn_exp2f(ce_near(m) && ce_near(top) ? ce_base<T>(top) - ce_base<T>(m) : (m - top) * CE_L2E);
+}
+
 struct CeArgs {
   const void *X, *Y;
   int64_t ldx, ldy;        // row strides in elements
@@ -66,7 +83,7 @@ struct CeArgs {
   int D;                   // columns of W's rows (h's packed copy has DP, zeros behind D)
   const int* count;        // packed rows
   const float* bias;       // (V) or null
-  const float* recs;       // backward: [chunk][3][64] log2 |g| − lse · log2 e, g, target (as int bits)
+  const float* recs;       // backward: [chunk][4][64], see k_ce_dh
   int nsplit, nblock, block0;   // blocks of X: nblock of them, from block0 on
   float *pm, *pl, *pO;     // forward: [split][row], [split][row][DP]; backward: pO slabs [split][items from block0 on][D], pl likewise
   void* dW;
@@ -90,7 +107,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
   constexpr bool REMAKE = DP == 256 && NX > 1;
   static_assert(LOADS >= 1, "a chunk is at least one load a wave");
   __shared__ __attribute__((aligned(16))) uint8_t y0[CE_CH * RB], y1[CE_CH * RB];
-  __shared__ __attribute__((aligned(16))) float r0[3 * CE_CH], r1[3 * CE_CH];
+  __shared__ __attribute__((aligned(16))) float r0[4 * CE_CH], r1[4 * CE_CH];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // neighbouring blocks of one split run on one XCD (workgroups go round the 8 XCDs) and share its L2
@@ -132,9 +149,9 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
                                                           nb < 0 ? 0 : nb, 0x00020000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)r, 4, lane * 4, 0, 0, 0);
       } else {
-        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.recs) + at * 3, 0,
-                                                          left > 0 ? 3 * CE_CH * 4 : 0, 0x00020000);
-        if (lane < 48) rg_blds16(rb, r, 16 * lane, 0);
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.recs) + at * 4, 0,
+                                                          left > 0 ? 4 * CE_CH * 4 : 0, 0x00020000);
+        rg_blds16(rb, r, 16 * lane, 0);
       }
     }
   };
@@ -142,6 +159,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 
   V xf[NX][KS];
   float ref[NX], sum[NX], xb[NX];
+  bool away = true;   // a reference of this wave lies beyond CE_FAR
   const T* X = (const T*)a.X;
   const int xcols = FWD ? DP : a.D;
 #pragma unroll
@@ -165,11 +183,12 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
 
   auto work = [&](int c, uint8_t* y, const float* r) __attribute__((always_inline)) {
     // backward: a target of this chunk among this wave's items; a negative g among this chunk's rows
-    bool mine = false, sign = false;
+    bool mine = false, sign = false, far = false;
     if constexpr (!FWD) {
       const int t = __float_as_int(r[2 * CE_CH + lane]) - x0;
       mine = __any(t >= 0 && t < 16 * NX);
       sign = __any(r[CE_CH + lane] < 0.f);
+      far = __any(r[3 * CE_CH + lane] != 0.f);
     }
     const bool tail = FWD && c * CE_CH + CE_CH > ny;
 #pragma unroll
@@ -206,9 +225,15 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
           bool up = false;
 #pragma unroll
           for (int t = 0; t < NX; ++t) {
-            const float b = CeT<T>::OFF - ref[t];
+            if (away) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
+              for (int i = 0; i < 8; ++i)
+                p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3] - ref[t], CE_L2E, CeT<T>::OFF));
+            } else {
+              const float b = ce_base<T>(ref[t]);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
+            }
             add[t] = ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
             up |= !(add[t] <= CeT<T>::LIM);
           }
@@ -221,13 +246,17 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
                             fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
-            const float now = fmaxf(ref[t], m * CE_L2E), fac = __builtin_amdgcn_exp2f(ref[t] - now);
+            const float now = fmaxf(ref[t], m), fac = ce_weight<T>(ref[t], now);
             ref[t] = now;
             sum[t] *= fac;
 #pragma unroll
             for (int f = 0; f < FB; ++f) O[f][t] *= fac;
           }
-          powers();
+          bool beyond = false;
+#pragma unroll
+          for (int t = 0; t < NX; ++t) beyond |= !ce_near(ref[t]);
+          away = __any(beyond);
+          powers();   // no power is above 2^OFF by more than ce_base's rounding now
         }
 #pragma unroll
         for (int t = 0; t < NX; ++t) {
@@ -239,6 +268,12 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
         f4 e[2];   // log2(|g| / Σ exp) of this lane's rows
 #pragma unroll
         for (int j = 0; j < 2; ++j) e[j] = *reinterpret_cast<const f4*>(r + at + 16 * j);
+        if (far) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int t = 0; t < NX; ++t) S[j][t] -= *reinterpret_cast<const f4*>(r + 3 * CE_CH + at + 16 * j);
+        }
         float p[NX][8];
 #pragma unroll
         for (int t = 0; t < NX; ++t)
@@ -410,7 +445,8 @@ __global__ __launch_bounds__(256) void k_ce_pack(const uint16_t* __restrict__ h,
   if (c < npad) ce_pack8(h, ldh, D, DP, c, rows[c], e % (DP / 8) * 8, hp);
 }
 
-// one wave per packed row: lse over the splits, the loss, and (GRAD) dh for g = 1 in fp32
+// One wave per packed row: the splits' sums joined, the loss, and (GRAD) dh for g = 1 in fp32.  For the backward pass the
+// row's log-sum-exp: `lse` in base 2, or, where it lies beyond CE_FAR, `top` the largest reference and `lse` what is added to it.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, const float* __restrict__ pl,
                                                  const float* __restrict__ pO, int nsplit, int N, int D, int DP,
@@ -418,7 +454,7 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
                                                  const float* __restrict__ bias, const int* __restrict__ count,
                                                  const int* __restrict__ rows, const int* __restrict__ tc,
                                                  float* __restrict__ loss, float* __restrict__ lse,
-                                                 float* __restrict__ dh) {
+                                                 float* __restrict__ top, float* __restrict__ dh) {
   const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (c >= *count) return;
   float m = CE_LOW;
@@ -427,7 +463,7 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
   float l = 0.f;
   for (int s = lane; s < nsplit; s += 64)
-    l += pl[(int64_t)s * N + c] * __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m);
+    l += pl[(int64_t)s * N + c] * ce_weight<T>(pm[(int64_t)s * N + c], m);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
   const int t = tc[c];
@@ -437,10 +473,13 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) z += __shfl_xor(z, o);
   // a target that is no item: NaN in the loss and, through lse, in the gradients
-  const float all = t < 0 ? __builtin_nanf("") : CE_LN2 * (m - CeT<T>::OFF + __log2f(l));
+  const bool near = ce_near(m);
+  const float low = t < 0 ? __builtin_nanf("") : __log2f(l) - (near ? ce_base<T>(m) : CeT<T>::OFF);
   if (lane == 0) {
-    loss[rows[c]] = all - (z + (bias != nullptr && t >= 0 ? bias[t] : 0.f));
-    lse[c] = all;
+    z += bias != nullptr && t >= 0 ? bias[t] : 0.f;
+    loss[rows[c]] = near ? CE_LN2 * low - z : (m - z) + CE_LN2 * low;
+    lse[c] = low;
+    top[c] = near ? 0.f : m;
   }
   if constexpr (GRAD) {
     // DP / 4 lanes per split, several splits at once
@@ -449,7 +488,7 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
     f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = lane / per; s < nsplit; s += 64 / per)
-      o += *reinterpret_cast<const f4*>(pO + ((int64_t)s * N + c) * DP + f) * __builtin_amdgcn_exp2f(pm[(int64_t)s * N + c] - m);
+      o += *reinterpret_cast<const f4*>(pO + ((int64_t)s * N + c) * DP + f) * ce_weight<T>(pm[(int64_t)s * N + c], m);
     for (int x = per; x < 64; x <<= 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
@@ -478,12 +517,14 @@ __global__ __launch_bounds__(1024) void k_ce_largest(const float* __restrict__ g
   }
 }
 
-// dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows, and the
-// factor that their scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
+// dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows (four
+// values: log2 |g| − lse in base 2, the scaled g, its target as int bits, and what the logits are taken from first, not 0
+// only beyond CE_FAR), and the factor that the scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
                                                const int* __restrict__ count, const int* __restrict__ tc,
-                                               const float* __restrict__ lse, const float* __restrict__ dh0, int N,
+                                               const float* __restrict__ lse, const float* __restrict__ far,
+                                               const float* __restrict__ dh0, int N,
                                                int npad, int D, const float* __restrict__ largest, T* __restrict__ dh,
                                                float* __restrict__ recs, float* __restrict__ scale) {
   const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -498,10 +539,11 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
   top = top < __builtin_inff() ? fmaxf(top, 0x1p-100f) : 1.f;
   if (r == 0 && lane == 0) *scale = top * 0x1p-13f;
   if (lane == 0 && r >= *count) {   // behind the last packed row
-    float* rec = recs + (int64_t)(r / CE_CH) * 3 * CE_CH + r % CE_CH;
+    float* rec = recs + (int64_t)(r / CE_CH) * 4 * CE_CH + r % CE_CH;
     rec[0] = -__builtin_inff();
     rec[CE_CH] = 0.f;
     rec[2 * CE_CH] = __int_as_float(-1);
+    rec[3 * CE_CH] = 0.f;
   }
   if (r >= N) return;
   const int c = inv[r];
@@ -512,11 +554,12 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
     *reinterpret_cast<T4*>(dh + (int64_t)r * D + f) = __builtin_convertvector(v, T4);
   }
   if (lane == 0 && c >= 0) {
-    float* rec = recs + (int64_t)(c / CE_CH) * 3 * CE_CH + c % CE_CH;
+    float* rec = recs + (int64_t)(c / CE_CH) * 4 * CE_CH + c % CE_CH;
     const float w = gr / top * 0x1p13f;
-    rec[0] = __log2f(fabsf(w)) - lse[c] * CE_L2E;
+    rec[0] = __log2f(fabsf(w)) - lse[c];
     rec[CE_CH] = w;
     rec[2 * CE_CH] = __int_as_float(tc[c]);
+    rec[3 * CE_CH] = far[c];
   }
 }
 
@@ -603,18 +646,18 @@ extern "C" int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass) {
   if (pass == 0) return 2 * (int64_t)p.fsplits * N + 64;
   if (pass == 1) return 2 * (int64_t)p.fsplits * N + 64 + (int64_t)p.fsplits * N * p.DP;
   const int64_t slabs = p.bsplits > 1 ? p.bsplits * p.items * (D + 1) + 64 : 0, groups = (N + 1023) / 1024;
-  return 64 + 3 * (int64_t)p.npad + (slabs > groups ? slabs : groups);
+  return 64 + 4 * (int64_t)p.npad + (slabs > groups ? slabs : groups);
 }
-// what the backward pass needs of the forward (bytes): packed h, lists, lse, dh for g = 1
+// what the backward pass needs of the forward (bytes): packed h, lists, lse (two values), dh for g = 1
 extern "C" int64_t rg_linear_ce_saved_bytes(int N, int V, int D) {
   if (ce_check(N, V, D, 1) != RG_OK) return 0;
   const int64_t npad = ce_up(N, CE_PAD);
-  return 256 + npad * (ce_dp(D) * 2 + 4 * 4) + (int64_t)N * D * 4;
+  return 256 + npad * (ce_dp(D) * 2 + 5 * 4) + (int64_t)N * D * 4;
 }
 struct CeSaved {
   void* hp;
   int *count, *rows, *tc, *inv;
-  float *lse, *dh0;
+  float *lse, *top, *dh0;
 };
 static CeSaved ce_saved(void* base, int N, int D) {
   const int64_t npad = ce_up(N, CE_PAD);
@@ -628,7 +671,8 @@ static CeSaved ce_saved(void* base, int N, int D) {
   s.tc = s.rows + npad;
   s.inv = s.tc + npad;
   s.lse = (float*)(s.inv + npad);
-  s.dh0 = s.lse + npad;
+  s.top = s.lse + npad;
+  s.dh0 = s.top + npad;
   return s;
 }
 
@@ -676,7 +720,7 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
   if (rc != RG_OK) return rc;
   auto join = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((N + 3) / 4), dim3(256), 0, st, a.pm, a.pl, a.pO, p.fsplits, N, D, p.DP,
-                       (const T*)s.hp, (const T*)W, ldw, bias, s.count, s.rows, s.tc, loss, s.lse, s.dh0);
+                       (const T*)s.hp, (const T*)W, ldw, bias, s.count, s.rows, s.tc, loss, s.lse, s.top, s.dh0);
   };
   if (grad)
     join(k_ce_join<T, true>);
@@ -692,9 +736,9 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
   const CePlan p = ce_plan(N, V, D);
   const CeSaved s = ce_saved(const_cast<void*>(saved), N, D);
   const int groups = (N + 1023) / 1024;
-  float *scale = work, *recs = work + 64, *largest = groups > 1 ? recs + 3 * (int64_t)p.npad : nullptr;
+  float *scale = work, *recs = work + 64, *largest = groups > 1 ? recs + 4 * (int64_t)p.npad : nullptr;
   if (groups > 1) hipLaunchKernelGGL(k_ce_largest, dim3(groups), dim3(1024), 0, st, g, sg, s.inv, N, largest);
-  hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.dh0, N,
+  hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.top, s.dh0, N,
                      p.npad, D, largest, (T*)dh, recs, scale);
   RG_LAUNCH_CHECK();
   CeArgs a = {};
@@ -710,7 +754,7 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
   }
   if (p.brest > 0) {
     a.nsplit = p.bsplits, a.nblock = p.brest, a.block0 = p.bwhole;
-    a.pO = recs + 3 * (int64_t)p.npad, a.pl = a.pO + ce_up(p.bsplits * p.items * D, 64);
+    a.pO = recs + 4 * (int64_t)p.npad, a.pl = a.pO + ce_up(p.bsplits * p.items * D, 64);
     const int rc = pass();
     if (rc != RG_OK) return rc;
   }
