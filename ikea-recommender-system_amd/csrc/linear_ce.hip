@@ -6,10 +6,13 @@
 // N x V logits kept).  A workgroup holds a block of one matrix ("X") in registers and streams the other ("Y") through
 // LDS in chunks of 64 rows:
 //     S = Y_c Xᵀ (MFMA),   P = f(S) rounded to the inputs' type,   Oᵀ += Y_cᵀ P (MFMA)
-//   forward   X = rows of h, Y = W: f = 2^(z − m) with a reference m of the row; O = Σ_v 2^(z − m) W_v and the sum of P per
-//             row and split of the vocabulary; joined by k_ce_join, which takes W[t] off in fp32 (a one-hot inside P
-//             would be rounded with it).
-//   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r); O = dW, and Σ_r P = db from the unrounded P.
+//   forward   X = rows of h, Y = W: f = 2^(z − m) with a reference m of the row, 0 at the row's target; O = Σ_v 2^(z − m) W_v
+//             and the sum of P per row and split of the vocabulary.  k_ce_join takes the target's logit in fp32 and has the
+//             odds q against it, loss = log(1 + q), and dh = (Σ_{v ≠ t} p_v W_v) − (1 − p_t) W_t with 1 − p_t = q / (1 + q):
+//             where a row is predicted well both are small, and neither is a difference of large rounded values (with
+//             the target inside P, dh was off by 0.4 % of |W_t| there, a third of itself at p_t = 0.996).
+//   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r), and −g_r (1 − p_t) at the row's target; O = dW, and
+//             Σ_r P = db from the unrounded P.
 // The accumulator of S (16 rows of Y x 16 of X per tile; lane (kg, n) holds rows 4·kg + i of column n) is already the B
 // operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  The biases are
 // S's start value and cost no instruction an element; backwards −lse and log2 |g| enter with the exponent's scaling (as a
@@ -79,6 +82,7 @@ __device__ __forceinline__ float ce_weight(float m, float top) {
 struct CeArgs {
   const void *X, *Y;
   int64_t ldx, ldy;        // row strides in elements
+  const int* tc;           // forward: targets of the packed rows
   int nx, ny;              // rows (host bounds)
   int D;                   // columns of W's rows (h's packed copy has DP, zeros behind D)
   const int* count;        // packed rows
@@ -108,6 +112,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
   static_assert(LOADS >= 1, "a chunk is at least one load a wave");
   __shared__ __attribute__((aligned(16))) uint8_t y0[CE_CH * RB], y1[CE_CH * RB];
   __shared__ __attribute__((aligned(16))) float r0[4 * CE_CH], r1[4 * CE_CH];
+  __shared__ int target[FWD ? 16 * NX * NW : 1];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // neighbouring blocks of one split run on one XCD (workgroups go round the 8 XCDs) and share its L2
@@ -173,6 +178,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     ref[t] = CE_LOW;
     sum[t] = 0.f;
     xb[t] = BIAS && x < nx ? a.bias[x] : 0.f;
+    if (FWD && kg == 0) target[wave * 16 * NX + 16 * t + n] = x < nx ? a.tc[x] : -1;
   }
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   f4 O[FB][NX];
@@ -182,12 +188,17 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     for (int t = 0; t < NX; ++t) O[f][t] = zero;
 
   auto work = [&](int c, uint8_t* y, const float* r) __attribute__((always_inline)) {
-    // backward: a target of this chunk among this wave's items; a negative g among this chunk's rows
+    // a target of this wave's rows among the chunk's items, or backwards one of the chunk's rows among this wave's items;
+    // a negative g among the chunk's rows, and one whose logits lie beyond CE_FAR
     bool mine = false, sign = false, far = false;
-    if constexpr (!FWD) {
+    if constexpr (FWD) {
+#pragma unroll
+      for (int t = 0; t < NX; ++t) mine |= (unsigned)(target[wave * 16 * NX + 16 * t + n] - c * CE_CH) < CE_CH;
+      mine = __any(mine);
+    } else {
       const int t = __float_as_int(r[2 * CE_CH + lane]) - x0;
       mine = __any(t >= 0 && t < 16 * NX);
-      sign = __any(r[CE_CH + lane] < 0.f);
+      sign = __any(!__builtin_signbitf(r[CE_CH + lane]));
       far = __any(r[3 * CE_CH + lane] != 0.f);
     }
     const bool tail = FWD && c * CE_CH + CE_CH > ny;
@@ -219,6 +230,15 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
             if (c * CE_CH + at + 16 * (i >> 2) + (i & 3) >= ny)
 #pragma unroll
               for (int t = 0; t < NX; ++t) S[i >> 2][t][i & 3] = -__builtin_inff();
+        }
+        if (mine) {
+#pragma unroll
+          for (int t = 0; t < NX; ++t) {
+            const int place = target[wave * 16 * NX + 16 * t + n] - c * CE_CH - at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (place == 16 * (i >> 2) + (i & 3)) S[i >> 2][t][i & 3] = -__builtin_inff();
+          }
         }
         float p[NX][8], add[NX];
         auto powers = [&]() __attribute__((always_inline)) {
@@ -283,12 +303,12 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
         if (mine || sign) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float g = r[CE_CH + at + 16 * (i >> 2) + (i & 3)];
+            const float share = r[CE_CH + at + 16 * (i >> 2) + (i & 3)];
             const int tg = __float_as_int(r[2 * CE_CH + at + 16 * (i >> 2) + (i & 3)]);
 #pragma unroll
             for (int t = 0; t < NX; ++t) {
-              if (g < 0.f) p[t][i] = -p[t][i];
-              if (tg == x0 + 16 * t + n) p[t][i] -= g;
+              if (!__builtin_signbitf(share)) p[t][i] = -p[t][i];
+              if (tg == x0 + 16 * t + n) p[t][i] = share;
             }
           }
         }
@@ -445,8 +465,10 @@ __global__ __launch_bounds__(256) void k_ce_pack(const uint16_t* __restrict__ h,
   if (c < npad) ce_pack8(h, ldh, D, DP, c, rows[c], e % (DP / 8) * 8, hp);
 }
 
-// One wave per packed row: the splits' sums joined, the loss, and (GRAD) dh for g = 1 in fp32.  For the backward pass the
-// row's log-sum-exp: `lse` in base 2, or, where it lies beyond CE_FAR, `top` the largest reference and `lse` what is added to it.
+// One wave per packed row: the splits' sums (without the target) and the target's logit joined.  With the odds q against the
+// target, as x = log2 q: loss = log(1 + q), and (GRAD) dh for g = 1 in fp32, with the target's share 1 − p_t = q / (1 + q).  For
+// the backward pass the row's log-sum-exp: `lse` in base 2, or, where it lies beyond CE_FAR, `top` the largest logit and
+// `lse` what is added to it.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, const float* __restrict__ pl,
                                                  const float* __restrict__ pO, int nsplit, int N, int D, int DP,
@@ -454,7 +476,8 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
                                                  const float* __restrict__ bias, const int* __restrict__ count,
                                                  const int* __restrict__ rows, const int* __restrict__ tc,
                                                  float* __restrict__ loss, float* __restrict__ lse,
-                                                 float* __restrict__ top, float* __restrict__ dh) {
+                                                 float* __restrict__ top, float* __restrict__ against,
+                                                 float* __restrict__ dh) {
   const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (c >= *count) return;
   float m = CE_LOW;
@@ -472,18 +495,24 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
   for (int f = lane; f < D; f += 64) z = __builtin_fmaf((float)hp[(int64_t)c * DP + f], (float)w[f], z);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) z += __shfl_xor(z, o);
-  // a target that is no item: NaN in the loss and, through lse, in the gradients
+  if (bias != nullptr && t >= 0) z += bias[t];
+  // a target that is no item: NaN in the loss and, through lse, in the gradients; so does an infinite logit of the target
+  if (t < 0 || z == __builtin_inff()) z = __builtin_nanf("");
   const bool near = ce_near(m);
-  const float low = t < 0 ? __builtin_nanf("") : __log2f(l) - (near ? ce_base<T>(m) : CeT<T>::OFF);
+  const float rest = __log2f(l) - (near ? ce_base<T>(m) : CeT<T>::OFF);   // of the others, to the base of m
+  const float x = near ? __builtin_fmaf(-z, CE_L2E, rest) : __builtin_fmaf(m - z, CE_L2E, rest);
+  const float e = __builtin_amdgcn_exp2f(-fabsf(x)), share = (x >= 0.f ? 1.f : e) / (1.f + e);
   if (lane == 0) {
-    z += bias != nullptr && t >= 0 ? bias[t] : 0.f;
-    loss[rows[c]] = near ? CE_LN2 * low - z : (m - z) + CE_LN2 * low;
-    lse[c] = low;
-    top[c] = near ? 0.f : m;
+    const bool own = !(x >= 0.f);   // the target's logit is the larger part of the sum
+    const float big = own ? z : m;
+    loss[rows[c]] = __builtin_fmaf(own ? 0.f : x, CE_LN2, log1pf(e));
+    lse[c] = (own ? ce_near(z) ? z * CE_L2E : 0.f : rest) + __log2f(1.f + e);
+    top[c] = ce_near(big) ? 0.f : big;
+    against[c] = share;
   }
   if constexpr (GRAD) {
     // DP / 4 lanes per split, several splits at once
-    const float one = 1.f / l;
+    const float one = l != 0.f ? share / l : 0.f;
     const int per = DP / 4, f = lane % per * 4;
     f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -495,7 +524,7 @@ __global__ __launch_bounds__(256) void k_ce_join(const float* __restrict__ pm, c
     if (lane < per && f < D) {
       f4 d;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = t < 0 ? __builtin_nanf("") : __builtin_fmaf(o[i], one, -(float)w[f + i]);
+      for (int i = 0; i < 4; ++i) d[i] = t < 0 ? __builtin_nanf("") : __builtin_fmaf(o[i], one, -share * (float)w[f + i]);
       *reinterpret_cast<f4*>(dh + (int64_t)c * D + f) = d;
     }
   }
@@ -518,13 +547,13 @@ __global__ __launch_bounds__(1024) void k_ce_largest(const float* __restrict__ g
 }
 
 // dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows (four
-// values: log2 |g| − lse in base 2, the scaled g, its target as int bits, and what the logits are taken from first, not 0
-// only beyond CE_FAR), and the factor that the scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
+// values: log2 |g| − lse in base 2; the target's −g (1 − p_t), whose sign bit is clear where g is negative; the target as
+// int bits; and what is taken off the logits first, not 0 only beyond CE_FAR), and the factor that the scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
                                                const int* __restrict__ count, const int* __restrict__ tc,
                                                const float* __restrict__ lse, const float* __restrict__ far,
-                                               const float* __restrict__ dh0, int N,
+                                               const float* __restrict__ against, const float* __restrict__ dh0, int N,
                                                int npad, int D, const float* __restrict__ largest, T* __restrict__ dh,
                                                float* __restrict__ recs, float* __restrict__ scale) {
   const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -541,7 +570,7 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
   if (lane == 0 && r >= *count) {   // behind the last packed row
     float* rec = recs + (int64_t)(r / CE_CH) * 4 * CE_CH + r % CE_CH;
     rec[0] = -__builtin_inff();
-    rec[CE_CH] = 0.f;
+    rec[CE_CH] = -0.f;
     rec[2 * CE_CH] = __int_as_float(-1);
     rec[3 * CE_CH] = 0.f;
   }
@@ -557,7 +586,7 @@ __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int6
     float* rec = recs + (int64_t)(c / CE_CH) * 4 * CE_CH + c % CE_CH;
     const float w = gr / top * 0x1p13f;
     rec[0] = __log2f(fabsf(w)) - lse[c];
-    rec[CE_CH] = w;
+    rec[CE_CH] = -w * against[c];
     rec[2 * CE_CH] = __int_as_float(tc[c]);
     rec[3 * CE_CH] = far[c];
   }
@@ -648,16 +677,16 @@ extern "C" int64_t rg_linear_ce_work_floats(int N, int V, int D, int pass) {
   const int64_t slabs = p.bsplits > 1 ? p.bsplits * p.items * (D + 1) + 64 : 0, groups = (N + 1023) / 1024;
   return 64 + 4 * (int64_t)p.npad + (slabs > groups ? slabs : groups);
 }
-// what the backward pass needs of the forward (bytes): packed h, lists, lse (two values), dh for g = 1
+// what the backward pass needs of the forward (bytes): packed h, lists, lse (two values), 1 − p_t, dh for g = 1
 extern "C" int64_t rg_linear_ce_saved_bytes(int N, int V, int D) {
   if (ce_check(N, V, D, 1) != RG_OK) return 0;
   const int64_t npad = ce_up(N, CE_PAD);
-  return 256 + npad * (ce_dp(D) * 2 + 5 * 4) + (int64_t)N * D * 4;
+  return 256 + npad * (ce_dp(D) * 2 + 6 * 4) + (int64_t)N * D * 4;
 }
 struct CeSaved {
   void* hp;
   int *count, *rows, *tc, *inv;
-  float *lse, *top, *dh0;
+  float *lse, *top, *against, *dh0;
 };
 static CeSaved ce_saved(void* base, int N, int D) {
   const int64_t npad = ce_up(N, CE_PAD);
@@ -672,7 +701,8 @@ static CeSaved ce_saved(void* base, int N, int D) {
   s.inv = s.tc + npad;
   s.lse = (float*)(s.inv + npad);
   s.top = s.lse + npad;
-  s.dh0 = s.top + npad;
+  s.against = s.top + npad;
+  s.dh0 = s.against + npad;
   return s;
 }
 
@@ -712,7 +742,7 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
   }
   RG_LAUNCH_CHECK();
   CeArgs a = {};
-  a.X = s.hp, a.ldx = p.DP, a.nx = N, a.Y = W, a.ldy = ldw, a.ny = V, a.D = D, a.count = s.count, a.bias = bias;
+  a.X = s.hp, a.ldx = p.DP, a.nx = N, a.Y = W, a.ldy = ldw, a.ny = V, a.D = D, a.count = s.count, a.bias = bias, a.tc = s.tc;
   a.nsplit = p.fsplits, a.nblock = p.fblocks;
   a.pm = work, a.pl = work + (int64_t)p.fsplits * N;
   a.pO = work + ce_up(2 * (int64_t)p.fsplits * N, 64);
@@ -720,7 +750,7 @@ static int ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const 
   if (rc != RG_OK) return rc;
   auto join = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((N + 3) / 4), dim3(256), 0, st, a.pm, a.pl, a.pO, p.fsplits, N, D, p.DP,
-                       (const T*)s.hp, (const T*)W, ldw, bias, s.count, s.rows, s.tc, loss, s.lse, s.top, s.dh0);
+                       (const T*)s.hp, (const T*)W, ldw, bias, s.count, s.rows, s.tc, loss, s.lse, s.top, s.against, s.dh0);
   };
   if (grad)
     join(k_ce_join<T, true>);
@@ -738,7 +768,7 @@ static int ce_bwd(const void* W, int64_t ldw, const float* bias, const float* g,
   const int groups = (N + 1023) / 1024;
   float *scale = work, *recs = work + 64, *largest = groups > 1 ? recs + 4 * (int64_t)p.npad : nullptr;
   if (groups > 1) hipLaunchKernelGGL(k_ce_largest, dim3(groups), dim3(1024), 0, st, g, sg, s.inv, N, largest);
-  hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.top, s.dh0, N,
+  hipLaunchKernelGGL(k_ce_dh<T>, dim3((p.npad + 3) / 4), dim3(256), 0, st, g, sg, s.inv, s.count, s.tc, s.lse, s.top, s.against, s.dh0, N,
                      p.npad, D, largest, (T*)dh, recs, scale);
   RG_LAUNCH_CHECK();
   CeArgs a = {};
