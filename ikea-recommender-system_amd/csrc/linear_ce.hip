@@ -12,7 +12,11 @@
 //             where a row is predicted well both are small, and neither is a difference of large rounded values (with
 //             the target inside P, dh was off by 0.4 % of |W_t| there, a third of itself at p_t = 0.996).
 //   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r), and −g_r (1 − p_t) at the row's target; O = dW, and
-//             Σ_r P = db from the unrounded P.
+//             Σ_r P = db from the unrounded P.  A target's share is most of a target item's gradient; rounded to the type it
+//             moved that by as much as the output's own rounding again (0.2 beside 1.0, clicks beside purchases: every
+//             click's share by 1e-3 the same way).  So what the rounding leaves off follows behind the last chunk, for the
+//             N rows of a whole pass alone: a wave remembers in which chunks it met targets of its items, lists those
+//             rows, and takes 32 of them for one more product; a popular item's rows are shared among the workgroup's waves.
 // The accumulator of S (16 rows of Y x 16 of X per tile; lane (kg, n) holds rows 4·kg + i of column n) is already the B
 // operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  The biases are
 // S's start value and cost no instruction an element; backwards −lse and log2 |g| enter with the exponent's scaling (as a
@@ -37,6 +41,7 @@
 #include "common.h"
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t ce_u2 __attribute__((ext_vector_type(2)));
 typedef short ce_s4 __attribute__((ext_vector_type(4)));
 typedef short ce_s8 __attribute__((ext_vector_type(8)));
 
@@ -103,7 +108,7 @@ __device__ __forceinline__ int ce_swz(int r) {
 
 // FWD: forward pass (else backward); GRAD: with the second product; BIAS: backward with biases
 template <typename T, int DP, int NX, int NW, bool FWD, bool GRAD, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
+__global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a) {
   typedef typename CeT<T>::V V;
   constexpr int KS = DP / 32, RB = DP * 2, FB = GRAD ? DP / 16 : 1;
   constexpr int LOADS = CE_CH * RB / (NW * 1024);
@@ -165,6 +170,9 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
   V xf[NX][KS];
   float ref[NX], sum[NX], xb[NX];
   bool away = true;   // a reference of this wave lies beyond CE_FAR
+  uint64_t met = 0;   // backward: a bit for each 2^fold chunks with targets among this wave's items
+  int fold = 2;
+  while (c1 - c0 > 64 << fold) ++fold;
   const T* X = (const T*)a.X;
   const int xcols = FWD ? DP : a.D;
 #pragma unroll
@@ -198,6 +206,7 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
     } else {
       const int t = __float_as_int(r[2 * CE_CH + lane]) - x0;
       mine = __any(t >= 0 && t < 16 * NX);
+      if (mine) met |= 1ull << ((c - c0) >> fold);
       sign = __any(!__builtin_signbitf(r[CE_CH + lane]));
       far = __any(r[3 * CE_CH + lane] != 0.f);
     }
@@ -347,6 +356,195 @@ __global__ __launch_bounds__(64 * NW) void k_ce_pass(CeArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       work(c + 1, y1, r1);
       __syncthreads();
+    }
+  }
+
+  if constexpr (!FWD) {   // what rounding left off the targets' shares
+    // each wave's rows with targets among its items, as item << 24 | row: as many as there is room for, the others are in
+    // the chunks from `resume` on.  Four chunks are looked through at once, four rows a lane.
+    constexpr int LIST = DP == 64 ? 640 : 1024;   // (two workgroups a CU at 64 columns, one at more)
+    static_assert(16 * NX <= 256, "");
+    __shared__ uint32_t list[NW][LIST];
+    __shared__ float left_off[NW][LIST];
+    __shared__ int have_of[NW], resume_of[NW];
+    auto next = [&](int c) {   // the first of the chunks c, c + 4, .. that may have some, or one behind the last
+      const int group = (c - c0) >> fold;
+      const uint64_t rest = c < c1 ? met >> group : 0;
+      return rest == 0 ? c1 : rest & 1 ? c : c0 + ((group + __builtin_ctzll(rest)) << fold);
+    };
+    int have = 0, resume = next(c0);
+    auto fill = [&]() __attribute__((always_inline)) {
+      have = 0;
+      for (bool room = true; resume < c1 && room;) {
+        constexpr int AHEAD = DP == 64 ? 2 : 4;
+        int c[AHEAD];
+        f4 share[AHEAD], target[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          c[i] = i == 0 ? resume : next(c[i - 1] + 4);
+          const float* rec = a.recs + (int64_t)min(c[i] + kg, c1 - 1) * 4 * CE_CH + 4 * n;
+          share[i] = *reinterpret_cast<const f4*>(rec + CE_CH);
+          target[i] = *reinterpret_cast<const f4*>(rec + 2 * CE_CH);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          uint64_t mask[4];
+          int more = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = __float_as_int(target[i][e]) - x0;
+            mask[e] = __ballot(c[i] + kg < c1 && at >= 0 && at < 16 * NX);
+            more += __popcll(mask[e]);
+          }
+          room = room && have + more <= LIST;
+          if (!room) continue;
+          if (more > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int place = have + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask[e] >> 32),
+                                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)mask[e], 0));
+              if (mask[e] >> lane & 1) {
+                list[wave][place] = (uint32_t)(__float_as_int(target[i][e]) - x0) << 24 |
+                                    (uint32_t)((c[i] + kg) * CE_CH + 4 * n + e);
+                left_off[wave][place] = share[i][e] - (float)(T)share[i][e];
+              }
+              have += __popcll(mask[e]);
+            }
+          }
+          resume = next(c[i] + 4);
+        }
+      }
+      if (lane == 0) {
+        have_of[wave] = have;
+        resume_of[wave] = resume;
+      }
+    };
+    auto entries = [&](uint32_t* e, int w, int first, int count) __attribute__((always_inline)) {   // 32 of wave w's list
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = first + 8 * kg + j;
+        e[j] = list[w][at < count ? at : 0];
+      }
+    };
+    auto shares = [&](V* P, const uint32_t* e, int w, int first, int count) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = first + 8 * kg + j;
+        const T rest = (T)(at < count ? left_off[w][at] : 0.f);
+#pragma unroll
+        for (int t = 0; t < NX; ++t) P[t][j] = e[j] >> 24 == 16 * t + n ? rest : (T)0.f;
+      }
+    };
+    auto columns = [&](uint32_t* v, const uint32_t* e, int f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = reinterpret_cast<const uint16_t*>(Y)[(int64_t)(e[j] & 0xffffff) * DP + 16 * f + n];
+    };
+    auto pack = [](const uint32_t* v) __attribute__((always_inline)) {
+      typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+      const u4 w = {v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+      return __builtin_bit_cast(V, w);
+    };
+    fill();
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += have_of[w];
+    // a long list that is a good part of the workgroup's is shared: each wave takes 64 of the columns and some of the rows.  A
+    // lane loads four neighbouring columns, so column 4·i + q of them is row i of the wave's tile q.
+    uint32_t together = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+      together |= resume_of[w] < c1 || (have_of[w] > 64 && have_of[w] > all / 4) ? 1u << w : 0;
+    together = __builtin_amdgcn_readfirstlane(together);
+    for (; together != 0; together &= together - 1) {
+      const int w = __builtin_ctz(together);
+      constexpr int SPLIT = NW * 64 / DP, AT_ONCE = DP == 64 ? 1 : 2;
+      const int group = wave / SPLIT, split = wave % SPLIT;
+      f4 part[4][NX];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int t = 0; t < NX; ++t) part[q][t] = zero;
+      while (true) {
+        const int count = __builtin_amdgcn_readfirstlane(have_of[w]);
+        const bool last = __builtin_amdgcn_readfirstlane(resume_of[w]) >= c1;
+        for (int k = split * 32 * AT_ONCE; k < count; k += SPLIT * 32 * AT_ONCE) {
+          uint32_t e[AT_ONCE][8];
+          ce_u2 v[AT_ONCE][8];
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i) entries(e[i], w, k + 32 * i, count);
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[i][j] = *reinterpret_cast<const ce_u2*>(Y + (int64_t)(e[i][j] & 0xffffff) * DP + 64 * group + 4 * n);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i) {
+            V P[NX];
+            shares(P, e[i], w, k + 32 * i, count);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t x[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = q & 1 ? v[i][j][q >> 1] >> 16 : v[i][j][q >> 1] & 0xffff;
+#pragma unroll
+              for (int t = 0; t < NX; ++t) part[q][t] = CeT<T>::mm(pack(x), P[t], part[q][t]);
+            }
+          }
+        }
+        if (last) break;
+        __syncthreads();
+        if (wave == w) fill();
+        __syncthreads();
+      }
+      // joined where a chunk was, one split after the other: [column][tile][item], 4 bytes
+      static_assert(sizeof(y0) >= DP * NX * 16 * 4, "");
+      float* parts = reinterpret_cast<float*>(y0);
+#pragma unroll
+      for (int x = 0; x < SPLIT; ++x) {
+        if (split == x) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int t = 0; t < NX; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float* p = parts + ((64 * group + 4 * (4 * kg + i) + q) * NX + t) * 16 + n;
+                *p = x == 0 ? part[q][t][i] : *p + part[q][t][i];
+              }
+        }
+        __syncthreads();
+      }
+      if (wave == w) {
+        have = 0;
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+#pragma unroll
+          for (int t = 0; t < NX; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[f][t][i] += parts[((16 * f + 4 * kg + i) * NX + t) * 16 + n];
+      }
+      __syncthreads();
+    }
+    for (int k = 0; k < have; k += 32) {
+      uint32_t e[8];
+      V P[NX];
+      entries(e, wave, k, have);
+      shares(P, e, wave, k, have);
+      constexpr int BATCH = FB < 8 ? FB : 8;   // tiles of columns whose loads are in flight at once
+#pragma unroll
+      for (int f0 = 0; f0 < FB; f0 += BATCH) {
+        uint32_t v[BATCH][8];
+#pragma unroll
+        for (int f = 0; f < BATCH; ++f) columns(v[f], e, f0 + f);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < BATCH; ++f)
+#pragma unroll
+          for (int t = 0; t < NX; ++t) O[f0 + f][t] = CeT<T>::mm(pack(v[f]), P[t], O[f0 + f][t]);
+      }
     }
   }
 

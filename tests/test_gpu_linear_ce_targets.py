@@ -13,7 +13,7 @@ share is not, and each output is rounded once.
 import pytest
 import torch
 
-from test_gpu_linear_ce import inputs
+from test_gpu_linear_ce import check, inputs
 
 pytestmark = pytest.mark.gpu
 TYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
@@ -64,3 +64,51 @@ def test_loss_and_dh_of_rows_that_are_predicted_well(D, bias, dtype):
     x = exact(h, W, b, t, g)
     assert x["rest"].min() < 1e-7 and x["rest"].max() > 0.5
     close(h, W, b, t, g, loss, linear_ce_backward(saved, g)[0])
+
+
+@pytest.mark.parametrize("weights", ["clicks and purchases", "uniform", "spread", "signed"])
+@pytest.mark.parametrize("bias", [False, True])
+@TYPES
+def test_rows_of_unlike_weights(weights, bias, dtype):
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = inputs(900, 4001, 64, dtype, bias, 0.0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    t = torch.randperm(4001, generator=g, device="cuda")[:900]
+    t[:200] = t[0]                            # one popular item, hit many times in a chunk of rows
+    r = torch.rand(900, generator=g, device="cuda")
+    dloss = {"clicks and purchases": torch.where(r < 0.8, 0.2, 1.0), "uniform": r + 0.01, "spread": torch.exp(-6 * r),
+             "signed": r - 0.5}[weights] / 900
+    loss, saved = linear_ce(h, W, t, bias=b, save=True)
+    close(h, W, b, t, dloss, loss, *linear_ce_backward(saved, dloss))
+
+
+@TYPES
+def test_a_popular_item_in_every_chunk(dtype):
+    """Most rows have the same target: its share is a long sum."""
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = inputs(3000, 500, 40, dtype, True, 0.0)
+    t[torch.rand(3000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.8] = 33
+    dloss = torch.full((3000,), 0.3 / 3000, device="cuda")
+    loss, saved = linear_ce(h, W, t, bias=b, save=True)
+    close(h, W, b, t, dloss, loss, *linear_ce_backward(saved, dloss))
+
+
+@TYPES
+def test_masked_targets_and_rows_with_nothing_else(dtype):
+    """A masked target: the loss is as large as its bias says and its gradients are those of probability 0.  Items that are all
+    masked but one: that one's rows lose nothing and leave no gradient."""
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = inputs(70, 300, 32, dtype, True, 0.0)
+    b[7] = -1e9
+    t[4] = 7
+    loss, saved = linear_ce(h, W, t, bias=b, save=True)
+    assert abs(loss[4].item() - 1e9) <= 64 and (loss[:4] < 100).all()
+    dh, dW, db = linear_ce_backward(saved, torch.ones(70, device="cuda"))
+    z = h.double() @ W.double().t() + b.double()
+    check(h, W, b, t, (z.logsumexp(1) - z.gather(1, t[:, None])[:, 0]).float(), torch.ones(70, device="cuda"), (dh, dW, db))
+    assert abs(db[7].item() + (t == 7).sum().item()) <= 1e-3
+    b[:] = -float("inf")
+    b[7], t[:] = 0.5, 7
+    loss, saved = linear_ce(h, W, t, bias=b, save=True)
+    dh, dW, db = linear_ce_backward(saved, torch.ones(70, device="cuda"))
+    assert (loss == 0).all() and (dh == 0).all() and (dW == 0).all() and (db == 0).all()
