@@ -118,6 +118,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
   __shared__ __attribute__((aligned(16))) uint8_t y0[CE_CH * RB], y1[CE_CH * RB];
   __shared__ __attribute__((aligned(16))) float r0[4 * CE_CH], r1[4 * CE_CH];
   __shared__ int target[FWD ? 16 * NX * NW : 1];
+  __shared__ float xbias[BIAS ? 16 * NX * NW : 1];   // (registers are short at 256 columns)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // neighbouring blocks of one split run on one XCD (workgroups go round the 8 XCDs) and share its L2
@@ -145,13 +146,13 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
     const int64_t left = ny - at;   // rows
     const int64_t bytes = left <= 0 ? 0 : ((left < CE_CH ? left : CE_CH) - 1) * a.ldy * 2 + ycols * 2;
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(Y) + at * a.ldy, 0, (int)bytes, 0x00020000);
+    // a load's rows are the first one's and ROWS more each, with the same swizzle: one register for all
+    constexpr int ROWS = NW * 1024 / RB;
+    static_assert(ROWS % 16 == 0, "");
+    const int e = wave * 64 + lane, row = e / (RB / 16), col = (e % (RB / 16) ^ ce_swz<DP>(row)) * 8;
+    const int off = col < ycols ? (int)(row * a.ldy + col) * 2 : 0x7ffffff0;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int e = (i * NW + wave) * 64 + lane, row = e / (RB / 16), p = e % (RB / 16);
-      const int col = (p ^ ce_swz<DP>(row)) * 8;
-      const int off = col < ycols ? (int)(row * a.ldy + col) * 2 : 0x7ffffff0;
-      rg_blds16(rs, y + (i * NW + wave) * 1024, off, 0);
-    }
+    for (int i = 0; i < LOADS; ++i) rg_blds16(rs, y + (i * NW + wave) * 1024, off, i * ROWS * (int)a.ldy * 2);
     if (wave == 0) {
       if constexpr (FWD) {   // 64 biases
         const int nb = a.bias != nullptr ? (int)(left < CE_CH ? left : CE_CH) * 4 : 0;
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
   if (c0 < c1) issue(c0, y0, r0);
 
   V xf[NX][KS];
-  float ref[NX], sum[NX], xb[NX];
+  float ref[NX], sum[NX];
   bool away = true;   // a reference of this wave lies beyond CE_FAR
   uint64_t met = 0;   // backward: a bit for each 2^fold chunks with targets among this wave's items
   int fold = 2;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
     }
     ref[t] = CE_LOW;
     sum[t] = 0.f;
-    xb[t] = BIAS && x < nx ? a.bias[x] : 0.f;
+    if (BIAS && kg == 0) xbias[wave * 16 * NX + 16 * t + n] = x < nx ? a.bias[x] : 0.f;
     if (FWD && kg == 0) target[wave * 16 * NX + 16 * t + n] = x < nx ? a.tc[x] : -1;
   }
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -219,10 +220,12 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
       f4 S[2][NX];
       const int at = 32 * h + 4 * kg;   // this lane's rows: at .. at + 3 and 16 further on
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int t = 0; t < NX; ++t) {
+        const float xb = BIAS ? xbias[wave * 16 * NX + 16 * t + nn] : 0.f;
 #pragma unroll
-        for (int t = 0; t < NX; ++t)
-          S[j][t] = FWD ? *reinterpret_cast<const f4*>(r + at + 16 * j) : BIAS ? (f4){xb[t], xb[t], xb[t], xb[t]} : zero;
+        for (int j = 0; j < 2; ++j)
+          S[j][t] = FWD ? *reinterpret_cast<const f4*>(r + at + 16 * j) : BIAS ? (f4){xb, xb, xb, xb} : zero;
+      }
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const uint8_t* p = y + (32 * h + nn) * RB + (((4 * s + kg) ^ ce_swz<DP>(nn)) << 4);
