@@ -11,6 +11,10 @@
 // small integers, are as good as exact, and the other planes', 2^-8 as large, run beside them and join at a group's
 // end: in one chain their low bits would be rounded at the size of 24·Σ x (1.3e-6 of the result instead of 1e-7).
 //
+// Infinities would meet their own negative in that offset, and values from 2^96 on could leave fp32 before the scale brings
+// them back: such rows of x are marked when x is split, and behind the last job the table is read once more and their
+// scores made as plain fp32 sums of x·w, w = s·(c − 8) an exact value.
+//
 // A lane's share of an item's group is G/4 consecutive codes; reading those straight from HBM makes 16 rows' short
 // pieces per instruction (64 lanes, 8 cache lines of which 4 B to 16 B are used), so a wave first copies the 16·U
 // items of a job, contiguous in memory, to LDS with 16-byte buffer -> LDS loads and reads them from there.  One buffer a
@@ -42,6 +46,8 @@ __device__ __forceinline__ bf16x8 q4_codes(uint32_t w) {
 }
 __device__ __forceinline__ int q4_order(int e) { return (e >> 1) + 4 * (e & 1); }
 
+#define Q4_LARGE 0x1p96f   // rows of x with larger values, infinities or NaN are summed plainly
+
 __device__ __forceinline__ float q4_x(const float* x, int64_t i) { return x[i]; }
 __device__ __forceinline__ float q4_x(const __bf16* x, int64_t i) { return (float)x[i]; }
 
@@ -65,6 +71,8 @@ __global__ __launch_bounds__(64 * Q4_WAVES, 4) void k_q4_scores(const XT* __rest
   bf16x8* xf = reinterpret_cast<bf16x8*>(lds);
   uint8_t* cl = lds + (size_t)steps * NP * 1024 + (size_t)wave * (cbytes + sbytes);
   const uint8_t* sl = cl + cbytes;
+  // behind them a word a wave, bit m: row m0 + m is marked
+  uint32_t* marks = reinterpret_cast<uint32_t*>(lds + (size_t)steps * NP * 1024 + (size_t)Q4_WAVES * (cbytes + sbytes));
 
   constexpr int per = 16 * U;
   const int64_t jobs = (N + per - 1) / per, stride = (int64_t)gridDim.x * Q4_WAVES;
@@ -84,17 +92,31 @@ __global__ __launch_bounds__(64 * Q4_WAVES, 4) void k_q4_scores(const XT* __rest
   };
   if (job < jobs) fetch(job);
 
-  for (int f = threadIdx.x; f < steps * 64; f += 64 * Q4_WAVES) {
+  uint32_t marked = 0;
+  for (int f = threadIdx.x; f < steps * 64; f += 64 * Q4_WAVES) {   // (a wave's lanes together)
     const int s = f >> 6, l = f & 63, m = m0 + (l & 15);
     const int k0 = (s / SG) * G + (G / 4) * (l >> 4) + 8 * (s % SG);
-    f4 v[2];
+    f4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    uint32_t top = 0;   // of the values' bits without their signs: infinities and NaN are above the finite ones
+    if (m < M) {
+      const XT* at = x + (int64_t)m * ldx + k0;
+      XT r[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = m < M ? q4_x(x, (int64_t)m * ldx + k0 + q4_order(e)) : 0.f;
+      for (int e = 0; e < 8; ++e) r[e] = at[q4_order(e)];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e >> 2][e & 3] = (float)r[e];
+        top = max(top, __float_as_uint(v[e >> 2][e & 3]) & 0x7fffffff);
+      }
+    }
+    const uint64_t on = __ballot(top >= __float_as_uint(Q4_LARGE));
+    marked |= (uint32_t)(on | on >> 16 | on >> 32 | on >> 48) & 0xffff;
     bf16x8 p[3];
     split3x8(v[0], v[1], p[0], p[1], p[2]);
 #pragma unroll
     for (int q = 0; q < NP; ++q) xf[(s * NP + q) * 64 + l] = p[q];
   }
+  if (lane == 0) marks[wave] = marked;
   __syncthreads();
 
   const bf16x8 minus24 = {(__bf16)-24.f, (__bf16)-24.f, (__bf16)-24.f, (__bf16)-24.f,
@@ -154,6 +176,38 @@ __global__ __launch_bounds__(64 * Q4_WAVES, 4) void k_q4_scores(const XT* __rest
       }
     }
   }
+
+  static_assert(Q4_WAVES == 4, "");
+  marked = __builtin_amdgcn_readfirstlane((marks[0] | marks[1]) | (marks[2] | marks[3]));
+  if (marked == 0) return;
+  for (job = (int64_t)blockIdx.x * Q4_WAVES + wave; job < jobs; job += stride) {
+    fetch(job);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (uint32_t left = marked; left != 0; left &= left - 1) {
+      const int m = m0 + __builtin_ctz(left);
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {   // a lane has the quarter kg of each group
+        const int row = 16 * u + n;
+        float sum = 0.f;
+        for (int g = 0; g < groups; ++g) {
+          const int off = row * (K / 2) + g * (G / 2) + kg * (G / 8);
+          const uint8_t* c = cl + 16 * slot(off >> 4) + (off & 15);
+          const float sc = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(sl)[row * groups + g] << 16);
+          for (int k = 0; k < G / 8; ++k) {
+            const int64_t at = (int64_t)m * ldx + g * G + kg * (G / 4) + 2 * k;
+            sum = __builtin_fmaf(sc * (float)((c[k] & 15) - 8), q4_x(x, at), sum);
+            sum = __builtin_fmaf(sc * (float)((c[k] >> 4) - 8), q4_x(x, at + 1), sum);
+          }
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const int64_t item = job * per + row;
+        if (kg == (m - m0) >> 2 && item < N)   // the lane that stored it before
+          y[(int64_t)m * ldy + item] = sum + (bias != nullptr ? bias[item] : 0.f);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
 }
 
 // codes and scales of a row-major table: s = bf16(max |w| / 7) of each group, c = clamp(round(w / s) + 8, 0, 15) with
@@ -207,7 +261,7 @@ template <typename XT, int NP, int G, int U>
 static int q4_launch(const void* x, int64_t ldx, const uint8_t* codes, const uint16_t* scales, const float* bias, int M,
                      int64_t N, int K, float* y, int64_t ldy, hipStream_t stream) {
   const int cbytes = (U * 8 * K + 1023) & ~1023, sbytes = (U * 32 * (K / G) + 1023) & ~1023;
-  const size_t shared = (size_t)(K / 32) * NP * 1024 + (size_t)Q4_WAVES * (cbytes + sbytes);
+  const size_t shared = (size_t)(K / 32) * NP * 1024 + (size_t)Q4_WAVES * (cbytes + sbytes + 4);
   int shift = 3;   // rows of 2^shift granules or fewer
   while ((K >> 5) >> (shift + 1)) ++shift;
   auto kern = k_q4_scores<XT, NP, G, U>;

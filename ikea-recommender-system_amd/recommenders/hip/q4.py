@@ -9,8 +9,9 @@ codes  (N, K / 2) uint8, two codes a byte, the even column in the low half;
 scales (N, K / group) bfloat16; a weight is scales[n, k // group]·(code − 8).
 K is a multiple of `group` (32, 64 or 128) and at most 1024; any number of
 items N, up to 1M rows M.  Sums are kept in fp32; x may be fp32 or bf16 and
-enters exactly.  Capturable; no workspace, no host synchronisation.  Weights
-have to be finite.
+enters exactly, infinities and NaN as a sum of x·w takes them (rows with values
+from 2^96 on are slower: the table is read twice for them).  Capturable; no
+workspace, no host synchronisation.  Weights have to be finite.
 """
 from __future__ import annotations
 
