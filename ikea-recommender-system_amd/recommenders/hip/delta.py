@@ -8,7 +8,8 @@ q, k (B, T, Hk, Dk); v (B, T, Hv, Dv), Hv a multiple of Hk (value heads h of
 key head h // (Hv / Hk)); g, beta (B, T, Hv) fp32, g <= 0 the log of the
 decay (−inf resets).  q, k, v are fp32 or bf16; states and every sum are fp32.
 Dk and Dv are multiples of 8 up to 128.  Strides are free as long as heads'
-rows are contiguous, start at multiples of 16 bytes and do not overlap along T.
+rows are contiguous, start at multiples of 16 bytes (delta_rule_step: anywhere)
+and do not overlap along T.
 
 `lens` (B) int64 on the device: positions at or behind a row's length are not
 read, leave the state as it is and get zeros (also as gradients); a length of
@@ -54,13 +55,14 @@ def _apart(name, t, width):
 
 
 class _Plan:
-    """Checks of the operands that forward, backward and step share.  lead: (B, T) or (B,)."""
+    """Checks of the operands that forward, backward and step share.  lead: 2 for (B, T), 1 for (B,)."""
 
     def __init__(self, q, k, v, g, beta, lead):
-        tensor("q", q, (*[None] * lead, None, None), _IO, align=16)
+        align = 16 if lead == 2 else 1   # (one token is read value by value)
+        tensor("q", q, (*[None] * lead, None, None), _IO, align=align)
         self.Hk, self.Dk = Hk, Dk = q.shape[-2:]
-        tensor("k", k, (*q.shape,), (q.dtype,), q.device, align=16)
-        tensor("v", v, (*q.shape[:-2], None, None), (q.dtype,), q.device, align=16)
+        tensor("k", k, (*q.shape,), (q.dtype,), q.device, align=align)
+        tensor("v", v, (*q.shape[:-2], None, None), (q.dtype,), q.device, align=align)
         self.Hv, self.Dv = Hv, Dv = v.shape[-2:]
         if Hk == 0 or Hv == 0 or Hv % Hk:
             fail("v", f"{Hv} value heads are no multiple of {Hk} key heads")
