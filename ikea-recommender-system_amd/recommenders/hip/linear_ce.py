@@ -8,9 +8,10 @@ activations of every position of a batch.
 h (N, D), W (V, D), both bf16 or both fp16; bias (V) fp32; target (N) int64.
 Rows with a negative target are ignored: loss 0, gradient 0, no work.  A
 target >= V gives NaN in the row's loss and in the gradients.  D is a multiple
-of 8 up to 256, rows start at multiples of 16 bytes, N up to 2^24.  Sums, the
-log-sum-exp and gradients are accumulated in fp32 and rounded once on output
-(probabilities are rounded to the inputs' type for the gradient products).
+of 8 up to 256, rows start at multiples of 16 bytes, N up to 2^24, V up to
+2^31 − 4112.  Sums, the log-sum-exp and gradients are accumulated in fp32 and
+rounded once on output (probabilities are rounded to the inputs' type for the
+gradient products, the target's share is not).
 At least one logit of a row has to lie above −2e38.  dh, dW have their
 inputs' type, db is fp32 (None without a bias).  Nothing synchronises with the
 host; calls can be captured in a graph.
@@ -36,6 +37,19 @@ class Saved:
 
 _plans, _plans_back = Plans(), Plans()
 
+N_MAX, V_MAX = 1 << 24, 0x7ffffff0 - 4096   # what the C entry takes: it counts in 32 bits
+
+
+def _sizes(N, V, D):
+    if D == 0 or D % 8 or D > 256:
+        fail("h", f"a width that is a multiple of 8 up to 256 is expected, got {D}")
+    if V == 0:
+        fail("W", "has no rows")
+    if V > V_MAX:
+        fail("W", f"at most {V_MAX} rows are expected, got {V}")
+    if N > N_MAX:
+        fail("h", f"at most 2^24 rows are expected, got {N}")
+
 
 class _Plan:
     def __init__(self, h, W, target, bias):
@@ -43,12 +57,7 @@ class _Plan:
         self.N, self.D = N, D = h.shape
         tensor("W", W, (None, D), (h.dtype,), h.device, align=16)
         self.V = V = W.shape[0]
-        if D == 0 or D % 8 or D > 256:
-            fail("h", f"a width that is a multiple of 8 up to 256 is expected, got {D}")
-        if V == 0:
-            fail("W", "has no rows")
-        if N > 1 << 24:
-            fail("h", f"at most 2^24 rows are expected, got {N}")
+        _sizes(N, V, D)
         for name, t in (("h", h), ("W", W)):
             if t.shape[0] > 1 and not D <= t.stride(0) < 1 << 23:
                 fail(name, f"rows overlap or lie too far apart: stride {t.stride(0)}")
