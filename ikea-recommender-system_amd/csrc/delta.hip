@@ -1411,7 +1411,8 @@ extern "C" int rg_delta_bwd(const void* q, const void* k, const void* v, const f
       dg == nullptr || dbeta == nullptr || (T > DL_C && (S0 == nullptr || dS == nullptr)) ||
       (a.nseg > 1 && (trans == nullptr || local == nullptr)))
     return RG_ERR_ARG;
-  if (!delta_aligned(q, a.qs, type) || !delta_aligned(k, a.ks, type) || !delta_aligned(d_o, a.dos, type) ||
+  if (!delta_aligned(q, a.qs, type) || !delta_aligned(k, a.ks, type) || !delta_aligned(v, a.vs, type) ||
+      !delta_aligned(d_o, a.dos, type) || (((uintptr_t)dq | (uintptr_t)dk) & 15) ||
       (((uintptr_t)state0 | (uintptr_t)dstate | (uintptr_t)U | (uintptr_t)S0 | (uintptr_t)dX | (uintptr_t)dS |
         (uintptr_t)trans | (uintptr_t)local) & 15))
     return RG_ERR_ARG;

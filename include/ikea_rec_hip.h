@@ -616,7 +616,7 @@ int rg_comm_reduce_scatter(void* comm, const void* send, void* recv, int64_t n, 
  * q, k (B, T, Hk, Dk), v and d_o (B, T, Hv, Dv) of `type` (0 fp32, 1 bf16), g, beta (B, T, Hv) fp32; Hv a multiple of
  * Hk; Dk, Dv multiples of 8 up to 128.  strides: HOST array of 18, the (B, T, H) strides in elements of q, k, v, g, beta,
  * d_o; rows (the last dimension) are contiguous, positions (T) at least a row and less than 2^23 elements apart, rows of
- * q, k, d_o start at multiples of 16 bytes.  lens (B) int64,
+ * q, k, d_o, for rg_delta_bwd of v, and dq, dk start at multiples of 16 bytes (rg_delta_step: anywhere).  lens (B) int64,
  * optional: positions at or behind it are not read, do not change the state and get zeros.  Contiguous: o, dv
  * (B, T, Hv, Dv), dq, dk (B, T, Hk, Dk), dg, dbeta (B, T, Hv), the states (B, Hv, Dk, Dv) fp32.
  * For the backward pass the forward leaves U (B, Hv, T, Dv) and S0 (rg_delta_chunk_floats values, when T > 32); both
