@@ -1234,6 +1234,8 @@ static int delta_check(const DeltaArgs& a, int type) {
 }
 // positions at least a row apart, a chunk's 32 of them within a buffer's 2 GB
 static bool delta_apart(const int64_t* s, int T, int width) { return T == 1 || (s[1] >= width && s[1] < (1 << 23)); }
+// so lie the contiguous outputs' positions, all heads of one next to another
+static bool delta_wide(int Hk, int Hv, int Dk, int Dv) { return (int64_t)Hk * Dk >= (1 << 23) || (int64_t)Hv * Dv >= (1 << 23); }
 // rows at multiples of 16 bytes
 static bool delta_aligned(const void* p, const int64_t* s, int type) {
   const int64_t e = type == 0 ? 4 : 2;
@@ -1377,6 +1379,7 @@ extern "C" int rg_delta_fwd(const void* q, const void* k, const void* v, const f
   a.S0 = U != nullptr && T > DL_C ? S0 : nullptr;
   const int rc = delta_check(a, type);
   if (rc != RG_OK) return rc;
+  if (delta_wide(Hk, Hv, Dk, Dv)) return RG_ERR_SHAPE;
   if (!delta_apart(a.qs, T, Dk) || !delta_apart(a.ks, T, Dk) || !delta_apart(a.vs, T, Dv) || !delta_apart(a.gs, T, 1) ||
       !delta_apart(a.bs, T, 1))
     return RG_ERR_ARG;
@@ -1402,6 +1405,7 @@ extern "C" int rg_delta_bwd(const void* q, const void* k, const void* v, const f
   a.dq = dq, a.dk = dk, a.dv = dv, a.dg = dg, a.dbeta = dbeta, a.dstate0 = dstate0;
   const int rc = delta_check(a, type);
   if (rc != RG_OK) return rc;
+  if (delta_wide(Hk, Hv, Dk, Dv)) return RG_ERR_SHAPE;
   if (!delta_apart(a.qs, T, Dk) || !delta_apart(a.ks, T, Dk) || !delta_apart(a.vs, T, Dv) || !delta_apart(a.gs, T, 1) ||
       !delta_apart(a.bs, T, 1))
     return RG_ERR_ARG;

@@ -54,6 +54,14 @@ def _apart(name, t, width):
         fail(name, f"positions overlap or lie too far apart: stride {t.stride(1)}")
 
 
+def _sizes(B, T, Hk, Hv, Dk, Dv, lead):
+    """lead: 2 for (B, T), 1 for (B,), whose kernel takes any number of heads."""
+    if B * Hv >= 1 << 24 or T > 65535 * 32:
+        fail("q", f"less than 2^24 rows times value heads and at most 2^21 − 32 positions are expected, got {B}·{Hv} and {T}")
+    if lead == 2 and max(Hk * Dk, Hv * Dv) >= 1 << 23:
+        fail("q" if Hk * Dk >= Hv * Dv else "v", f"all heads of a position have to be less than 2^23 values, got {max(Hk * Dk, Hv * Dv)}")
+
+
 class _Plan:
     """Checks of the operands that forward, backward and step share.  lead: 2 for (B, T), 1 for (B,)."""
 
@@ -74,8 +82,7 @@ class _Plan:
                 fail(name, f"a tensor of shape {(*q.shape[:-2], Hv)} is expected")
             tensor(name, t[..., None], (*q.shape[:-2], Hv, 1), (torch.float32,), q.device)   # any strides
         self.B, self.T = q.shape[0], q.shape[1] if lead == 2 else 1
-        if self.B * Hv >= 1 << 24 or self.T > 65535 * 32:
-            fail("q", f"less than 2^24 rows times value heads and at most 2^21 − 32 positions are expected, got {self.B}·{Hv} and {self.T}")
+        _sizes(self.B, self.T, Hk, Hv, Dk, Dv, lead)
         if self.T > 1:
             for name, t, d in (("q", q, Dk), ("k", k, Dk), ("v", v, Dv), ("g", g, 1), ("beta", beta, 1)):
                 _apart(name, t, d)

@@ -614,7 +614,7 @@ int rg_comm_reduce_scatter(void* comm, const void* send, void* recv, int64_t n, 
 /* ---- Gated delta rule (csrc/delta.hip): a linear-attention recurrence beside rg_gru_fwd / rg_gru_bwd.  Per value head
  * S_t = exp(g_t) S_{t-1} + beta_t k_t (v_t - exp(g_t) S_{t-1}^T k_t)^T, o_t = scale S_t^T q_t, S a Dk x Dv matrix.
  * q, k (B, T, Hk, Dk), v and d_o (B, T, Hv, Dv) of `type` (0 fp32, 1 bf16), g, beta (B, T, Hv) fp32; Hv a multiple of
- * Hk; Dk, Dv multiples of 8 up to 128.  strides: HOST array of 18, the (B, T, H) strides in elements of q, k, v, g, beta,
+ * Hk; Dk, Dv multiples of 8 up to 128; Hk Dk and Hv Dv less than 2^23 (rg_delta_step: any).  strides: HOST array of 18, the (B, T, H) strides in elements of q, k, v, g, beta,
  * d_o; rows (the last dimension) are contiguous, positions (T) at least a row and less than 2^23 elements apart, rows of
  * q, k, d_o, for rg_delta_bwd of v, and dq, dk start at multiples of 16 bytes (rg_delta_step: anywhere).  lens (B) int64,
  * optional: positions at or behind it are not read, do not change the state and get zeros.  Contiguous: o, dv
