@@ -27,7 +27,7 @@ import ctypes as C
 import torch
 
 from . import call, ptr
-from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole, wrote
+from .operands import TYPES, Plans, entry, fail, held, layout, run, stride, tensor, whole, wrote
 
 _IO = (torch.float32, torch.bfloat16)
 
@@ -38,7 +38,7 @@ class Saved:
 
     def __init__(self, plan, operands, scale, U, S0, trans):
         self.plan, self.operands, self.scale, self.U, self.S0, self.trans = plan, operands, scale, U, S0, trans
-        self.versions = [version(t) for t in operands]
+        self.held = [held(t) for t in operands]
 
 
 _plans, _plans_back, _plans_step = Plans(), Plans(), Plans()
@@ -157,8 +157,8 @@ def delta_rule_backward(saved, do, dstate=None):
     if not isinstance(saved, Saved):
         fail("saved", "what delta_rule(..., save=True) returned is expected")
     p, (q, k, v, g, beta, lens, state) = saved.plan, saved.operands
-    if [version(t) for t in saved.operands] != saved.versions:
-        raise RuntimeError("delta_rule_backward: an operand of the forward call was changed in place since")
+    if [held(t) for t in saved.operands] != saved.held:
+        raise RuntimeError("delta_rule_backward: an operand of the forward call was changed in place or given other memory since")
     key = (p, layout(do), layout(dstate)) if isinstance(do, torch.Tensor) else None
     strides = _plans_back.get(key) or _plans_back.put(key, _back_plan(p, do, dstate))
     if (do.data_ptr() | (ptr(dstate) or 0)) & 15 and not p.empty:

@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import call, ptr
-from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, version, whole
+from .operands import TYPES, Plans, entry, fail, held, layout, run, stride, tensor, whole
 
 _HALF = (torch.bfloat16, torch.float16)
 _I64 = (torch.int64,)
@@ -32,7 +32,7 @@ class Saved:
 
     def __init__(self, plan, W, bias, buffer):
         self.plan, self.W, self.bias, self.buffer = plan, W, bias, buffer
-        self.versions = version(W), version(bias)
+        self.held = held(W), held(bias)
 
 
 _plans, _plans_back = Plans(), Plans()
@@ -102,8 +102,8 @@ def linear_ce_backward(saved, dloss):
     if not isinstance(saved, Saved):
         fail("saved", "what linear_ce(..., save=True) returned is expected")
     p, W, bias = saved.plan, saved.W, saved.bias
-    if (version(W), version(bias)) != saved.versions:
-        raise RuntimeError("linear_ce_backward: W or bias was changed in place since the forward call")
+    if (held(W), held(bias)) != saved.held:
+        raise RuntimeError("linear_ce_backward: W or bias was changed in place or given other memory since the forward call")
     key = (p.N, layout(dloss), p.device) if isinstance(dloss, torch.Tensor) else None
     step = _plans_back.get(key)
     if step is None:

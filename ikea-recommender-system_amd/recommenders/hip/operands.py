@@ -62,6 +62,11 @@ def version(t):
     return None if t is None or t.is_inference() else t._version
 
 
+def held(t):
+    """What a backward pass that reads an operand again compares: its version, and where and how it lies."""
+    return None if t is None else (version(t), t.data_ptr(), t.stride(), t.shape)
+
+
 def wrote(t):
     """After a kernel wrote a caller's tensor in place: counted as a write, so that a backward pass that still needs the
     old values says so."""
