@@ -27,7 +27,7 @@ import ctypes as C
 import torch
 
 from . import call, ptr
-from .operands import TYPES, Plans, entry, fail, held, layout, run, stride, tensor, whole, wrote
+from .operands import TYPES, Plans, entry, fail, held, keep, layout, run, stream, stride, tensor, whole, wrote
 
 _IO = (torch.float32, torch.bfloat16)
 
@@ -38,7 +38,7 @@ class Saved:
 
     def __init__(self, plan, operands, scale, U, S0, trans):
         self.plan, self.operands, self.scale, self.U, self.S0, self.trans = plan, operands, scale, U, S0, trans
-        self.held = [held(t) for t in operands]
+        self.held, self.stream = [held(t) for t in operands], stream(plan.device)
 
 
 _plans, _plans_back, _plans_step = Plans(), Plans(), Plans()
@@ -173,6 +173,7 @@ def delta_rule_backward(saved, do, dstate=None):
         if dstate0 is not None:
             dstate0.copy_(dstate) if dstate is not None else dstate0.zero_()
     else:
+        keep(p.device, saved.stream, saved.U, saved.S0, saved.trans)
         dX = torch.empty(p.B, p.Hv, p.T, p.Dv, **full)
         dS = torch.empty(p.chunks, **full) if p.chunks else None
         local = torch.empty(p.local, **full) if p.local else None

@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import call, ptr
-from .operands import TYPES, Plans, entry, fail, held, layout, run, stride, tensor, whole
+from .operands import TYPES, Plans, entry, fail, held, keep, layout, run, stream, stride, tensor, whole
 
 _HALF = (torch.bfloat16, torch.float16)
 _I64 = (torch.int64,)
@@ -32,7 +32,7 @@ class Saved:
 
     def __init__(self, plan, W, bias, buffer):
         self.plan, self.W, self.bias, self.buffer = plan, W, bias, buffer
-        self.held = held(W), held(bias)
+        self.held, self.stream = (held(W), held(bias)), stream(plan.device)
 
 
 _plans, _plans_back = Plans(), Plans()
@@ -119,6 +119,7 @@ def linear_ce_backward(saved, dloss):
         if db is not None:
             db.zero_()
     else:
+        keep(p.device, saved.stream, saved.buffer)
         work = torch.empty(p.work[2], dtype=torch.float32, device=p.device)
         run(p.backward, p.device, W.data_ptr(), p.ldw, ptr(bias), dloss.data_ptr(), *step, p.type, p.N, p.V, p.D,
             saved.buffer.data_ptr(), work.data_ptr(), dh.data_ptr(), dW.data_ptr(), ptr(db))

@@ -74,6 +74,21 @@ def wrote(t):
         torch._C._increment_version([t])
 
 
+def stream(device):
+    """The current stream of a device, as run() uses it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def keep(device, since, *buffers):
+    """Buffers that a call on stream `since` left are read on the current stream: if that is another one, their memory is not
+    given away before it has passed."""
+    if stream(device) != since:
+        now = torch.cuda.current_stream(device)
+        for t in buffers:
+            if t is not None:
+                t.record_stream(now)
+
+
 class Plans(dict):
     """Checked argument layouts -> what a call needs of them.  Bounded: a program has few layouts; one that keeps making
     new ones starts over now and then."""
