@@ -52,6 +52,28 @@ def stride(t, dim):
     return 0 if t.shape[dim] == 1 else t.stride(dim)
 
 
+def shares_memory(t, rows):
+    """Whether the bytes of a tensor lie among `rows` (dimensions 0 and 1; rows of contiguous values, the rows apart): for an
+    output that is written while t is still read."""
+    if t is None or not t.numel() or not rows.numel():
+        return False
+    size, step = rows.element_size(), rows.stride(0) * rows.element_size()
+    first, width = rows.data_ptr(), rows.shape[1] * size
+    last = first + (rows.shape[0] - 1) * step + width
+    each = t.element_size()
+    # t as rows of its own: its first dimension, if any, and what a row spans
+    n = t.shape[0] if t.dim() > 1 else 1
+    lead = t.stride(0) * each if t.dim() > 1 else 0
+    span = (sum((s - 1) * st for s, st in zip(t.shape[-1:], t.stride()[-1:])) + 1) * each
+    lo, hi = t.data_ptr(), t.data_ptr() + (n - 1) * lead + span
+    if hi <= first or last <= lo:
+        return False
+    if n > 1 and rows.shape[0] > 1 and lead == step:   # columns of one matrix: do they meet?
+        off = (lo - first) % step
+        return off < width or off + span > step
+    return True
+
+
 def layout(t):
     """What the checks of a tensor argument look at, apart from its address: calls with known layouts skip them."""
     return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else None if t is None else type(t)

@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import ptr
-from .operands import TYPES, Plans, entry, fail, layout, run, stride, tensor, whole, wrote
+from .operands import TYPES, Plans, entry, fail, layout, run, shares_memory, stride, tensor, whole, wrote
 
 GROUPS = (32, 64, 128)
 K_MAX, M_MAX = 1024, 65535 * 16
@@ -72,7 +72,8 @@ def _plan(x, codes, scales, bias):
 
 
 def q4_scores(x, codes, scales, bias=None, out=None):
-    """x (M, K) · table (N, K)ᵀ + bias -> (M, N) fp32.  out: written instead of a new tensor; its rows may be strided."""
+    """x (M, K) · table (N, K)ᵀ + bias -> (M, N) fp32.  out: written instead of a new tensor; its rows may be strided, and
+    it must not share memory with the operands."""
     key = (layout(x), layout(codes), layout(scales), layout(bias)) if isinstance(x, torch.Tensor) else None
     fn, device, M, N, K, group, kind, ldx = _plans.get(key) or _plans.put(key, _plan(x, codes, scales, bias))
     at = codes.data_ptr(), scales.data_ptr()
@@ -85,6 +86,9 @@ def q4_scores(x, codes, scales, bias=None, out=None):
         tensor("out", out, (M, N), (torch.float32,), device)
         if M > 1 and out.stride(0) < N:
             fail("out", f"rows overlap: stride {out.stride(0)}, {N} items")
+        for name, t in (("x", x), ("codes", codes), ("scales", scales), ("bias", bias)):
+            if shares_memory(t, out):
+                fail("out", f"shares memory with {name}, which is read while it is written")
         ldy = stride(out, 0) or N
     if M and N:
         run(fn, device, x.data_ptr(), kind, ldx, *at, ptr(bias), M, N, K, group, out.data_ptr(), ldy)
