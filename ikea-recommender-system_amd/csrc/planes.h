@@ -41,15 +41,6 @@ struct PlaneMat {
       f[q] = __builtin_bit_cast(bf16x8, v);
     }
   }
-  __device__ __forceinline__ void put(int r, int c, float x) const {
-    __bf16* a = p + r * LD + pl_place(c);
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-      const __bf16 b = (__bf16)x;
-      a[q * PLANE] = b;
-      x -= (float)b;
-    }
-  }
   // 8 consecutive columns c .. c + 7 (c a multiple of 8)
   __device__ __forceinline__ void put8(int r, int c, const bf16x8* v) const {
     __bf16* a = p + r * LD + pl_place(c);
