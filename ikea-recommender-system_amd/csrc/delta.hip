@@ -11,8 +11,9 @@
 // and, per chunk and independent of the others, dP = dO Uᵀ, dA = −dX Uᵀ and the rest (k_delta_grads).
 //
 // One wave owns 16·CT value columns of one (row, value head) and their part of the state, in accumulators; it makes the
-// chunk's P and T itself and never waits for another wave.  What bounds these kernels is the chain of dependent steps
-// inside a chunk (about 20 products and a triangular solve of 16 steps), not bandwidth or MFMAs: sessions are
+// chunk's P and T itself and never waits for another wave.  What bounds these kernels is latency inside a chunk (about 20
+// products and a triangular solve of 16 steps), not bandwidth or MFMAs; T needs no state, so its part of that is not
+// in the chain from chunk to chunk, but every wave makes it for itself, in every pass.  Sessions are
 // short, so the answer is many independent waves with little LDS, and each step small.  Forwards, 8192 sessions x
 // heads of up to 50 positions of width 64, bf16: 104 us.  (Workgroups of four waves with 64-position chunks, K, Q, P and T
 // shared through LDS and a barrier between steps, two to a CU: 320 us.  Three waves a SIMD spill: 602 us a
@@ -783,7 +784,8 @@ __global__ __launch_bounds__(4 * DP) void k_delta_join(DeltaArgs a) {
 // What bounds it is vector instructions, most of them splitting operands into planes, and the chain of loads, products and sums.  (Two
 // waves, one per tile of positions, each splitting all of S, dS', dX and U for itself: 270 us against 157 on 4 x 8
 // heads x 4096 positions of width 128, 181 against 165 on 8192 sessions x heads of up to 50 positions of width 64.  Waves a
-// SIMD: with three, fp32 spills 23 registers, 91 us against 75 on 2048 sessions x heads; bf16 does not, 165 us against 219 with two.
+// SIMD: with three, fp32 spills 23 registers at width 64, 91 us against 75 on 2048 sessions x heads; bf16 does not, 165 us against
+// 219 with two.  At width 128 fp32 spills 37 with two: 547 us for the whole backward pass of 2048 sessions x heads, bf16 158.
 // Rows of one chunk, which have no states, in a kernel of their own with four waves a SIMD: 56 + 118 us against 165.)
 template <int DP, int NI>
 struct DlGradLds {

@@ -27,17 +27,17 @@
 // has met only masked items, or logits beyond CE_FAR, pays one subtraction more an element.  Per 32
 // rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D MFMA flops.
 //
-// Measured, whole step: 4096 rows x 1M items x 128 bf16 3.42 ms, 1250 TFLOP/s of these 8 N V D (91 % of what a large
-// library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.15 ms, 1090 TFLOP/s;
-// 64 x 10001 x 32 34 us, of which the launches and the waits between its five kernels (3 to 8 us each) are most.
+// Measured, whole step: 4096 rows x 1M items x 128 bf16 3.49 to 3.65 ms, 1150 to 1200 TFLOP/s of these 8 N V D (85 to 89 % of
+// what a large library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.23 to
+// 1.26 ms, 1000 to 1030 TFLOP/s, 0.08 ms of it the shares of the 256 items that half of these targets are among (one
+// workgroup's; rounded shares 1.15 ms; added row by row, by one wave each: 4.4 ms); 64 x 10001 x 32 32 to 35 us, of which the
+// launches and the waits between its five kernels (3 to 8 us each) are most.
 //
 // Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
 // packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
 // P is rounded to bf16 / fp16 for the second product (half a step of the type, once, as its other operand is held); sums
 // of P, lse, O and the gradients are fp32, and each output is rounded once.  Backwards g is scaled so that the largest
-// |g| is 2^13, and back in fp32: a mean's g is one number for every row and most of a target item's gradient, and
-// rounded as it stands it moved all of dW the same way (2.2 times the error of the output's own rounding; scaled it
-// enters exactly).  It also keeps fp16's small probabilities out of its subnormals; forwards P <= 2^15 does.
+// |g| is 2^13, and back in fp32: it keeps fp16's small probabilities out of its subnormals; forwards P <= 2^15 does.
 #include "common.h"
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
@@ -818,7 +818,7 @@ static int ce_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // a workgroup holds CE_NW · CE_NX · 16 = 256 rows of X: eight waves, two on a SIMD, so that one's exponentials run beside
 // the other's MFMAs, and two tiles a wave.  Measured (4096 x 1M x 128 bf16 / 7867 rows x 78K x 256 fp16, whole
-// step): two tiles 3.52 / 1.31 ms (now 3.42 / 1.15), three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
+// step, as the passes were then): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
 // two to six tiles each 5.2 ms and more (nothing beside the exponentials).  Exponentials woven between the MFMAs of the tiles
 // before and after by hand (three buffers, sched_group_barrier): 116 to 800 registers spilled, 14.9 / 9.5 ms.
 #define CE_NX 2

@@ -21,17 +21,18 @@
 // wave; the next job's copy starts when the last code has been read, before this job's scores are stored.  A second
 // buffer a wave halves the waves that fit and measured 36 us against 30 on 1M x 128.
 //
-// Measured: 1M x 128 for one fp32 session, G = 32: 28 us, 76 MB, 2.7 TB/s with the launch (the vector instructions take
-// 18 of the 28: 44 a step of 16 items x 32 codes, of which 8 expand the codes); 5M x 256 for 16 bf16 sessions,
-// G = 64: 250 us, 0.68 GB read and 0.32 GB written, 4.0 TB/s, 78 % of a large copy's rate: the scores of 16 rows end
-// anywhere in a cache line.  10K x 64: 3.5 us of kernel, less than a launch costs.
+// Measured: 1M x 128 for one fp32 session, G = 32: 25 to 28 us, 76 MB, 2.7 to 3 TB/s with the launch (the vector instructions
+// take 18 of them: 44 a step of 16 items x 32 codes, of which 8 expand the codes; the three planes are three MFMAs and three
+// operand reads, each for one row of 16); 5M x 256 for 16 bf16 sessions, G = 64: 248 us, 0.68 GB read and 0.32 GB
+// written, 4.0 TB/s, 78 % of a large copy's rate: the scores of 16 rows end anywhere in a cache line.  10K x 64: 3 to
+// 4 us of kernel, less than a launch costs.  64 rows of 1M x 128: 110 us.
 #include "common.h"
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 #define Q4_WAVES 4
 #define Q4_K_MAX 1024
-#define Q4_GRID 2048   // 5M x 256: 250 us; 1024 305, 1280 257, 4096 259
+#define Q4_GRID 2048   // 5M x 256: 250 us; 1024 305, 1280 257, 4096 259 (before x was loaded under one guard: now 248)
 
 // two bf16 values (16 + c) of the codes at bits 4j .. and 16 + 4j .. of w
 template <int J>

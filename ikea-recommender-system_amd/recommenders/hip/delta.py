@@ -6,15 +6,16 @@ serving.  Per value head, with a Dk x Dv state:
 
 q, k (B, T, Hk, Dk); v (B, T, Hv, Dv), Hv a multiple of Hk (value heads h of
 key head h // (Hv / Hk)); g, beta (B, T, Hv) fp32, g <= 0 the log of the
-decay (−inf resets).  q, k, v are fp32 or bf16; states and every sum are fp32.
-Dk and Dv are multiples of 8 up to 128.  Strides are free as long as heads'
-rows are contiguous, start at multiples of 16 bytes (delta_rule_step: anywhere)
-and do not overlap along T.
+decay (−inf resets a finite state, in delta_rule_step any).  q, k, v are fp32
+or bf16; states and every sum are fp32.  Dk and Dv are multiples of 8 up to
+128.  Strides are free as long as heads' rows are contiguous, start at
+multiples of 16 bytes (delta_rule_step: anywhere) and do not overlap along T.
 
 `lens` (B) int64 on the device: positions at or behind a row's length are not
 read, leave the state as it is and get zeros (also as gradients); a length of
 0 returns the initial state.  Nothing synchronises with the host; every call
-can be captured in a graph.
+can be captured in a graph.  Plain tensors in and out: no autograd graph is
+built, whatever requires a gradient.
 
     o, state, saved = delta_rule(q, k, v, g, beta, lens=lens, save=True)
     dq, dk, dv, dg, dbeta, _ = delta_rule_backward(saved, do)

@@ -14,7 +14,8 @@ rounded once on output (probabilities are rounded to the inputs' type for the
 gradient products, the target's share is not).
 At least one logit of a row has to lie above −2e38.  dh, dW have their
 inputs' type, db is fp32 (None without a bias).  Nothing synchronises with the
-host; calls can be captured in a graph.
+host; calls can be captured in a graph.  Plain tensors in and out: no autograd
+graph is built, whatever requires a gradient.
 """
 from __future__ import annotations
 
