@@ -87,3 +87,30 @@ def test_popular_items(N, V, D, dtype):
     compare(h, W, b, t, dloss, loss, *grads)
     for x, y in zip(grads, linear_ce_backward(saved, dloss)):
         assert x is None or torch.equal(x, y)
+
+
+@pytest.mark.parametrize("N,V,D", [(1500, 65537, 64), (2500, 3001, 136)])
+def test_captured_and_replayed(N, V, D):
+    """More rows than one workgroup lists, whole rounds or splits, a popular item that changes between replays."""
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = inputs(N, V, D, torch.bfloat16, True, 0.3)
+    g = torch.rand(N, device="cuda")
+
+    def whole():
+        loss, saved = linear_ce(h, W, t, bias=b, save=True)
+        return (loss, *linear_ce_backward(saved, g))
+    whole()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = whole()
+    for k in range(4):
+        h.copy_(n(N, D))
+        t.copy_(torch.randint(-V // 2 if k else 0, V, (N,), device="cuda"))
+        t[: N * k // 4] = 17 + 900 * k
+        b[100:200] = -1e9 if k % 2 else 0.0
+        graph.replay()
+        eager = whole()
+        torch.cuda.synchronize()
+        for x, y in zip(held, eager):
+            assert torch.equal(x, y)
+    compare(h, W, b, t, g, *held)
