@@ -10,7 +10,7 @@
 //             and the sum of P per row and split of the vocabulary.  k_ce_join takes the target's logit in fp32 and has the
 //             odds q against it, loss = log(1 + q), and dh = (Σ_{v ≠ t} p_v W_v) − (1 − p_t) W_t with 1 − p_t = q / (1 + q):
 //             where a row is predicted well both are small, and neither is a difference of large rounded values (with
-//             the target inside P, dh was off by 0.4 % of |W_t| there, a third of itself at p_t = 0.996).
+//             the target inside P, dh is off by up to 0.36 % of |W_t|: 7 % of itself at p_t = 0.98, nine times at 0.9998).
 //   backward  X = items of W, Y = rows of h: f = g_r e^(z − lse_r), and −g_r (1 − p_t) at the row's target; O = dW, and
 //             Σ_r P = db from the unrounded P.  A target's share is most of a target item's gradient; rounded to the type it
 //             moved that by as much as the output's own rounding again (0.2 beside 1.0, clicks beside purchases: every
@@ -749,7 +749,8 @@ __global__ __launch_bounds__(1024) void k_ce_largest(const float* __restrict__ g
 
 // dh = g times what the forward left, zeros for ignored rows; the backward pass's records of the packed rows (four
 // values: log2 |g| − lse in base 2; the target's −g (1 − p_t), whose sign bit is clear where g is negative; the target as
-// int bits; and what is taken off the logits first, not 0 only beyond CE_FAR), and the factor that the scaled g leave out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
+// int bits; and what is taken off the logits first, not 0 only beyond CE_FAR), and the factor that the scaled g leave
+// out.  largest: of every 1024 rows, or null, and each wave looks at the rows itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_dh(const float* __restrict__ g, int64_t sg, const int* __restrict__ inv,
                                                const int* __restrict__ count, const int* __restrict__ tc,
@@ -818,9 +819,9 @@ static int ce_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int64_t ce_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // a workgroup holds CE_NW · CE_NX · 16 = 256 rows of X: eight waves, two on a SIMD, so that one's exponentials run beside
 // the other's MFMAs, and two tiles a wave.  Measured (4096 x 1M x 128 bf16 / 7867 rows x 78K x 256 fp16, whole
-// step, as the passes were then): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms, four waves with
-// two to six tiles each 5.2 ms and more (nothing beside the exponentials).  Exponentials woven between the MFMAs of the tiles
-// before and after by hand (three buffers, sched_group_barrier): 116 to 800 registers spilled, 14.9 / 9.5 ms.
+// step, as the passes were then): two tiles 3.52 / 1.31 ms, three (128 columns; registers full) 4.36 ms, one 4.17 / 1.41 ms,
+// four waves with two to six tiles each 5.2 ms and more (nothing beside the exponentials).  Exponentials woven between the
+// MFMAs of the tiles before and after by hand (three buffers, sched_group_barrier): 116 to 800 registers spilled, 14.9 / 9.5 ms.
 #define CE_NX 2
 #define CE_NW 8
 
