@@ -52,3 +52,31 @@ def test_delta(B, T):
     x, n = test_gpu_delta.inputs(B, T, 1, 2, 64, 64, torch.float32)
     do = n(B, T, 2, 64)
     on_two_streams(lambda: delta_rule(**x, save=True)[2], lambda saved: delta_rule_backward(saved, do))
+
+
+def test_backward_captured_behind_an_eager_forward():
+    """The captured backward call runs on the capture's stream; what the forward call left is held by the program."""
+    from recommenders.hip.delta import delta_rule, delta_rule_backward
+    from recommenders.hip.linear_ce import linear_ce, linear_ce_backward
+    h, W, b, t, n = test_gpu_linear_ce.inputs(300, 2000, 64, torch.bfloat16, True, 0.1)
+    x, m = test_gpu_delta.inputs(3, 90, 1, 2, 32, 32, torch.float32)
+    g, do = torch.rand(300, device="cuda"), m(3, 90, 2, 32)
+    kept, saved = linear_ce(h, W, t, bias=b, save=True)[1], delta_rule(**x, save=True)[2]
+
+    def both():
+        return [*linear_ce_backward(kept, g), *delta_rule_backward(saved, do)[:5]]
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for _ in range(3):
+        g.copy_(torch.rand(300, device="cuda"))
+        do.copy_(m(3, 90, 2, 32))
+        graph.replay()
+        eager = both()
+        torch.cuda.synchronize()
+        for a, e in zip(held, eager):
+            assert torch.equal(a, e)
+    del kept, saved
+    torch.cuda.synchronize()
