@@ -17,6 +17,8 @@
 //             click's share by 1e-3 the same way).  So what the rounding leaves off follows behind the last chunk, for the
 //             N rows of a whole pass alone: a wave remembers in which chunks it met targets of its items, lists those
 //             rows, and takes 32 of them for one more product; a popular item's rows are shared among the workgroup's waves.
+//             Less than 2^-16 of a share stays off (1/32 of fp16's half step): with the weights of a mean, scaled to 2^13,
+//             2^13 (1 - p_t) is so near 2^13 for most rows of a large vocabulary.
 // The accumulator of S (16 rows of Y x 16 of X per tile; lane (kg, n) holds rows 4·kg + i of column n) is already the B
 // operand of the second product, whose A operand is Y_c read from LDS with ds_read_b64_tr_b16.  The biases are
 // S's start value and cost no instruction an element; backwards −lse and log2 |g| enter with the exponent's scaling (as a
@@ -50,6 +52,7 @@ typedef short ce_s8 __attribute__((ext_vector_type(8)));
 #define CE_L2E 1.4426950408889634f
 #define CE_LN2 0.6931471805599453f
 #define CE_LOW (-2.0e38f)  // the running reference before any logit
+#define CE_REST 0x1p-16f   // what is left off a target's share and is less than this of it stays off
 #define CE_FAR 32768.f     // references beyond it: exponents from differences of logits
 
 template <typename T>
@@ -375,6 +378,9 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
       const uint64_t rest = c < c1 ? met >> group : 0;
       return rest == 0 ? c1 : rest & 1 ? c : c0 + ((group + __builtin_ctzll(rest)) << fold);
     };
+    int n = threadIdx.x & 15, kg = (threadIdx.x & 63) >> 4;
+    asm volatile("" : "+v"(n), "+v"(kg));   // what is derived from them is not kept over the loop above
+    const int lane = 16 * kg + n;
     int have = 0, resume = next(c0);
     auto fill = [&]() __attribute__((always_inline)) {
       have = 0;
@@ -396,7 +402,9 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int at = __float_as_int(target[i][e]) - x0;
-            mask[e] = __ballot(c[i] + kg < c1 && at >= 0 && at < 16 * NX);
+            const float all = share[i][e];
+            share[i][e] = all - (float)(T)all;
+            mask[e] = __ballot(c[i] + kg < c1 && at >= 0 && at < 16 * NX && fabsf(share[i][e]) > CE_REST * fabsf(all));
             more += __popcll(mask[e]);
           }
           room = room && have + more <= LIST;
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
               if (mask[e] >> lane & 1) {
                 list[wave][place] = (uint32_t)(__float_as_int(target[i][e]) - x0) << 24 |
                                     (uint32_t)((c[i] + kg) * CE_CH + 4 * n + e);
-                left_off[wave][place] = share[i][e] - (float)(T)share[i][e];
+                left_off[wave][place] = share[i][e];
               }
               have += __popcll(mask[e]);
             }
