@@ -26,14 +26,14 @@
 // the exponentials, not the MFMAs, take the longer at small D: an element costs a scaling, an exponential (four
 // issue slots), a sum and half a conversion, so there is no running maximum either: forwards the reference only
 // moves when a lane's eight powers sum to more than LIM, which needs one comparison per eight elements.  A wave that
-// has met only masked items, or logits beyond CE_FAR, pays one subtraction more an element.  Per 32
+// has met only masked items, or logits beyond CE_FAR, looks for the largest one each time and takes it off first.  Per 32
 // rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D MFMA flops.
 //
-// Measured, whole step: 4096 rows x 1M items x 128 bf16 3.49 to 3.65 ms, 1150 to 1200 TFLOP/s of these 8 N V D (85 to 89 % of
-// what a large library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.23 to
-// 1.26 ms, 1000 to 1030 TFLOP/s, 0.08 ms of it the shares of the 256 items that half of these targets are among (one
-// workgroup's; rounded shares 1.15 ms; added row by row, by one wave each: 4.4 ms); 64 x 10001 x 32 32 to 35 us, of which the
-// launches and the waits between its five kernels (3 to 8 us each) are most.
+// Measured, whole step: 4096 rows x 1M items x 128 bf16 3.47 to 3.53 ms, 1190 to 1210 TFLOP/s of these 8 N V D (88 to 90 % of
+// what a large library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.18
+// to 1.19 ms, 1060 to 1070 TFLOP/s, and 1.25 ms where the rows' weights differ: half of these targets are among 256 items, whose
+// shares one workgroup adds (row by row, by one wave each: 4.4 ms); 64 x 10001 x 32 32 to 36 us, of which the launches and the
+// waits between its five kernels (3 to 8 us each) are most.
 //
 // Rows with a negative target are left out from the start: k_ce_rows lists the others in order, and the passes run on a
 // packed copy of h (padded to 64 / 128 / 256 columns), so an ignored position costs nothing.
@@ -239,20 +239,61 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
         for (int t = 0; t < NX; ++t) S[1][t] = CeT<T>::mm(f1, xf[t][s], S[1][t]);
       }
       if constexpr (FWD) {
-        if (tail) {
+        float base[NX];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c * CE_CH + at + 16 * (i >> 2) + (i & 3) >= ny)
-#pragma unroll
-              for (int t = 0; t < NX; ++t) S[i >> 2][t][i & 3] = -__builtin_inff();
-        }
-        if (mine) {
+        for (int t = 0; t < NX; ++t) base[t] = ce_base<T>(ref[t]);
+        // the reference moves up to the logits in hand, what was summed follows, and the powers are made from differences
+        auto move = [&]() __attribute__((always_inline)) {
+          bool up = false, beyond = false;
+          float now[NX];
 #pragma unroll
           for (int t = 0; t < NX; ++t) {
-            const int place = target[wave * 16 * NX + 16 * t + n] - c * CE_CH - at;
+            float m = fmaxf(fmaxf(fmaxf(S[0][t][0], S[0][t][1]), fmaxf(S[0][t][2], S[0][t][3])),
+                            fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            now[t] = fmaxf(ref[t], m);
+            up |= now[t] != ref[t];
+            beyond |= !ce_near(now[t]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) S[j][t][i] -= now[t];
+            base[t] = CeT<T>::OFF;
+          }
+          if (__any(up)) {
+#pragma unroll
+            for (int t = 0; t < NX; ++t) {
+              const float fac = ce_weight<T>(ref[t], now[t]);
+              ref[t] = now[t];
+              sum[t] *= fac;
+#pragma unroll
+              for (int f = 0; f < FB; ++f) O[f][t] *= fac;
+            }
+          }
+          away = __any(beyond);
+        };
+        bool fresh = false;
+        if (tail || mine || away) {
+          if (tail) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (place == 16 * (i >> 2) + (i & 3)) S[i >> 2][t][i & 3] = -__builtin_inff();
+              if (c * CE_CH + at + 16 * (i >> 2) + (i & 3) >= ny)
+#pragma unroll
+                for (int t = 0; t < NX; ++t) S[i >> 2][t][i & 3] = -__builtin_inff();
+          }
+          if (mine) {
+#pragma unroll
+            for (int t = 0; t < NX; ++t) {
+              const int place = target[wave * 16 * NX + 16 * t + n] - c * CE_CH - at;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (place == 16 * (i >> 2) + (i & 3)) S[i >> 2][t][i & 3] = -__builtin_inff();
+            }
+          }
+          if (away) {
+            move();
+            fresh = true;
           }
         }
         float p[NX][8], add[NX];
@@ -260,38 +301,16 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 4 : 2) void k_ce_pass(CeArgs a)
           bool up = false;
 #pragma unroll
           for (int t = 0; t < NX; ++t) {
-            if (away) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3] - ref[t], CE_L2E, CeT<T>::OFF));
-            } else {
-              const float b = ce_base<T>(ref[t]);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, b));
-            }
+            for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i >> 2][t][i & 3], CE_L2E, base[t]));
             add[t] = ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
             up |= !(add[t] <= CeT<T>::LIM);
           }
           return up;
         };
-        if (__any(powers())) {   // rare after a split's first chunk: the reference moves, what was summed follows
-#pragma unroll
-          for (int t = 0; t < NX; ++t) {
-            float m = fmaxf(fmaxf(fmaxf(S[0][t][0], S[0][t][1]), fmaxf(S[0][t][2], S[0][t][3])),
-                            fmaxf(fmaxf(S[1][t][0], S[1][t][1]), fmaxf(S[1][t][2], S[1][t][3])));
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float now = fmaxf(ref[t], m), fac = ce_weight<T>(ref[t], now);
-            ref[t] = now;
-            sum[t] *= fac;
-#pragma unroll
-            for (int f = 0; f < FB; ++f) O[f][t] *= fac;
-          }
-          bool beyond = false;
-#pragma unroll
-          for (int t = 0; t < NX; ++t) beyond |= !ce_near(ref[t]);
-          away = __any(beyond);
-          powers();   // no power is above 2^OFF by more than ce_base's rounding now
+        if (__any(powers()) && !fresh) {   // rare: no power is above 2^OFF afterwards
+          move();
+          powers();
         }
 #pragma unroll
         for (int t = 0; t < NX; ++t) {
