@@ -30,8 +30,8 @@
 // rows of Y a wave reads 2·32·D values from LDS for 4·16·NX·32·D MFMA flops.
 //
 // Measured, whole step: 4096 rows x 1M items x 128 bf16 3.47 to 3.53 ms, 1190 to 1210 TFLOP/s of these 8 N V D (88 to 90 % of
-// what a large library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.18
-// to 1.19 ms, 1060 to 1070 TFLOP/s, and 1.25 ms where the rows' weights differ: half of these targets are among 256 items, whose
+// what a large library product reaches, with the exponentials beside it); 7867 of 13111 rows x 78341 items x 256 fp16 1.17
+// to 1.19 ms, 1060 to 1080 TFLOP/s, and 1.25 ms where the rows' weights differ: half of these targets are among 256 items, whose
 // shares one workgroup adds (row by row, by one wave each: 4.4 ms); 64 x 10001 x 32 32 to 36 us, of which the launches and the
 // waits between its five kernels (3 to 8 us each) are most.
 //
